@@ -1,0 +1,332 @@
+"""The serving operators that are measured: attention of new tokens over a paged KV cache, copies of cache pages, and
+the choice of the next token.
+
+``run`` computes each in plain torch operations, or, where ``own`` is true, through ``paddle2_amd.serving``:
+
+* ``chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table)`` - the packed new tokens of a ragged
+  batch attend to everything their sequence holds in the cache up to and including themselves;
+* ``copy_kv_blocks(k_caches, v_caches, src, dst)`` - page ``src[i]`` of every layer's K and V pool is copied to page
+  ``dst[i]`` (forked sequences, reordered beams, compaction);
+* ``sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)`` - one token per row from a given random number.
+"""
+import math
+import random
+
+import numpy as np
+import torch
+
+own = False
+
+_DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def listed():
+    return [
+        # a few drafted tokens per sequence are checked against a short context
+        dict(name="attn_draft_check", op="attention", batch=8, new=4, ragged_new=False, context=700, lengths=1, heads=32,
+             kv_heads=32, dim=128, block=64, dtype="bf16"),
+        # the first chunk of a prompt: nothing is in the cache before it
+        dict(name="attn_first_chunk", op="attention", batch=1, new=2048, ragged_new=False, context=0, lengths=2, heads=32,
+             kv_heads=32, dim=128, block=64, dtype="bf16"),
+        # a later chunk of a long prompt, grouped heads
+        dict(name="attn_long_prompt", op="attention", batch=1, new=2048, ragged_new=False, context=30720, lengths=3,
+             heads=32, kv_heads=8, dim=128, block=64, dtype="bf16"),
+        # a step that mixes decoding sequences with pieces of prompts, odd lengths everywhere
+        dict(name="attn_mixed_step", op="attention", batch=45, new=301, ragged_new=True, context=2500, lengths=4, heads=16,
+             kv_heads=4, dim=64, block=16, dtype="fp16"),
+        # single tokens of many sequences over long caches
+        dict(name="attn_single_tokens", op="attention", batch=64, new=1, ragged_new=False, context=8000, lengths=5,
+             heads=32, kv_heads=8, dim=128, block=64, dtype="bf16"),
+        # one stream, nucleus sampling
+        dict(name="sample_one_stream", op="sample", rows=1, vocab=32000, dtype="bf16", settings="top_p", banned=False),
+        # a served batch with top-k and top-p, odd vocabulary in 32 bits
+        dict(name="sample_batch_odd", op="sample", rows=32, vocab=50257, dtype="fp32", settings="top_k_top_p",
+             banned=False),
+        # warm text: a floor on the probability relative to the best token
+        dict(name="sample_min_p", op="sample", rows=64, vocab=32000, dtype="fp16", settings="min_p", banned=True),
+        # the largest: every row has settings of its own
+        dict(name="sample_own_settings", op="sample", rows=256, vocab=131072, dtype="bf16", settings="each",
+             banned=True),
+        # one sequence is forked: its last, partly filled page is copied in every layer
+        dict(name="pages_fork", op="pages", layers=32, block=64, kv_heads=32, dim=128, dtype="bf16", pool=64, pairs=1,
+             sources=1),
+        # beams are reordered: each kept beam's last page goes to several
+        dict(name="pages_beams", op="pages", layers=24, block=16, kv_heads=40, dim=128, dtype="fp16", pool=257, pairs=61,
+             sources=17),
+        # a pool is compacted: pages move to the free places in front
+        dict(name="pages_compact", op="pages", layers=32, block=64, kv_heads=8, dim=128, dtype="bf16", pool=1024,
+             pairs=500, sources=500),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(["attention", "attention", "sample", "pages"])
+    if op == "attention":
+        heads, kv = rng.choice([(32, 32), (32, 8), (16, 4), (8, 1), (40, 40), (12, 4), (14, 2)])
+        dim = rng.choice([64, 128])
+        form = rng.choice(["single", "few", "chunk", "mixed"])
+        batch = _log(rng, 1, 64)
+        if form == "single":
+            new, context = 1, _log(rng, 1, 16000)
+        elif form == "few":
+            new, context = rng.randint(2, 16), _log(rng, 1, 16000)
+        elif form == "chunk":
+            batch, new, context = rng.randint(1, 4), _log(rng, 100, 2500), _log(rng, 1, 16000)
+        else:
+            new, context = _log(rng, 20, 700), _log(rng, 50, 6000)
+        while batch > 1 and batch * new * (context + new) * heads * dim > 1e11:
+            batch //= 2
+        return dict(op="attention", batch=batch, new=new, ragged_new=form == "mixed", context=context,
+                    lengths=rng.randrange(1 << 30), heads=heads, kv_heads=kv, dim=dim,
+                    block=rng.choice([16, 32, 64, 128]), dtype=rng.choice(["bf16", "fp16"]))
+    if op == "sample":
+        return dict(op="sample", rows=_log(rng, 1, 256), vocab=_log(rng, 1000, 131000),
+                    dtype=rng.choice(["bf16", "fp16", "fp32"]),
+                    settings=rng.choice(["plain", "greedy", "top_k", "top_p", "top_k_top_p", "min_p", "each"]),
+                    banned=rng.random() < 0.5)
+    layers = rng.randint(2, 32)
+    block, kv, dim = rng.choice([16, 32, 64, 128]), rng.choice([1, 2, 4, 8, 32]), rng.choice([64, 128])
+    pairs = _log(rng, 1, 400)
+    while pairs > 1 and pairs * layers * block * kv * dim > 1e9:
+        pairs //= 2
+    return dict(op="pages", layers=layers, block=block, kv_heads=kv, dim=dim, dtype=rng.choice(["bf16", "fp16"]),
+                pool=2 * pairs + rng.randint(1, 40), pairs=pairs, sources=rng.randint(1, pairs))
+
+
+def _lengths(case):
+    """The new tokens and the tokens held before them, for each sequence: what the batch is, not its values."""
+    rng = random.Random(case["lengths"])
+    new, held = [], []
+    for _ in range(case["batch"]):
+        if case["ragged_new"]:   # two of three sequences decode, the others bring a piece of a prompt
+            new.append(1 if rng.random() < 0.67 else rng.randint(2, case["new"]))
+        else:
+            new.append(case["new"])
+        c = case["context"]
+        held.append(c if case["batch"] == 1 else rng.randint(c // 2, c))
+    return new, held
+
+
+def _pairs(case):
+    """Sources (some several times where there are fewer of them than pairs) and places, apart from each other."""
+    rng = random.Random(case["pairs"] * 1009 + case["pool"])
+    pages = rng.sample(range(case["pool"]), case["sources"] + case["pairs"])
+    src = pages[:case["sources"]]
+    src = src + [rng.choice(src) for _ in range(case["pairs"] - case["sources"])]
+    return src, pages[case["sources"]:]
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    dt = _DT[case["dtype"]]
+
+    def normal(*shape, dtype=dt):
+        return torch.empty(shape, dtype=dtype, device="cuda").normal_(generator=g)
+
+    if case["op"] == "attention":
+        new, held = _lengths(case)
+        bs = case["block"]
+        need = [(n + h + bs - 1) // bs for n, h in zip(new, held)]
+        pool = sum(need) + 3
+        order = torch.randperm(pool, generator=g, device="cuda").to(torch.int32)
+        table = torch.zeros(len(new), max(need), dtype=torch.int32, device="cuda")
+        at = 0
+        for b, k in enumerate(need):
+            table[b, :k] = order[at:at + k]
+            at += k
+        cu = [0]
+        for n in new:
+            cu.append(cu[-1] + n)
+        return dict(op="attention", new=new, held=held, scale=1.0 / math.sqrt(case["dim"]),
+                    q=normal(cu[-1], case["heads"], case["dim"]),
+                    k=normal(pool, bs, case["kv_heads"], case["dim"]), v=normal(pool, bs, case["kv_heads"], case["dim"]),
+                    cu=torch.tensor(cu, dtype=torch.int32, device="cuda"),
+                    lens=torch.tensor([n + h for n, h in zip(new, held)], dtype=torch.int32, device="cuda"), table=table)
+    if case["op"] == "sample":
+        B, V = case["rows"], case["vocab"]
+        # a broad floor of unlikely tokens, some rows flat and some sharp, and a few tokens that stand out
+        sharp = torch.empty(B, 1, device="cuda").uniform_(0.7, 2.5, generator=g)
+        x = normal(B, V, dtype=torch.float32) * sharp
+        few = torch.randint(0, V, (B, 24), generator=g, device="cuda")
+        x.scatter_(1, few, normal(B, 24, dtype=torch.float32) * 2.5 + 3.5 * sharp)
+        if case["banned"]:   # tokens that the caller does not allow
+            x.masked_fill_(torch.rand(B, V, generator=g, device="cuda") < 0.1, float("-inf"))
+        u = torch.rand(B, generator=g, device="cuda")
+        how = case["settings"]
+        t, k, p, m = 1.0, 0, 1.0, 0.0
+        if how == "greedy":
+            t = 0.0
+        elif how == "top_k":
+            t, k = 0.7, 40
+        elif how == "top_p":
+            t, p = 0.8, 0.95
+        elif how == "top_k_top_p":
+            t, k, p = 0.9, 50, 0.9
+        elif how == "min_p":
+            t, m = 1.5, 0.05
+        elif how == "each":
+            t = torch.empty(B, device="cuda").uniform_(0.3, 1.6, generator=g)
+            t[torch.rand(B, generator=g, device="cuda") < 0.1] = 0.0
+            k = torch.randint(0, 200, (B,), generator=g, device="cuda").to(torch.int32)
+            k[torch.rand(B, generator=g, device="cuda") < 0.5] = 0
+            p = torch.empty(B, device="cuda").uniform_(0.5, 1.0, generator=g)
+            m = torch.empty(B, device="cuda").uniform_(0.0, 0.1, generator=g)
+            m[torch.rand(B, generator=g, device="cuda") < 0.5] = 0.0
+        return dict(op="sample", logits=x.to(dt), uniform=u, temperature=t, top_k=k, top_p=p, min_p=m)
+    src, dst = _pairs(case)
+    shape = (case["pool"], case["block"], case["kv_heads"], case["dim"])
+    return dict(op="pages", k=[normal(*shape) for _ in range(case["layers"])],
+                v=[normal(*shape) for _ in range(case["layers"])], src=src, dst=dst)
+
+
+def _attention(s):
+    """Softmax over each row's visible keys in 32 bits, sequence by sequence and kv head by kv head."""
+    q, out, at = s["q"], torch.empty_like(s["q"]), 0
+    bs, kv, dim = s["k"].shape[1:]
+    group = q.shape[1] // kv
+    for b, (n, held) in enumerate(zip(s["new"], s["held"])):
+        pages = s["table"][b, :(n + held + bs - 1) // bs].long()
+        keys = s["k"][pages].reshape(-1, kv, dim)[:n + held].float()
+        vals = s["v"][pages].reshape(-1, kv, dim)[:n + held].float()
+        hidden = (torch.arange(n + held, device=q.device)[None] > held + torch.arange(n, device=q.device)[:, None])
+        for h in range(kv):
+            rows = q[at:at + n, h * group:(h + 1) * group].float().transpose(0, 1)       # [group, n, dim]
+            sc = torch.matmul(rows * s["scale"], keys[:, h].t().contiguous())
+            sc = sc.masked_fill_(hidden, float("-inf"))
+            p = sc.sub_(sc.amax(-1, keepdim=True)).exp_()
+            o = torch.matmul(p, vals[:, h].contiguous()) / p.sum(-1, keepdim=True)
+            out[at:at + n, h * group:(h + 1) * group] = o.transpose(0, 1).to(out.dtype)
+        at += n
+    return out
+
+
+def _column(v, like, dtype):
+    """A setting as a [rows, 1] column of 64-bit values (settings are numbers of 32 bits)."""
+    t = v if torch.is_tensor(v) else torch.full((like.shape[0],), v, dtype=dtype, device=like.device)
+    return t.to(dtype).double()[:, None]
+
+
+def _sample(s):
+    """Sort, keep, and invert the cumulative sum in index order; 64 bits, since a choice next to a border turns on them."""
+    x = s["logits"].double()
+    V = x.shape[1]
+    t, k = _column(s["temperature"], x, torch.float32), _column(s["top_k"], x, torch.int32)
+    p, m = _column(s["top_p"], x, torch.float32), _column(s["min_p"], x, torch.float32)
+    top = x.amax(1, keepdim=True)
+    w = ((x - top) / torch.where(t > 0, t, 1.0)).exp()
+    sx, order = torch.sort(x, dim=1, descending=True, stable=True)      # ties: the lowest index first
+    sw = w.gather(1, order)
+    rank = torch.arange(V, device=x.device)[None]
+    sw = torch.where((k > 0) & (rank >= k), 0.0, sw)
+    before = sw.cumsum(1) - sw
+    keep = (before < p * sw.sum(1, keepdim=True)) | (p >= 1.0) | (rank == 0)
+    sw = torch.where(keep & (sw >= m), sw, 0.0)
+    w = torch.zeros_like(w).scatter_(1, order, sw)
+    c = w.cumsum(1)
+    token = (c <= s["uniform"].double()[:, None] * c[:, -1:]).sum(1).clamp_(max=V - 1)
+    return torch.where(t[:, 0] > 0, token, x.argmax(1))
+
+
+def _pages(s):
+    src = torch.tensor(s["src"], device="cuda")
+    dst = torch.tensor(s["dst"], device="cuda")
+    for pool in s["k"] + s["v"]:
+        pool[dst] = pool[src]
+    return s["k"] + s["v"]
+
+
+def run(state):
+    if not own:
+        return {"attention": _attention, "sample": _sample, "pages": _pages}[state["op"]](state)
+    from paddle2_amd import serving
+
+    if state["op"] == "attention":
+        return serving.chunk_attention(state["q"], state["k"], state["v"], state["cu"], state["lens"], state["table"])
+    if state["op"] == "sample":
+        return serving.sample_tokens(state["logits"], state["uniform"], state["temperature"], state["top_k"],
+                                     state["top_p"], state["min_p"])
+    serving.copy_kv_blocks(state["k"], state["v"], state["src"], state["dst"])
+    return state["k"] + state["v"]
+
+
+def work(case):
+    if case["op"] == "attention":
+        new, held = _lengths(case)
+        seen = sum(n * h + n * (n + 1) // 2 for n, h in zip(new, held))
+        tokens, keys = sum(new), sum(new) + sum(held)
+        return {"bytes": 2 * case["dim"] * (2 * tokens * case["heads"] + 2 * keys * case["kv_heads"]),
+                "flops": 4 * case["dim"] * case["heads"] * seen}
+    if case["op"] == "sample":
+        n = case["rows"] * case["vocab"]
+        return {"bytes": n * (4 if case["dtype"] == "fp32" else 2) + 12 * case["rows"], "flops": 2 * n}
+    page = 2 * case["block"] * case["kv_heads"] * case["dim"]
+    return {"bytes": 2 * case["layers"] * page * (case["sources"] + case["pairs"]), "flops": 0}
+
+
+def _exact_attention(s):
+    """The definition in 64 bits: a weighted mean of values with the weights exp(q . k - log-sum-exp), rows in pieces."""
+    out = torch.empty(s["q"].shape, dtype=torch.float64, device="cuda")
+    bs, kv = s["k"].shape[1:3]
+    group, start = s["q"].shape[1] // kv, 0
+    for b, n in enumerate(s["new"]):
+        total = int(s["lens"][b])
+        j = torch.arange(total, device="cuda")
+        page, row = s["table"][b].long()[torch.div(j, bs, rounding_mode="floor")], j % bs
+        for head in range(s["q"].shape[1]):
+            K = s["k"][page, row, head // group].double()
+            V = s["v"][page, row, head // group].double()
+            for lo in range(0, n, 1024):
+                hi = min(n, lo + 1024)
+                pos = total - n + torch.arange(lo, hi, device="cuda")
+                z = s["q"][start + lo:start + hi, head].double() @ K.t() * s["scale"]
+                z = torch.where(j[None, :] <= pos[:, None], z, -math.inf)
+                out[start + lo:start + hi, head] = torch.exp(z - torch.logsumexp(z, 1, keepdim=True)) @ V
+        start += n
+    return out
+
+
+def _exact_sample(s):
+    """Row by row on the host: candidates in order of (value, index), kept while the definition keeps them."""
+    x = s["logits"].double().cpu().numpy()
+    u = s["uniform"].double().cpu().numpy()
+
+    def each(v, dtype):
+        if torch.is_tensor(v):
+            return v.cpu().numpy().astype(dtype)
+        return np.full(len(x), v, dtype=dtype)
+
+    t, k = each(s["temperature"], np.float32), each(s["top_k"], np.int32)
+    p, m = each(s["top_p"], np.float32), each(s["min_p"], np.float32)
+    tokens = []
+    for row, ui, ti, ki, pi, mi in zip(x, u, t, k, p, m):
+        if ti == 0:
+            tokens.append(int(np.argmax(row)))
+            continue
+        w = np.exp((row - row.max()) / np.float64(ti))
+        ranked = np.lexsort((np.arange(len(row)), -row))
+        if ki > 0:
+            ranked = ranked[:ki]
+        if pi < 1:
+            mass = np.cumsum(w[ranked])
+            ranked = ranked[:1 + int(np.searchsorted(mass, np.float64(pi) * mass[-1], side="left"))]
+        kept = np.sort(ranked[w[ranked] >= np.float64(mi)])
+        mass = np.cumsum(w[kept])
+        tokens.append(int(kept[min(len(kept) - 1, int(np.searchsorted(mass, ui * mass[-1], side="right")))]))
+    return torch.tensor(tokens, device="cuda")
+
+
+def _exact_pages(s):
+    """Bytes are moved, nothing is computed: page by page."""
+    for pool in s["k"] + s["v"]:
+        for a, b in zip(s["src"], s["dst"]):
+            pool[b].copy_(pool[a])
+    return s["k"] + s["v"]
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"attention": _exact_attention, "sample": _exact_sample, "pages": _exact_pages}[case["op"]](s)
