@@ -67,8 +67,9 @@ def _run(cmd):
 def build(verbose=False, jobs=None):
     os.makedirs(BUILD, exist_ok=True)
     hips, binding = _sources()
+    # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): some of its forms have given wrong results on this part
     hip_flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-munsafe-fp-atomics",
-                 "-I", os.path.join(CSRC, "kernels")]
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-I", os.path.join(CSRC, "kernels")]
     import pybind11
 
     py_inc = sysconfig.get_paths()["include"]
