@@ -74,6 +74,13 @@ int pd_decode_attn(const void*, long, long, const void*, const void*, long, long
                    const int*, int, float*, float*, void*, long, long, int, int, int, int, int, float, int, void*);
 int pd_cache_write(const void*, const void*, long, long, void*, void*, long, long, long, const int*, int, int,
                    const int*, const int*, int, int, int, void*);
+int pd_chunk_attn_tiles(int, int, int);
+int pd_chunk_attn(int, const void*, long, long, const void*, const void*, long, long, long, const int*, int, int, int,
+                  const int*, const int*, void*, long, long, int, int, int, int, int, int, int, float, float*, float*,
+                  void*);
+int pd_kv_copy(const uint64_t*, int, const int*, const int*, int, long, long, void*);
+int pd_sample(int, const void*, long, int, int, const float*, const float*, float, const int*, int, const float*, float,
+              const float*, float, int64_t*, void*);
 long pd_bn_workspace(int, long, int);
 int pd_wo_splits(int, int, int, int);
 int pd_dec_splits(int, int, int);
@@ -117,6 +124,20 @@ static inline T P(uintptr_t v) {
 
 static void check(int rc, const char* what) {
   if (rc != 0) throw std::runtime_error(std::string("paddle2_amd._C.") + what + " failed with code " + std::to_string(rc));
+}
+
+static void check_pages(const std::vector<long>& src, const std::vector<long>& dst, long num_blocks) {
+  if (src.size() != dst.size()) throw std::invalid_argument("src and dst differ in length");
+  std::vector<char> seen(num_blocks > 0 ? num_blocks : 0, 0);
+  for (long b : dst) {
+    if (b < 0 || b >= num_blocks) throw std::invalid_argument("page " + std::to_string(b) + " is not in the pool");
+    if (seen[b]) throw std::invalid_argument("page " + std::to_string(b) + " is a destination twice");
+    seen[b] = 1;
+  }
+  for (long b : src) {
+    if (b < 0 || b >= num_blocks) throw std::invalid_argument("page " + std::to_string(b) + " is not in the pool");
+    if (seen[b]) throw std::invalid_argument("page " + std::to_string(b) + " is both a source and a destination");
+  }
 }
 
 PYBIND11_MODULE(_C, m) {
@@ -345,6 +366,43 @@ PYBIND11_MODULE(_C, m) {
     check(pd_fp8_update_scale(n, hist.data(), len.data(), amax.data(), scale.data(), inv.data(), snap.data(),
                               fmax.data(), mp2.data(), P<void*>(st)),
           "fp8_update_scale");
+  });
+  m.def("chunk_attn_tiles", [](int T, int B, int G) {
+    if (T < 0 || B < 0 || G < 1 || G > 128) throw std::invalid_argument("chunk_attn_tiles: bad sizes");
+    return pd_chunk_attn_tiles(T, B, G);
+  });
+  m.def("chunk_attn", [](int f16, uintptr_t q, long sq_tok, long sq_head, uintptr_t k, uintptr_t v, long s_blk,
+                         long s_tok, long s_head, uintptr_t table, int max_blocks, int num_blocks, int block,
+                         uintptr_t cu, uintptr_t lens, uintptr_t out, long so_tok, long so_head, int B, int T, int Hq,
+                         int Hk, int D, int splits, int min_keys, float scale, uintptr_t part_o, uintptr_t part_ml,
+                         uintptr_t st) {
+    check(pd_chunk_attn(f16, P<const void*>(q), sq_tok, sq_head, P<const void*>(k), P<const void*>(v), s_blk, s_tok,
+                        s_head, P<const int*>(table), max_blocks, num_blocks, block, P<const int*>(cu),
+                        P<const int*>(lens), P<void*>(out), so_tok, so_head, B, T, Hq, Hk, D, splits, min_keys, scale,
+                        P<float*>(part_o), P<float*>(part_ml), P<void*>(st)),
+          "chunk_attn");
+  });
+  // src / dst: page numbers; every page inside the pool, no destination twice, none also a source (std::invalid_argument
+  // -> ValueError)
+  m.def("kv_copy_check", [](const std::vector<long>& src, const std::vector<long>& dst, long num_blocks) {
+    check_pages(src, dst, num_blocks);
+  });
+  m.def("kv_copy", [](const std::vector<uintptr_t>& pool, const std::vector<long>& src, const std::vector<long>& dst,
+                      long num_blocks, long page_bytes, long page_stride, uintptr_t st) {
+    check_pages(src, dst, num_blocks);
+    const std::vector<uint64_t> pools(pool.begin(), pool.end());
+    const std::vector<int> s(src.begin(), src.end()), d(dst.begin(), dst.end());
+    check(pd_kv_copy(pools.data(), (int)pools.size(), s.data(), d.data(), (int)s.size(), page_bytes, page_stride,
+                     P<void*>(st)),
+          "kv_copy");
+  });
+  m.def("sample", [](int dt, uintptr_t logits, long stride, int B, int V, uintptr_t uniform, uintptr_t temps, float temp,
+                     uintptr_t top_ks, int top_k, uintptr_t top_ps, float top_p, uintptr_t min_ps, float min_p,
+                     uintptr_t out, uintptr_t st) {
+    check(pd_sample(dt, P<const void*>(logits), stride, B, V, P<const float*>(uniform), P<const float*>(temps), temp,
+                    P<const int*>(top_ks), top_k, P<const float*>(top_ps), top_p, P<const float*>(min_ps), min_p,
+                    P<int64_t*>(out), P<void*>(st)),
+          "sample");
   });
   m.def("decode_attn", [](uintptr_t q, long sq_b, long sq_h, uintptr_t kc, uintptr_t vc, long s_blk, long s_tok,
                           long s_head, uintptr_t table, int max_blocks, int block_size, uintptr_t seq_lens, int max_len,

@@ -1,0 +1,496 @@
+// Attention of a chunk of new tokens over a paged KV cache (chunked prefill, drafted tokens, mixed steps).
+//
+// Packed queries q[cu[b] .. cu[b+1]) are the last n_b of the len_b tokens that sequence b holds in the cache (their
+// own K / V rows are there already); query i of them, at position p = len_b - n_b + i, sees the keys 0 .. p:
+//   o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),   s_j = scale * q . k_j
+// Token t of sequence b lives at page(b, t) * s_blk + (t % block) * s_tok + kv_head * s_head, in 64 bits.
+//
+//  * A workgroup (4 waves) owns 128 rows of one (sequence, kv head): rows are (token, query head of the group), so a
+//    K / V tile read once serves the whole group.  Its sequence is found from cu by a prefix sum over the lanes: the
+//    host never reads lengths, and the launch is the same for every batch of a shape (it can be captured).
+//  * S^T = K . Q^T on 32x32x16 MFMA: a lane owns one row's scores, the softmax needs one exchange between lane
+//    halves, and the bf16 / fp16 P is the next product's operand as it stands.  P is rounded to 16 bits because the
+//    matrix unit takes 16-bit operands; each P is off by half a step of a value <= 2^8 relative to the row's sum,
+//    which averages out below the rounding of the output.  Scores, maxima, sums and O stay in 32 bits.
+//  * 64-key tiles go global -> registers -> LDS, two stages, page numbers one tile further ahead.  Keys past the
+//    rows' reach and pages outside the pool are read from a block of zeros, so stale pages (NaN among them) never
+//    reach a product.
+//  * A hidden key has P = 0, but 0 * inf is NaN: where a tile on the diagonal holds a value that is not finite, its
+//    product runs on the finite values, and infinities and NaN are added to the rows that see them (counted by two
+//    products with a 0 / 1 visibility operand).
+//  * Few rows over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
+//    second kernel.  How often is decided per tile, from its own length.
+#include "common.h"
+
+namespace pd {
+namespace ca {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kDefer = 8.f;   // the running maximum moves only when a row outgrows it by 2^8
+constexpr int kBM = 128, kBN = 64;
+
+__device__ const u16x8 kZeros = {0, 0, 0, 0, 0, 0, 0, 0};
+
+struct Args {
+  const unsigned short *q, *k, *v;
+  unsigned short* out;
+  long sq_tok, sq_head, so_tok, so_head;   // in elements
+  long s_blk, s_tok, s_head;
+  const int *cu, *lens, *table;
+  int B, T, Hq, Hk, G;
+  int max_blocks, num_blocks, block, block_shift;   // block_shift < 0: block is no power of two
+  int tiles, splits, min_keys;                      // tiles: upper bound over the batch
+  float scale_log2;
+  float *part_o, *part_ml;                          // [splits][T][Hq][D], [splits][T][Hq][2]
+};
+
+struct Seq {
+  int b, q0, n, len, tile;   // first query row, new tokens, keys, tile within the sequence (-1: none)
+};
+
+__device__ __forceinline__ void bounds_of(const Args& a, int b, int& q0, int& n) {
+  q0 = min(max(a.cu[b], 0), a.T);
+  n = max(min(a.cu[b + 1], a.T) - q0, 0);
+}
+__device__ __forceinline__ int len_of(const Args& a, int b) {
+  return (int)min((long)max(a.lens[b], 0), (long)a.max_blocks * a.block);
+}
+
+// the sequence that holds tile `tile` of the batch; every wave computes it for itself
+__device__ __forceinline__ Seq find_tile(const Args& a, int tile, int tile_tokens, int lane) {
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    int q0 = 0, n = 0;
+    if (b0 + lane < a.B) bounds_of(a, b0 + lane, q0, n);
+    const int mine = (n + tile_tokens - 1) / tile_tokens;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += t;
+    }
+    const unsigned long long hit = __ballot(base + incl > tile);
+    if (hit) {
+      const int l = __ffsll((long long)hit) - 1;
+      Seq s;
+      s.b = __builtin_amdgcn_readfirstlane(b0 + l);
+      s.q0 = __builtin_amdgcn_readfirstlane(__shfl(q0, l, 64));
+      s.n = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+      // the tile that sees the most keys first
+      const int in_seq = __shfl(mine, l, 64) - 1 - (tile - (base + __shfl(incl - mine, l, 64)));
+      s.tile = __builtin_amdgcn_readfirstlane(in_seq);
+      s.len = len_of(a, s.b);
+      return s;
+    }
+    base += __shfl(incl, 63, 64);
+  }
+  return Seq{0, 0, 0, 0, -1};
+}
+
+// keys per piece of a tile that sees `keys` keys: whole 64-key tiles, at least min_keys, at most `splits` pieces
+__device__ __forceinline__ int piece_of(const Args& a, int keys) {
+  const int pieces = max(1, min(a.splits, (keys + a.min_keys - 1) / a.min_keys));
+  const int per = (keys + pieces - 1) / pieces;
+  return max((per + kBN - 1) / kBN * kBN, kBN);
+}
+
+template <int D>
+__device__ __forceinline__ int swz(int row, int ch) {
+  return ch ^ ((((row & 3) << 2) | ((row >> 2) & 3)) & (D / 8 - 1));
+}
+__device__ __forceinline__ s16x4 lds_tr(const char* base, int off) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)((lds_char*)base + off));
+}
+template <bool F16>
+__device__ __forceinline__ unsigned short cvt16(float f) {
+  if constexpr (F16) return f2h(f);
+  else return f2bf(f);
+}
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+template <bool F16>
+__device__ __forceinline__ bf16x8 pack8(const f32x16& acc, int s) {
+  if constexpr (F16) {
+    f16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (_Float16)acc[8 * s + j];
+    return __builtin_bit_cast(bf16x8, r);
+  } else {
+    bf16x8 r;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r[j] = (__bf16)acc[8 * s + j];
+    return r;
+  }
+}
+__device__ __forceinline__ int xcd_remap(int bid, int n) {
+  const int q = n / 8, r = n % 8, xcd = bid % 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void chunk_kernel(Args a) {
+  constexpr int NCH = D / 8, KS = D / 16, DT = D / 32, TILE = kBN * D * 2;
+  constexpr int NLOAD = kBN * NCH / 256, ROWS = 256 / NCH;   // loads per thread and tile; rows between them
+  __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
+  __shared__ int odd_tile[2];   // per stage: the first key of the last tile staged with a value that is not finite
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 31, h = lane >> 5;
+  const int tile_tokens = kBM / a.G;
+
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int sp = id % a.splits, tile = (id / a.splits) % a.tiles, hk = id / (a.splits * a.tiles);
+  const Seq s = find_tile(a, tile, tile_tokens, lane);
+  if (s.tile < 0) return;
+  const int tok0 = s.tile * tile_tokens;                        // first token of the tile within the sequence
+  const int ntok = min(tile_tokens, s.n - tok0);
+  const int pos0 = s.len - s.n + tok0;                          // its position (negative: it sees nothing)
+  const int keys = max(pos0 + ntok, 0);                         // keys the tile's last token sees
+  const int piece = piece_of(a, keys);
+  const int k0 = sp * piece, k1 = min(keys, k0 + piece);
+  const bool whole = piece >= keys;
+  if (sp > 0 && k0 >= keys) return;
+
+  const int row = wv * 32 + r;                                  // this lane's row: token row / G, head row % G
+  const int rt = row / a.G, rh = hk * a.G + row % a.G;
+  const bool live = rt < ntok;
+  const int pos = pos0 + rt;
+
+  bf16x8 qf[KS];
+  {
+    const unsigned short* qp = a.q + (long)(s.q0 + tok0 + (live ? rt : 0)) * a.sq_tok + (long)(live ? rh : 0) * a.sq_head + 8 * h;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      qf[ks] = *reinterpret_cast<const bf16x8*>(qp + ks * 16);
+      if (!live) qf[ks] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+
+  // page numbers, then rows, of the tile's 64 keys; a thread loads chunk tid % NCH of rows tid / NCH + ROWS * i
+  const int lrow = tid / NCH, lch = tid % NCH;
+  const int* tab = a.table + (long)s.b * a.max_blocks;
+  const long head_off = (long)hk * a.s_head + lch * 8;
+  auto block_of = [&](int key) { return a.block_shift >= 0 ? key >> a.block_shift : key / a.block; };
+  int pid[NLOAD];
+  auto pages = [&](int n0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) pid[i] = tab[block_of(min(n0 + lrow + ROWS * i, k1 - 1))];
+  };
+  u16x8 stk[NLOAD], stv[NLOAD];
+  auto gload = [&](int n0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) {
+      const int key = n0 + lrow + ROWS * i;
+      const bool ok = key < k1 && (unsigned)pid[i] < (unsigned)a.num_blocks;
+      const int in_page = a.block_shift >= 0 ? key & (a.block - 1) : key % a.block;
+      const long off = (long)pid[i] * a.s_blk + (long)in_page * a.s_tok + head_off;
+      const u16x8* pk = ok ? reinterpret_cast<const u16x8*>(a.k + off) : &kZeros;
+      const u16x8* pv = ok ? reinterpret_cast<const u16x8*>(a.v + off) : &kZeros;
+      stk[i] = *pk;
+      stv[i] = *pv;
+    }
+  };
+  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;   // exponent bits: all set in infinities and NaN
+  auto lstore = [&](int buf, int n0) {
+    char* kt = smem + buf * 2 * TILE;
+    if (n0 + kBN - 1 > pos0) {   // a tile with hidden keys
+      bool odd = false;
+#pragma unroll
+      for (int i = 0; i < NLOAD; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) odd |= (stv[i][j] & kExp) == kExp;
+      if (odd) odd_tile[buf] = n0;
+    }
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) {
+      const int rr = lrow + ROWS * i, o = rr * (D * 2) + swz<D>(rr, lch) * 16;
+      *reinterpret_cast<u16x8*>(kt + o) = stk[i];
+      *reinterpret_cast<u16x8*>(kt + TILE + o) = stv[i];
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16{};
+  float m = -INFINITY, l = 0.f;
+  const float sl2 = a.scale_log2;
+  const int wave_rt0 = wv * 32 / a.G, wave_rt1 = min((wv * 32 + 31) / a.G, ntok - 1);
+  const int wave_first = pos0 + wave_rt0;                             // keys up to here are seen by all of its rows
+  const int wave_last = wave_rt0 < ntok ? pos0 + wave_rt1 : -1;       // and none past here by any
+
+  const int ntiles = k1 > k0 ? (k1 - k0 + kBN - 1) / kBN : 0;
+  if (tid < 2) odd_tile[tid] = -1;
+  __syncthreads();
+  if (ntiles > 0) {
+    pages(k0);
+    gload(k0);
+    if (ntiles > 1) pages(k0 + kBN);
+    lstore(0, k0);
+  }
+  __syncthreads();
+  // V^T reads: rows 16 s + 8 (j >> 2) + 4 hh + qq of the tile, 16-byte chunks 4 dt + cbits
+  const int g = lane >> 4, qq = (lane & 15) >> 2, pp = lane & 3, hh = g >> 1, cbits = ((g & 1) << 1) | (pp >> 1);
+
+  for (int t = 0; t < ntiles; ++t) {
+    const int n0 = k0 + t * kBN;
+    const char* kt = smem + (t & 1) * 2 * TILE;
+    const char* vt = kt + TILE;
+    const bool next = t + 1 < ntiles;
+    if (n0 <= wave_last) {
+      f32x16 sc[2];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        sc[kb] = f32x16{};
+        const int kr = kb * 32 + r;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(kt + kr * (D * 2) + swz<D>(kr, 2 * ks + h) * 16), qf[ks], sc[kb]);
+      }
+      if (next) gload(n0 + kBN);
+      if (n0 + kBN > k1 || n0 + kBN - 1 > wave_first) {
+        const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int c = kb * 32 + (i & 3) + 8 * (i >> 2);
+            sc[kb][i] = c >= lim ? -INFINITY : sc[kb][i];
+          }
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[kb][i]);
+      float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      {
+        const unsigned mu = __builtin_bit_cast(unsigned, mt);
+        const auto sw = __builtin_amdgcn_permlane32_swap(mu, mu, false, false);
+        mt = fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1]));
+      }
+      const float mc = fmaxf(m, mt * sl2);
+      if (__builtin_expect(__any(mc > m + kDefer), 0)) {
+        asm volatile("" ::: "memory");
+        const float alpha = __builtin_amdgcn_exp2f(m - (mc == -INFINITY ? 0.f : mc));
+        l *= alpha;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+        m = mc;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], sl2, -base));
+          sc[kb][i] = p;
+          ls[i & 3] += p;
+        }
+      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+      auto v_frag = [&](int kb, int ss, int dt) {
+        const int ra = kb * 32 + 16 * ss + 4 * hh + qq, rb = ra + 8;
+        const s16x4 lo = lds_tr(vt, ra * (D * 2) + swz<D>(ra, 4 * dt + cbits) * 16 + 8 * (pp & 1));
+        const s16x4 hi = lds_tr(vt, rb * (D * 2) + swz<D>(rb, 4 * dt + cbits) * 16 + 8 * (pp & 1));
+        return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      };
+      if (__builtin_expect(n0 + kBN - 1 <= wave_first || odd_tile[t & 1] != n0, 1)) {
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int ss = 0; ss < 2; ++ss) {
+            const bf16x8 pb = pack8<F16>(sc[kb], ss);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, v_frag(kb, ss, dt)), pb, o[dt]);
+          }
+      } else {
+        const int lim = min(k1, pos + 1) - n0 - 4 * h;
+        bf16x8 pb[4], seen[4];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int ss = 0; ss < 2; ++ss) pb[2 * kb + ss] = pack8<F16>(sc[kb], ss);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[kb][i] = kb * 32 + (i & 3) + 8 * (i >> 2) < lim ? 1.f : 0.f;
+#pragma unroll
+          for (int ss = 0; ss < 2; ++ss) seen[2 * kb + ss] = pack8<F16>(sc[kb], ss);
+        }
+        constexpr short kOne = F16 ? 0x3c00 : 0x3f80;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          f32x16 up = f32x16{}, down = f32x16{};   // infinities of each sign seen by a row; NaN counts in both
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const s16x8 vv = v_frag(i >> 1, i & 1, dt);
+            s16x8 fin, pos_inf, neg_inf;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const unsigned short w = (unsigned short)vv[j], mag = w & 0x7fff;
+              fin[j] = mag >= kExp ? (short)0 : vv[j];
+              pos_inf[j] = (mag > kExp || w == kExp) ? kOne : (short)0;
+              neg_inf[j] = (mag > kExp || w == (kExp | 0x8000)) ? kOne : (short)0;
+            }
+            o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, fin), pb[i], o[dt]);
+            up = mfma<F16>(__builtin_bit_cast(bf16x8, pos_inf), seen[i], up);
+            down = mfma<F16>(__builtin_bit_cast(bf16x8, neg_inf), seen[i], down);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            o[dt][i] += up[i] > 0.f ? INFINITY : 0.f;
+            o[dt][i] += down[i] > 0.f ? -INFINITY : 0.f;
+          }
+        }
+      }
+    } else if (next) {
+      gload(n0 + kBN);
+    }
+    if (next) {
+      if (t + 2 < ntiles) pages(n0 + 2 * kBN);
+      lstore((t + 1) & 1, n0 + kBN);
+    }
+    __syncthreads();
+  }
+
+  // lane (row, half h) holds O[row][32 dt + 8 c + 4 h + e] in o[dt][4 c + e]
+  l += __shfl_xor(l, 32, 64);
+  if (whole) {
+    const float inv = l != 0.f ? 1.f / l : 0.f;   // l is 0 only where a row saw no key; a NaN sum stays NaN
+    if (live) {
+      unsigned short* op = a.out + (long)(s.q0 + tok0 + rt) * a.so_tok + (long)rh * a.so_head + 4 * h;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+          u16x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = cvt16<F16>(o[dt][4 * c + e] * inv);
+          *reinterpret_cast<u16x4*>(op + 32 * dt + 8 * c) = w;
+        }
+    }
+  } else if (live) {
+    const long pi = ((long)sp * a.T + s.q0 + tok0 + rt) * a.Hq + rh;
+    float* po = a.part_o + pi * D + 4 * h;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        f32x4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = o[dt][4 * c + e];
+        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * c) = w;
+      }
+    if (h == 0) {
+      a.part_ml[pi * 2] = m;
+      a.part_ml[pi * 2 + 1] = l;
+    }
+  }
+}
+
+// joins the pieces of every row that was split: one workgroup per token, D / 4 lanes per query head
+template <int D, bool F16>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  constexpr int LANES = D / 4, HEADS = 256 / LANES;
+  const int tok = blockIdx.x;
+  // the sequence of this token: the last b with cu[b] <= tok
+  int lo = 0, hi = a.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (a.cu[mid] <= tok) lo = mid;
+    else hi = mid - 1;
+  }
+  int q0, n;
+  bounds_of(a, lo, q0, n);
+  if (tok < q0 || tok >= q0 + n) return;
+  const int tile_tokens = kBM / a.G, tok0 = (tok - q0) / tile_tokens * tile_tokens;
+  const int keys = max(len_of(a, lo) - n + min(tok0 + tile_tokens, n), 0);
+  const int piece = piece_of(a, keys);
+  if (piece >= keys) return;
+  const int pieces = (keys + piece - 1) / piece;
+  const int d = (threadIdx.x % LANES) * 4;
+  for (int hq = threadIdx.x / LANES; hq < a.Hq; hq += HEADS) {
+    float M = -INFINITY;
+    for (int p = 0; p < pieces; ++p) M = fmaxf(M, a.part_ml[(((long)p * a.T + tok) * a.Hq + hq) * 2]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < pieces; ++p) {
+      const long pi = ((long)p * a.T + tok) * a.Hq + hq;
+      const float w = __builtin_amdgcn_exp2f(a.part_ml[pi * 2] - base);
+      L += a.part_ml[pi * 2 + 1] * w;
+      acc += *reinterpret_cast<const f32x4*>(a.part_o + pi * D + d) * w;
+    }
+    const float inv = L != 0.f ? 1.f / L : 0.f;
+    unsigned short* op = a.out + (long)tok * a.so_tok + (long)hq * a.so_head + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) op[e] = cvt16<F16>(acc[e] * inv);
+  }
+}
+
+}  // namespace ca
+}  // namespace pd
+
+using namespace pd;
+
+// upper bound of the batch's row tiles: every sequence may end in a part of one
+extern "C" int pd_chunk_attn_tiles(int T, int B, int G) {
+  const int tt = ca::kBM / G, some = B < T ? B : T;
+  return (int)((T + (long)some * (tt - 1)) / tt);
+}
+
+extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, const void* k, const void* v, long s_blk,
+                             long s_tok, long s_head, const int* table, int max_blocks, int num_blocks, int block,
+                             const int* cu, const int* lens, void* out, long so_tok, long so_head, int B, int T, int Hq,
+                             int Hk, int D, int splits, int min_keys, float scale, float* part_o, float* part_ml,
+                             void* stream) {
+  if (T <= 0 || B <= 0) return 0;
+  if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1) return -1;
+  if (splits > 1 && (!part_o || !part_ml)) return -1;
+  ca::Args a;
+  a.q = (const unsigned short*)q;
+  a.k = (const unsigned short*)k;
+  a.v = (const unsigned short*)v;
+  a.out = (unsigned short*)out;
+  a.sq_tok = sq_tok, a.sq_head = sq_head, a.so_tok = so_tok, a.so_head = so_head;
+  a.s_blk = s_blk, a.s_tok = s_tok, a.s_head = s_head;
+  a.cu = cu, a.lens = lens, a.table = table;
+  a.B = B, a.T = T, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk;
+  a.max_blocks = max_blocks, a.num_blocks = num_blocks, a.block = block;
+  a.block_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if ((1 << s) == block) a.block_shift = s;
+  a.tiles = pd_chunk_attn_tiles(T, B, a.G);
+  a.splits = splits, a.min_keys = min_keys < ca::kBN ? ca::kBN : min_keys;
+  a.scale_log2 = scale * ca::kLog2e;
+  a.part_o = part_o, a.part_ml = part_ml;
+  const long wgs = (long)a.tiles * Hk * splits;
+  if (wgs > 0x7fffffffL) return -1;
+  hipStream_t st = (hipStream_t)stream;
+#define PD_CHUNK(DV)                                                                        \
+  do {                                                                                      \
+    if (f16) ca::chunk_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);                  \
+    else ca::chunk_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);                     \
+    if (splits > 1) {                                                                       \
+      if (f16) ca::join_kernel<DV, true><<<T, 256, 0, st>>>(a);                             \
+      else ca::join_kernel<DV, false><<<T, 256, 0, st>>>(a);                                \
+    }                                                                                       \
+  } while (0)
+  if (D == 64) PD_CHUNK(64);
+  else if (D == 128) PD_CHUNK(128);
+  else return -2;
+#undef PD_CHUNK
+  return (int)hipGetLastError();
+}

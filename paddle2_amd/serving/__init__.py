@@ -11,6 +11,9 @@ MI355X design:
     split), GQA heads served from one K/V read, fp32 split merge), same kernel for the
     contiguous MMHA cache and the paged block cache via stride/block-table addressing;
   * new K/V rows land in the cache with one gather-free write kernel (block-table addressed);
+  * a chunk of new tokens over a cache that holds their past (chunked prefill, drafted tokens, mixed steps) =
+    ``chunk_attention``, one launch for a ragged batch; forked, truncated and compacted caches = ``copy_kv_blocks``,
+    one launch for all layers; the next token from given random numbers = ``sample_tokens``;
   * the per-token decode step of a fixed batch is a static-shape graph: ``LlamaGenerator`` can
     capture it once in a HIP graph and replay it (launch-bound loops -> one graph launch).
 """
@@ -25,6 +28,8 @@ from ..framework.tensor import Tensor
 from ..ops import _native as N
 from ..ops import torch_ops as T
 from ..distributed.collective import ring_all_reduce
+from .paged import KVBlockCopier, chunk_attention, copy_kv_blocks  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401
 
 _wrap = Tensor._wrap
 
@@ -144,7 +149,10 @@ def write_kv(k, v, k_cache, v_cache, tok_batch, tok_pos, block_table=None, layou
 
 # ============================================================================ paged KV cache
 class PagedKVCache:
-    """Per-layer K/V block pools [num_blocks, block_size, Hk, D] with a free list and block tables."""
+    """Per-layer K/V block pools [num_blocks, block_size, Hk, D] with a free list and block tables.
+
+    Pages may be shared: ``fork`` gives another sequence the full pages of one, and a page goes back to the free list
+    when its last holder lets go.  Full pages are only read; the page a sequence still writes is always its own."""
 
     def __init__(self, num_layers, num_blocks, block_size, num_kv_heads, head_dim, max_batch, max_seq_len,
                  dtype=torch.bfloat16, device=None):
@@ -159,26 +167,128 @@ class PagedKVCache:
         self.seq_lens = torch.zeros(max_batch, dtype=torch.int32, device=dev)
         self._free = list(range(num_blocks - 1, -1, -1))
         self._owned = {}
+        self._holders = [0] * num_blocks
+        self._copier = None
+
+    def _take(self):
+        if not self._free:
+            raise RuntimeError("PagedKVCache out of blocks")
+        b = self._free.pop()
+        self._holders[b] = 1
+        return b
+
+    def _drop(self, b):
+        self._holders[b] -= 1
+        if self._holders[b] == 0:
+            self._free.append(b)
 
     def allocate(self, slot, num_tokens):
         """Make sure sequence ``slot`` has blocks for ``num_tokens`` tokens."""
         have = self._owned.setdefault(slot, [])
         need = (num_tokens + self.block_size - 1) // self.block_size
         while len(have) < need:
-            if not self._free:
-                raise RuntimeError("PagedKVCache out of blocks")
-            b = self._free.pop()
+            if len(have) >= self.max_blocks_per_seq:
+                raise IndexError(f"PagedKVCache: {num_tokens} tokens do not fit {self.max_blocks_per_seq} blocks per sequence")
+            b = self._take()
             self.block_table[slot, len(have)] = b
             have.append(b)
 
     def free(self, slot):
         for b in self._owned.pop(slot, []):
-            self._free.append(b)
+            self._drop(b)
         self.seq_lens[slot] = 0
 
     @property
     def num_free_blocks(self):
         return len(self._free)
+
+    # ------------------------------------------------------------------ shared pages
+    def copy_blocks(self, src, dst):
+        """Page src[i] -> page dst[i] in the K and V pools of every layer, one launch (KVBlockCopier.copy)."""
+        if self._copier is None or any(a is not b for a, b in zip(self._copier.pools, self.k + self.v)):
+            self._copier = KVBlockCopier(self.k, self.v)
+        self._copier.copy(src, dst)
+
+    def _write_rows(self, slots):
+        """The block-table rows of ``slots`` from the host's lists, in one copy."""
+        rows = torch.zeros(len(slots), self.max_blocks_per_seq, dtype=torch.int32)
+        for i, s in enumerate(slots):
+            rows[i, :len(self._owned[s])] = torch.tensor(self._owned[s], dtype=torch.int32)
+        dev = self.block_table.device
+        self.block_table[torch.tensor(slots, device=dev)] = rows.to(dev)
+
+    def _slot(self, slot):
+        if not 0 <= slot < self.block_table.shape[0]:
+            raise IndexError(f"PagedKVCache: slot {slot} of {self.block_table.shape[0]}")
+        return slot
+
+    def fork(self, slot, new_slots, num_tokens=None):
+        """Sequences ``new_slots`` (free ones) become copies of the first ``num_tokens`` tokens of ``slot`` (default: its
+        seq_lens).  Full pages are shared, the last, partly filled one is copied for each, so all of them may grow on
+        their own.  RuntimeError, with nothing changed, when there are too few free pages."""
+        new_slots = [self._slot(int(s)) for s in new_slots]
+        have = self._owned.get(self._slot(slot), [])
+        n = int(self.seq_lens[slot]) if num_tokens is None else int(num_tokens)
+        if not 0 <= n <= len(have) * self.block_size:
+            raise ValueError(f"PagedKVCache.fork: {n} tokens, slot {slot} holds {len(have)} blocks of {self.block_size}")
+        if len(set(new_slots)) < len(new_slots) or any(self._owned.get(s) for s in new_slots):
+            raise ValueError(f"PagedKVCache.fork: slots {new_slots} must be different and free")
+        full, rest = n // self.block_size, n % self.block_size
+        if rest and len(self._free) < len(new_slots):
+            raise RuntimeError("PagedKVCache out of blocks")
+        if not new_slots:
+            return
+        own = []
+        for s in new_slots:
+            for b in have[:full]:
+                self._holders[b] += 1
+            self._owned[s] = have[:full]
+            if rest:
+                own.append(self._take())
+                self._owned[s].append(own[-1])
+        if own:
+            self.copy_blocks([have[full]] * len(own), own)
+        self._write_rows(new_slots)
+        self.seq_lens[torch.tensor(new_slots, device=self.seq_lens.device)] = n
+
+    def truncate(self, slot, num_tokens):
+        """Sequence ``slot`` goes back to its first ``num_tokens`` tokens: the pages behind them are given up, and a last
+        page that it will write again but shares is replaced by a copy."""
+        have = self._owned.get(self._slot(slot), [])
+        n = int(num_tokens)
+        if not 0 <= n <= len(have) * self.block_size:
+            raise ValueError(f"PagedKVCache.truncate: {n} tokens, slot {slot} holds {len(have)} blocks of {self.block_size}")
+        keep = -(-n // self.block_size)
+        last = have[keep - 1] if n % self.block_size else None
+        shared = last is not None and self._holders[last] > 1
+        if shared and not self._free and all(self._holders[b] > 1 for b in have[keep:]):
+            raise RuntimeError("PagedKVCache out of blocks")
+        while len(have) > keep:
+            self._drop(have.pop())
+        if shared:
+            have[-1] = self._take()
+            self.copy_blocks([last], [have[-1]])
+            self._drop(last)
+            self._write_rows([slot])
+        self.seq_lens[slot] = n
+
+    def compact(self):
+        """Move the pages in use to the front of the pools, so that pages 0 .. in use - 1 are the used ones; block tables
+        follow.  Returns the number of pages moved."""
+        used = [b for b, h in enumerate(self._holders) if h]
+        src = [b for b in used if b >= len(used)]
+        if src:
+            dst = [b for b in range(len(used)) if not self._holders[b]]
+            self.copy_blocks(src, dst)
+            to = dict(zip(src, dst))
+            slots = [s for s, have in self._owned.items() if any(b in to for b in have)]
+            for s in slots:
+                self._owned[s] = [to.get(b, b) for b in self._owned[s]]
+            for a, b in to.items():
+                self._holders[a], self._holders[b] = 0, self._holders[a]
+            self._write_rows(slots)
+        self._free = list(range(len(self._holders) - 1, len(used) - 1, -1))
+        return len(src)
 
 
 # ============================================================================ Paddle APIs
@@ -227,7 +337,8 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
                               quant_min_bound=-127.0, out_scale=-1, compute_dtype="default", rope_theta=10000.0):
     """Ragged batch over a paged cache [blocks, nh, block_size, hd]: sequences with
     seq_lens_encoder > 0 run causal prefill (flash kernel) and fill the cache; the others append
-    one token and run decode attention.  Returns (out [token_num, nh*hd], qkv, key_cache, value_cache)."""
+    seq_lens_this_time tokens behind their seq_lens_decoder cached ones: decode attention for one token,
+    chunk attention for several.  Returns (out [token_num, nh*hd], qkv, key_cache, value_cache)."""
     t = _u(qkv)
     if qkv_bias is not None:
         t = t + _u(qkv_bias).reshape(1, -1)
@@ -246,6 +357,7 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
     if rope_emb is not None:
         re = _u(rope_emb)  # [2, b, max_s, 1, D/2]
     dec_rows, dec_b = [], []
+    several = []   # (sequence, first row, rows, q): more than one new token over a cache
     for b in range(len(now)):
         if now[b] == 0:
             continue
@@ -269,6 +381,8 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
         if enc[b] > 0:
             o, _ = T.flash_attention(q[None], k[None], v[None], causal=True)
             out[s0:s0 + n] = o[0]
+        elif n > 1:
+            several.append((b, s0, n, q))
         else:
             dec_rows.append(s0)
             dec_b.append((b, q))
@@ -279,6 +393,14 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
         od = decode_attention(qd, kc, vc, lens, bt[idx], layout="paddle_block")
         for i, r in enumerate(dec_rows):
             out[r] = od[i]
+    if several:
+        cu_q = torch.zeros(len(several) + 1, dtype=torch.int32)
+        cu_q[1:] = torch.tensor([n for _, _, n, _ in several], dtype=torch.int32).cumsum(0)
+        lens = torch.tensor([dec[b] + n for b, _, n, _ in several], dtype=torch.int32, device=t.device)
+        oc = chunk_attention(torch.cat([q for _, _, _, q in several]), kc, vc, cu_q.to(t.device), lens,
+                             bt[torch.tensor([b for b, _, _, _ in several], device=t.device)], layout="paddle_block")
+        for (_, s0, n, _), r in zip(several, cu_q.tolist()):
+            out[s0:s0 + n] = oc[r:r + n]
     return _wrap(out.reshape(tok, Hq * D)), qkv, key_cache, value_cache
 
 

@@ -19,7 +19,7 @@ import torch
 
 from ..framework.tensor import Tensor
 from ..ops import torch_ops as T
-from . import PagedKVCache, decode_attention, write_kv
+from . import PagedKVCache, chunk_attention, decode_attention, sample_tokens, write_kv
 
 
 def sample_logits(logits, temperature=1.0, top_k=0, top_p=1.0, generator=None):
@@ -264,6 +264,61 @@ class LlamaGenerator:
             self.cache.seq_lens[s] = n
         return self._logits_of(x[:, last], residual[:, last])[0]
 
+    @torch.no_grad()
+    def extend(self, slots, chunks, held=None):
+        """Append the tokens ``chunks[i]`` to sequence ``slots[i]``, over the ``held[i]`` tokens that the cache holds of it
+        already: the next chunk of a prompt, another turn, drafted tokens.  ``held`` is the cache's seq_lens by default,
+        which prefill and extend keep and decode_step does not.  All chunks run as one packed token batch; a
+        sequence's first chunk may be its prompt's start.  Returns the last-token logits [len(slots), V]."""
+        lens = [len(c) for c in chunks]
+        if len(lens) != len(slots) or len(set(slots)) < len(lens) or min(lens, default=0) < 1:
+            raise ValueError("extend: one non-empty chunk for each slot, every slot once")
+        total = sum(lens)
+        nh, nkv, d = self.nh, self.nkv, self.d
+        slot_t = torch.tensor(list(slots), dtype=torch.long, device=self.dev)
+        held = self.cache.seq_lens[slot_t].tolist() if held is None else [int(h) for h in held]
+        if len(held) != len(lens) or min(held, default=0) < 0:
+            raise ValueError(f"extend: held {held} for {len(lens)} slots")
+        for s, n, h in zip(slots, lens, held):
+            self.cache.allocate(s, h + n + 1)
+        ids = torch.as_tensor([int(t) for c in chunks for t in c], dtype=torch.long).to(self.dev)
+        pos = torch.cat([torch.arange(h, h + n, dtype=torch.int32) for h, n in zip(held, lens)]).to(self.dev)
+        tok_batch = torch.cat([torch.full((n,), s, dtype=torch.int32) for s, n in zip(slots, lens)]).to(self.dev)
+        cu = torch.zeros(len(lens) + 1, dtype=torch.int32)
+        cu[1:] = torch.cumsum(torch.as_tensor(lens, dtype=torch.int32), 0)
+        last = (cu[1:] - 1).to(torch.long).to(self.dev)
+        cu = cu.to(self.dev)
+        keys = torch.tensor([h + n for h, n in zip(held, lens)], dtype=torch.int32).to(self.dev)
+        table = self.cache.block_table[slot_t]
+        pos_l = pos.long()[None]
+        x = self.model.llama.embed_tokens.weight._t[ids][None]
+        residual = None
+        for li, layer in enumerate(self.model.llama.layers):
+            qkv, residual = self._layer_qkv(layer, x, residual)
+            qkv = qkv.view(1, total, nh + 2 * nkv, d)
+            qk = T.rope(qkv[:, :, :nh + nkv], self.cos, self.sin, pos_l, style=0)
+            q, k, v = qk[0, :, :nh], qk[0, :, nh:], qkv[0, :, nh + nkv:]
+            write_kv(k, v, self.cache.k[li], self.cache.v[li], tok_batch, pos, self.cache.block_table)
+            o = chunk_attention(q, self.cache.k[li], self.cache.v[li], cu, keys, table)
+            x, residual = self._layer_out(layer, o.reshape(1, total, nh * d), residual)
+        self.cache.seq_lens[slot_t] = keys
+        return self._logits_of(x[:, last], residual[:, last])[0]
+
+    @torch.no_grad()
+    def prefill_chunks(self, slots, prompts, chunk_size):
+        """Prompts in pieces of at most ``chunk_size`` tokens, all sequences' pieces of a round in one ``extend``: the
+        activations of a long prompt are chunk_size rows instead of the whole length.  Last-token logits [n, V]."""
+        if chunk_size < 1 or min((len(p) for p in prompts), default=1) < 1:
+            raise ValueError(f"prefill_chunks: chunk_size {chunk_size}, prompts of {[len(p) for p in prompts]} tokens")
+        out = [None] * len(slots)
+        for at in range(0, max((len(p) for p in prompts), default=0), chunk_size):
+            some = [i for i, p in enumerate(prompts) if len(p) > at]
+            logits = self.extend([slots[i] for i in some], [prompts[i][at:at + chunk_size] for i in some])
+            for row, i in zip(logits, some):
+                if len(prompts[i]) <= at + chunk_size:
+                    out[i] = row
+        return torch.stack(out)
+
     # ------------------------------------------------------------------ decode
     def _decode_body(self):
         nh, nkv, d = self.nh, self.nkv, self.d
@@ -313,32 +368,75 @@ class LlamaGenerator:
     # ------------------------------------------------------------------ generate
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens=32, temperature=0.0, top_k=0, top_p=1.0, eos_token_id=None,
-                 seed=0):
-        """prompts: list of 1-D id sequences (<= max_batch). Returns list of generated id lists."""
-        assert len(prompts) <= self.max_batch
+                 seed=0, min_p=0.0, sampler=None, chunk_size=None, num_return_sequences=1):
+        """prompts: list of 1-D id sequences (<= max_batch). Returns list of generated id lists.
+
+        ``num_return_sequences`` n > 1: n continuations of every prompt, one after the other in the result; a prompt is
+        computed once and its pages are shared (PagedKVCache.fork).  ``chunk_size``: prompts run in pieces of that many
+        tokens (prefill_chunks).  ``sampler``: "multinomial" draws with torch.multinomial (``sample_logits``), "fused" with
+        ``sample_tokens``; the default is "multinomial", except where only ``sample_tokens`` can serve: ``min_p`` above 0, or
+        a list of one value per prompt for temperature, top_k, top_p or min_p."""
+        n_ret = int(num_return_sequences)
+        assert n_ret >= 1 and len(prompts) * n_ret <= self.max_batch
+        if n_ret > 1:
+            prompts = list(prompts)
+        n_seq = len(prompts) * n_ret
+        settings = dict(temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        own = {k for k, v in settings.items() if isinstance(v, (list, tuple))}
+        fused_only = bool(own) or min_p > 0
+        sampler = sampler or ("fused" if fused_only else "multinomial")
+        if sampler not in ("fused", "multinomial") or (sampler == "multinomial" and fused_only):
+            raise ValueError(f"generate: sampler {sampler!r} with temperature={temperature}, top_k={top_k}, top_p={top_p}, "
+                             f"min_p={min_p}")
         gen = torch.Generator(device=self.dev).manual_seed(seed) if self.dev.type == "cuda" else \
             torch.Generator().manual_seed(seed)
         B = self.max_batch
         toks = torch.zeros(B, dtype=torch.long, device=self.dev)
         pos = torch.zeros(B, dtype=torch.int32, device=self.dev)
-        outs = [[] for _ in prompts]
-        done = [False] * len(prompts)
-        # one packed prefill for all prompts (per-prompt when a single one is given)
-        first = (self.prefill_batch(list(range(len(prompts))), prompts) if len(prompts) > 1 else
-                 self.prefill(0, torch.as_tensor(prompts[0], dtype=torch.long))[None]) if prompts else None
-        for i, p in enumerate(prompts):
-            t = sample_logits(first[i:i + 1], temperature, top_k, top_p, gen)[0]
+        outs = [[] for _ in range(n_seq)]
+        done = [False] * n_seq
+        for k in own:
+            if len(settings[k]) != len(prompts):
+                raise ValueError(f"generate: {len(settings[k])} values of {k} for {len(prompts)} prompts")
+            v = [x for x in settings[k] for _ in range(n_ret)] + [0] * (B - n_seq)
+            settings[k] = torch.tensor(v, dtype=torch.int32 if k == "top_k" else torch.float32, device=self.dev)
+
+        def draw(logits):
+            if sampler == "multinomial":
+                return sample_logits(logits, temperature, top_k, top_p, gen)
+            u = torch.rand(logits.shape[0], generator=gen, device=self.dev)
+            rows = {k: v[:logits.shape[0]] if torch.is_tensor(v) else v for k, v in settings.items()}
+            return sample_tokens(logits, u, **rows)
+
+        heads = list(range(0, n_seq, n_ret))   # the slot that runs each prompt
+        if not prompts:
+            first = None
+        elif chunk_size is not None:
+            first = self.prefill_chunks(heads, prompts, int(chunk_size))
+        elif len(prompts) > 1:   # one packed prefill for all prompts (per-prompt when a single one is given)
+            first = self.prefill_batch(heads, prompts)
+        else:
+            first = self.prefill(0, torch.as_tensor(prompts[0], dtype=torch.long))[None]
+        if n_ret > 1 and prompts:
+            for s, p in zip(heads, prompts):
+                self.cache.fork(s, range(s + 1, s + n_ret), len(p))
+            first = first.repeat_interleave(n_ret, 0)
+        if sampler == "fused" and prompts:
+            first_toks = draw(first)
+        for i in range(n_seq):
+            t = first_toks[i] if sampler == "fused" else draw(first[i:i + 1])[0]
+            n = len(prompts[i // n_ret])
             toks[i] = t
-            pos[i] = len(p)
+            pos[i] = n
             outs[i].append(int(t))
-            self.cache.allocate(i, len(p) + max_new_tokens + 1)
-        for i in range(len(prompts), B):  # idle slots decode a dummy token at position 0
+            self.cache.allocate(i, n + max_new_tokens + 1)
+        for i in range(n_seq, B):  # idle slots decode a dummy token at position 0
             self.cache.allocate(i, max_new_tokens + 2)
         for _ in range(max_new_tokens - 1):
             logits = self.decode_step(toks, pos)
-            nxt = sample_logits(logits, temperature, top_k, top_p, gen)
+            nxt = draw(logits)
             pos = pos + 1
-            for i in range(len(prompts)):
+            for i in range(n_seq):
                 if done[i]:
                     continue
                 ti = int(nxt[i])

@@ -1,0 +1,216 @@
+"""Paged-cache operators of the serving runtime: attention of new tokens over cache pages, and copies of pages.
+
+Both run on hand-written kernels (csrc/kernels/chunk_attn.hip, csrc/kernels/kv_pages.hip) on the GPU; on CPU tensors the
+same definitions run in PyTorch.  Inference only: nothing here records a gradient.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+
+import torch
+
+from ..framework.tensor import Tensor
+from ..ops import _native as N
+
+_HEAD_DIMS = (64, 128)
+# split of a tile's keys over workgroups: enough of them to fill the chip, each with at least this many keys
+_CHUNK_WG_TARGET = 512
+_CHUNK_MIN_KEYS = 256
+
+
+def _u(x):
+    return x._t if isinstance(x, Tensor) else x
+
+
+def _on(dev):
+    """The device of the operands as the current one, for the launch and its stream."""
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _ints(t, name, size, dev):
+    """A 1-D or 2-D int tensor on ``dev`` as contiguous int32."""
+    t = _u(t)
+    if not torch.is_tensor(t) or t.is_floating_point() or t.dtype == torch.bool:
+        raise TypeError(f"chunk_attention: {name} must be an integer tensor")
+    if t.device != dev:
+        raise ValueError(f"chunk_attention: {name} is on {t.device}, the queries on {dev}")
+    if t.dim() != len(size) or any(s is not None and s != n for s, n in zip(size, t.shape)):
+        raise ValueError(f"chunk_attention: {name} has shape {tuple(t.shape)}, expected {size}")
+    return t.to(torch.int32).contiguous()
+
+
+@torch.no_grad()
+def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=None, layout="paged", scale=None, out=None):
+    """Attention of the new tokens of a ragged batch over a paged KV cache.
+
+    q [T, Hq, D] holds the new tokens of all sequences back to back: sequence b owns rows cu_seqlens_q[b] ..
+    cu_seqlens_q[b + 1] (int32 [B + 1], not decreasing).  seq_lens[b] (int32 [B]) counts the tokens of sequence b in the
+    cache, these new ones included (write_kv comes first), so its new token i stands at position
+    seq_lens[b] - n_b + i and sees the keys up to and including its own.  n_b may be 0, 1 (decoding) or any length, all in
+    one call; the lengths are read on the device, so the call can be captured in a graph and replayed with others.
+
+    Caches and ``block_table`` [B, max_blocks] as in :func:`decode_attention`: layout "paged" [num_blocks, block_size,
+    Hk, D], "paddle_block" [num_blocks, Hk, block_size, D], "bhsd" [B, Hk, max_s, D] without a table.  A row that sees
+    no key (position below 0) gives zeros; a page number outside the pool reads as zeros; lengths past the table are
+    cut to it.  Rows past cu_seqlens_q[B] are left as they are in ``out`` and are undefined in a new output.
+
+    bfloat16 and float16 with D 64 or 128 on the GPU, any Hq / Hk up to 128; rows of q, out and the caches must be
+    16-byte aligned.  Returns out [T, Hq, D]."""
+    wrap = isinstance(q, Tensor)
+    q, k_cache, v_cache, out = _u(q), _u(k_cache), _u(v_cache), _u(out)
+    dev = q.device
+    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
+        raise ValueError(f"chunk_attention: q {tuple(q.shape)}, caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise TypeError(f"chunk_attention: q {q.dtype}, caches {k_cache.dtype}, {v_cache.dtype}")
+    if k_cache.device != dev or v_cache.device != dev:
+        raise ValueError(f"chunk_attention: q on {dev}, caches on {k_cache.device}, {v_cache.device}")
+    T, Hq, D = q.shape
+    tok, head = {"paged": (1, 2), "paddle_block": (2, 1), "bhsd": (2, 1)}.get(layout, (None, None))
+    if tok is None:
+        raise ValueError(f"chunk_attention: layout {layout!r}")
+    bs, Hk = k_cache.shape[tok], k_cache.shape[head]
+    if k_cache.shape[3] != D or Hk == 0 or bs == 0 or Hq % Hk:
+        raise ValueError(f"chunk_attention: q {tuple(q.shape)} does not fit the {layout} cache {tuple(k_cache.shape)}")
+    lens = _ints(seq_lens, "seq_lens", (None,), dev)
+    B = lens.shape[0]
+    cu = _ints(cu_seqlens_q, "cu_seqlens_q", (B + 1,), dev)
+    if layout == "bhsd":
+        if k_cache.shape[0] < B:
+            raise ValueError(f"chunk_attention: {B} sequences, caches for {k_cache.shape[0]}")
+        table = torch.arange(B, dtype=torch.int32, device=dev)[:, None]
+    elif block_table is None:
+        raise ValueError(f"chunk_attention: layout {layout!r} needs a block_table")
+    else:
+        table = _ints(block_table, "block_table", (B, None), dev)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"chunk_attention: scale {scale}")
+    if out is None:
+        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        raise ValueError(f"chunk_attention: out {tuple(out.shape)} {out.dtype} on {out.device}")
+    if T and B and table.shape[1] and k_cache.shape[0]:
+        if dev.type == "cuda" and N.use_native(q):
+            _chunk_native(q, k_cache, v_cache, cu, lens, table, tok, head, scale, out)
+        else:
+            _chunk_reference(q, k_cache, v_cache, cu, lens, table, tok, scale, out)
+    elif T and B:   # an empty cache: no row sees a key
+        out[:int(cu[-1])] = 0
+    return Tensor._wrap(out) if wrap else out
+
+
+def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
+    T, Hq, D = q.shape
+    B, max_blocks = table.shape
+    bs, Hk = kc.shape[tok], kc.shape[head]
+    if q.dtype not in (torch.bfloat16, torch.float16) or D not in _HEAD_DIMS or Hq // Hk > 128:
+        raise ValueError(f"chunk_attention: {q.dtype} with head dim {D} and {Hq // Hk} query heads per kv head (bfloat16 or "
+                         f"float16, {_HEAD_DIMS}, at most 128)")
+    if kc.stride() != vc.stride():
+        raise ValueError("chunk_attention: the K and V caches have different strides")
+    if q.stride(2) != 1 or (q.data_ptr() | (q.stride(0) * 2) | (q.stride(1) * 2)) & 15:
+        q = q.clone(memory_format=torch.contiguous_format)
+    for name, t in (("k_cache", kc), ("v_cache", vc), ("out", out)):
+        if t.stride(-1) != 1 or any((s * 2) & 15 for s in t.stride()[:-1]) or t.data_ptr() & 15:
+            raise ValueError(f"chunk_attention: {name} needs contiguous, 16-byte aligned rows")
+    m = N.native()
+    wgs = m.chunk_attn_tiles(T, B, Hq // Hk) * Hk
+    splits = max(1, min(-(-_CHUNK_WG_TARGET // wgs), max_blocks * bs // _CHUNK_MIN_KEYS, 64))
+    with _on(q.device):
+        po = pm = None
+        if splits > 1:
+            po = torch.empty(splits * T * Hq * D, dtype=torch.float32, device=q.device)
+            pm = torch.empty(splits * T * Hq * 2, dtype=torch.float32, device=q.device)
+        m.chunk_attn(int(q.dtype == torch.float16), q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
+                     kc.stride(0), kc.stride(tok), kc.stride(head), table.data_ptr(), max_blocks, kc.shape[0], bs,
+                     cu.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), B, T, Hq, Hk, D,
+                     splits, _CHUNK_MIN_KEYS, scale, N.ptr(po), N.ptr(pm), N.stream())
+
+
+def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):
+    T, Hq, D = q.shape
+    acc = torch.float64 if q.dtype == torch.float64 else torch.float32
+    if tok == 2:
+        kc, vc = kc.transpose(1, 2), vc.transpose(1, 2)
+    nb, bs, Hk = kc.shape[:3]
+    cu, lens = cu.clamp(0, T).tolist(), lens.tolist()
+    for b, L in enumerate(lens):
+        q0, n = cu[b], cu[b + 1] - cu[b]
+        if n <= 0:
+            continue
+        L = max(0, min(L, table.shape[1] * bs))
+        j = torch.arange(L, device=q.device)
+        page = table[b].long()[j // bs]
+        ok = (page >= 0) & (page < nb)
+        ks, vs = (torch.where(ok[:, None, None], c[page.clamp(0, nb - 1), j % bs], 0).to(acc) for c in (kc, vc))
+        qs = q[q0:q0 + n].to(acc).reshape(n, Hk, Hq // Hk, D)
+        hidden = j[None] > torch.arange(L - n, L, device=q.device)[:, None]
+        s = torch.einsum("nhgd,lhd->hgnl", qs, ks) * scale
+        s = s.masked_fill(hidden, float("-inf"))
+        # rows that see no key: zeros.  Hidden values are left out, not multiplied by zero (they may be infinite)
+        top = s.amax(-1, keepdim=True) if L else s.new_zeros(s.shape[:-1] + (1,))
+        p = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
+        z = p.sum(-1, keepdim=True)
+        bad = ~torch.isfinite(vs).all(-1).all(-1)
+        o = torch.einsum("hgnl,lhd->nhgd", p, torch.where(bad[:, None, None], 0.0, vs))
+        for i in bad.nonzero().flatten().tolist():
+            first = max(0, i - (L - n))
+            o[first:] += torch.einsum("hgn,hd->nhgd", p[:, :, first:, i], vs[i])
+        z = z.permute(2, 0, 1, 3)
+        out[q0:q0 + n] = torch.where(z == 0, 0.0, o / z).reshape(n, Hq, D).to(out.dtype)
+
+
+class KVBlockCopier:
+    """Copies pages inside the K and V pools of all layers in one launch.
+
+    ``k_caches`` / ``v_caches``: one tensor per layer, [num_blocks, ...], all of one shape, type, device and stride, each
+    page contiguous.  The pools are checked once here and kept; ``copy`` may then be called as often as wanted."""
+
+    def __init__(self, k_caches, v_caches):
+        pools = [_u(t) for t in (list(k_caches) + list(v_caches))]
+        if not pools:
+            raise ValueError("copy_kv_blocks: no caches")
+        a = pools[0]
+        if a.dim() < 2 or not a[:1].is_contiguous() or (a.shape[0] > 1 and a.stride(0) < a[0].numel()):
+            raise ValueError("copy_kv_blocks: the pages of a cache must be contiguous")
+        for t in pools:
+            if t.shape != a.shape or t.dtype != a.dtype or t.device != a.device or t.stride() != a.stride():
+                raise ValueError("copy_kv_blocks: the caches differ in shape, type, device or stride")
+        self.pools = pools
+        self._dev = a.device
+        self._blocks = a.shape[0]
+        self._bytes = (a.numel() // max(a.shape[0], 1)) * a.element_size()
+        self._stride = a.stride(0) * a.element_size()
+        self._native = self._dev.type == "cuda" and N.use_native(a)
+        self._ptrs = [t.data_ptr() for t in pools] if self._native else None
+
+    @torch.no_grad()
+    def copy(self, src, dst):
+        """Page src[i] -> page dst[i] in every pool, on the current stream.  ``src`` / ``dst``: host integers.  A page may be
+        a source many times, a destination once, and never both; ValueError otherwise, with nothing copied."""
+        if self._native:
+            with _on(self._dev):
+                N.native().kv_copy(self._ptrs, src, dst, self._blocks, self._bytes, self._stride, N.stream())
+            return
+        src, dst = [int(i) for i in src], [int(i) for i in dst]
+        if len(src) != len(dst):
+            raise ValueError("src and dst differ in length")
+        for i in src + dst:
+            if not 0 <= i < self._blocks:
+                raise ValueError(f"page {i} is not in the pool")
+        if len(set(dst)) < len(dst):
+            raise ValueError("a page is a destination twice")
+        if set(src) & set(dst):
+            raise ValueError("a page is both a source and a destination")
+        if src:
+            s, d = (torch.tensor(i, device=self._dev) for i in (src, dst))
+            for t in self.pools:
+                t[d] = t[s]
+
+
+def copy_kv_blocks(k_caches, v_caches, src, dst):
+    """``KVBlockCopier(k_caches, v_caches).copy(src, dst)``: page src[i] of every layer's K and V pool -> page dst[i].  A
+    program that copies often keeps the copier (PagedKVCache.copy_blocks does)."""
+    KVBlockCopier(k_caches, v_caches).copy(src, dst)

@@ -1,0 +1,110 @@
+"""The next token of every row of logits, from given random numbers (csrc/kernels/sampling.hip)."""
+from __future__ import annotations
+
+import math
+import numbers
+
+import torch
+
+from ..framework.tensor import Tensor
+from ..ops import _native as N
+from .paged import _on, _u
+
+_MAX_VOCAB = 1 << 20
+
+
+def _setting(v, name, rows, dev, dtype, lo, hi):
+    """(tensor or None, number): one value per row, or one for all, checked where the host can see it."""
+    v = _u(v)
+    if torch.is_tensor(v):
+        if v.shape != (rows,) or v.device != dev:
+            raise ValueError(f"sample_tokens: {name} {tuple(v.shape)} on {v.device}, expected ({rows},) on {dev}")
+        if dtype == torch.int32:
+            if v.is_floating_point() or v.dtype == torch.bool:
+                raise TypeError(f"sample_tokens: {name} must hold integers")
+            if v.dtype == torch.int64:
+                v = v.clamp(-1, 2 ** 31 - 1)
+        return v.to(dtype).contiguous(), 0
+    if not isinstance(v, numbers.Real) or not lo <= v <= hi or (dtype == torch.int32 and v != int(v)):
+        raise ValueError(f"sample_tokens: {name} = {v!r} (a number in [{lo}, {hi}] or a tensor of one per row)")
+    return None, int(min(v, 2 ** 31 - 1)) if dtype == torch.int32 else float(v)
+
+
+@torch.no_grad()
+def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """Draw one token per row: logits [B, V] (float32, bfloat16, float16) and a random number per row,
+    ``uniform`` [B] float32 in [0, 1) -> int64 [B].
+
+    With w_i = exp((x_i - max x) / temperature) and the tokens ordered by logit, equal ones by index:
+    ``top_k`` > 0 keeps the first k; ``top_p`` < 1 then keeps the shortest head whose mass reaches top_p of what is left
+    (one token at least); ``min_p`` > 0 then keeps w_i >= min_p, that is, tokens at least min_p times as likely as the
+    best.  The token is the first, in index order, whose cumulative kept mass exceeds uniform * (kept mass).
+    ``temperature`` 0 takes the largest logit, the lowest index among equals.
+
+    Every setting is a number or a tensor of one per row ([B] on the logits' device; a temperature there that is not
+    above 0 is greedy, values outside the other ranges act as the nearest bound, NaN as off).  Logits of -inf are never
+    drawn, NaN counts as -inf, +inf shares all mass among its like; a row with nothing else gives 0.  A number at or
+    above 1 in ``uniform`` draws the last kept token.
+
+    Weights are computed and summed in 64 bits, as integers, so the token depends on the row and its number alone: the
+    same in every launch, batch and graph.  V is at most 1,048,576 on the GPU."""
+    wrap = isinstance(logits, Tensor)
+    x, u, out = _u(logits), _u(uniform), _u(out)
+    if x.dim() != 2 or x.shape[1] < 1 or not x.is_floating_point():
+        raise ValueError(f"sample_tokens: logits {tuple(x.shape)} {x.dtype}")
+    B, V = x.shape
+    dev = x.device
+    if u.shape != (B,) or u.dtype != torch.float32 or u.device != dev:
+        raise ValueError(f"sample_tokens: uniform {tuple(u.shape)} {u.dtype} on {u.device}, expected ({B},) float32 on {dev}")
+    t = _setting(temperature, "temperature", B, dev, torch.float32, 0.0, 1e30)
+    k = _setting(top_k, "top_k", B, dev, torch.int32, -1, math.inf)
+    p = _setting(top_p, "top_p", B, dev, torch.float32, 0.0, 1.0)
+    m = _setting(min_p, "min_p", B, dev, torch.float32, 0.0, 1.0)
+    if out is None:
+        out = torch.empty(B, dtype=torch.int64, device=dev)
+    elif out.shape != (B,) or out.dtype != torch.int64 or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"sample_tokens: out {tuple(out.shape)} {out.dtype} on {out.device}")
+    if B == 0:
+        pass
+    elif dev.type == "cuda" and N.use_native(x):
+        if x.dtype not in N.DT_CODE or V > _MAX_VOCAB:
+            raise ValueError(f"sample_tokens: {x.dtype} logits over {V} tokens (float32, bfloat16 or float16, at most "
+                             f"{_MAX_VOCAB})")
+        if x.stride(1) != 1 and V > 1:
+            x = x.contiguous()
+        u = u.contiguous()
+        with _on(dev):
+            N.native().sample(N.DT_CODE[x.dtype], x.data_ptr(), x.stride(0), B, V, u.data_ptr(), N.ptr(t[0]), t[1],
+                              N.ptr(k[0]), k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), N.stream())
+    else:
+        out.copy_(_reference(x, u, t, k, p, m))
+    return Tensor._wrap(out) if wrap else out
+
+
+def _reference(x, u, t, k, p, m):
+    B, V = x.shape
+
+    def column(s, dtype):
+        v = s[0] if s[0] is not None else torch.full((B,), s[1], dtype=dtype, device=x.device)
+        return v.to(dtype).double()[:, None]
+
+    t, k, p, m = (column(s, d) for s, d in zip((t, k, p, m), (torch.float32, torch.int32) + (torch.float32,) * 2))
+    t, p, m = torch.nan_to_num(t, nan=0.0), torch.nan_to_num(p, nan=1.0), torch.nan_to_num(m, nan=0.0).clamp(max=1.0)
+    x = torch.where(torch.isnan(x), float("-inf"), x.double())
+    top = x.amax(1, keepdim=True)
+    w = torch.exp((x - top) / torch.where(t > 0, t, 1.0))
+    w = torch.where(x == top, 1.0, torch.where(torch.isnan(w) | (x == float("-inf")), 0.0, w))
+    sx, order = torch.sort(x, dim=1, descending=True, stable=True)
+    sw = w.gather(1, order)
+    rank = torch.arange(V, device=x.device)[None]
+    sw = torch.where((k > 0) & (rank >= k), 0.0, sw)
+    before = sw.cumsum(1) - sw
+    keep = ((p >= 1) | (before < p * sw.sum(1, keepdim=True)) | (rank == 0)) & (sw >= m)
+    kept = torch.zeros_like(w).scatter_(1, order, torch.where(keep, sw, 0.0))
+    c = kept.cumsum(1)
+    z = c[:, -1:]
+    u = torch.nan_to_num(u.double(), nan=0.0).clamp(0.0, 1.0)[:, None]
+    token = (c <= u * z).sum(1)
+    last = V - 1 - (kept.flip(1) > 0).int().argmax(1)
+    token = torch.minimum(token, last)
+    return torch.where((t[:, 0] > 0) & (top[:, 0] > float("-inf")), token, x.argmax(1))
