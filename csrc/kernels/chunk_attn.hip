@@ -15,12 +15,13 @@
 //  * 64-key tiles go global -> registers -> LDS, two stages, page numbers one tile further ahead.  Keys past the
 //    rows' reach and pages outside the pool are read from a block of zeros, so stale pages (NaN among them) never
 //    reach a product.
-//  * A hidden key has P = 0, but 0 * inf is NaN: where a tile on the diagonal holds a value that is not finite, its
-//    product runs on the finite values, and infinities and NaN are added to the rows that see them (counted by two
-//    products with a 0 / 1 visibility operand).
+//  * A hidden key has P = 0, but 0 * inf is NaN: in tiles that some row does not see in full, values that are not
+//    finite enter the product as 0 and are added at the end to the rows that see them.
 //  * Few rows over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
 //    second kernel.  How often is decided per tile, from its own length.
 #include "common.h"
+
+#include <type_traits>
 
 namespace pd {
 namespace ca {
@@ -30,6 +31,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -43,7 +45,7 @@ struct Args {
   const unsigned short *q, *k, *v;
   unsigned short* out;
   long sq_tok, sq_head, so_tok, so_head;   // in elements
-  long s_blk, s_tok, s_head;
+  int s_blk, s_tok, s_head;
   const int *cu, *lens, *table;
   int B, T, Hq, Hk, G;
   int max_blocks, num_blocks, block, block_shift;   // block_shift < 0: block is no power of two
@@ -139,12 +141,21 @@ __device__ __forceinline__ int xcd_remap(int bid, int n) {
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
 }
 
-template <int D, bool F16>
-__global__ __launch_bounds__(256, D > 128 ? 1 : 2) void chunk_kernel(Args a) {
+// Barrier for LDS hand-offs: this wave's LDS operations are done, its global loads may stay in flight (__syncthreads
+// would wait for them too)
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+template <int D, bool F16, bool POW2>
+__global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
   constexpr int NCH = D / 8, KS = D / 16, DT = D / 32, TILE = kBN * D * 2;
+  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;         // exponent bits: all set in infinities and NaN
   constexpr int NLOAD = kBN * NCH / 256, ROWS = 256 / NCH;   // loads per thread and tile; rows between them
   __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
-  __shared__ int odd_tile[2];   // per stage: the first key of the last tile staged with a value that is not finite
+  __shared__ int odd_values;   // finite_only took something out
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 31, h = lane >> 5;
   const int tile_tokens = kBM / a.G;
@@ -180,43 +191,51 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void chunk_kernel(Args a) {
   // page numbers, then rows, of the tile's 64 keys; a thread loads chunk tid % NCH of rows tid / NCH + ROWS * i
   const int lrow = tid / NCH, lch = tid % NCH;
   const int* tab = a.table + (long)s.b * a.max_blocks;
-  const long head_off = (long)hk * a.s_head + lch * 8;
-  auto block_of = [&](int key) { return a.block_shift >= 0 ? key >> a.block_shift : key / a.block; };
+  const int head_off = hk * a.s_head + lch * 8;
+  auto block_of = [&](int key) { return POW2 ? key >> a.block_shift : key / a.block; };
+  auto row_offset = [&](int page, int key) {   // in elements, for this thread's 8; the part within the page fits 32 bits
+    const int in_page = POW2 ? key & (a.block - 1) : key % a.block;
+    return (long)page * a.s_blk + (unsigned)(in_page * a.s_tok + head_off);
+  };
   int pid[NLOAD];
   auto pages = [&](int n0) {
 #pragma unroll
     for (int i = 0; i < NLOAD; ++i) pid[i] = tab[block_of(min(n0 + lrow + ROWS * i, k1 - 1))];
   };
-  u16x8 stk[NLOAD], stv[NLOAD];
-  auto gload = [&](int n0) {
+  u16x8 st[NLOAD];
+  auto gload = [&](const unsigned short* cache, int n0) {
 #pragma unroll
     for (int i = 0; i < NLOAD; ++i) {
       const int key = n0 + lrow + ROWS * i;
       const bool ok = key < k1 && (unsigned)pid[i] < (unsigned)a.num_blocks;
-      const int in_page = a.block_shift >= 0 ? key & (a.block - 1) : key % a.block;
-      const long off = (long)pid[i] * a.s_blk + (long)in_page * a.s_tok + head_off;
-      const u16x8* pk = ok ? reinterpret_cast<const u16x8*>(a.k + off) : &kZeros;
-      const u16x8* pv = ok ? reinterpret_cast<const u16x8*>(a.v + off) : &kZeros;
-      stk[i] = *pk;
-      stv[i] = *pv;
+      const unsigned short* p = cache + row_offset(pid[i], key);
+      st[i] = *(ok ? reinterpret_cast<const u16x8*>(p) : &kZeros);
     }
   };
-  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;   // exponent bits: all set in infinities and NaN
-  auto lstore = [&](int buf, int n0) {
-    char* kt = smem + buf * 2 * TILE;
-    if (n0 + kBN - 1 > pos0) {   // a tile with hidden keys
-      bool odd = false;
+  // (the swizzle has the row's lowest 4 bits, which ROWS leaves alone)
+  const int o_st = lrow * (D * 2) + swz<D>(lrow, lch) * 16;
+  auto lstore = [&](char* dst) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) *reinterpret_cast<u16x8*>(dst + o_st + i * ROWS * (D * 2)) = st[i];
+  };
+
+  // V rows in registers, of a tile that some row does not see in full: values that are not finite become 0 (rare)
+  auto finite_only = [&](int n0) {
+    if (n0 + kBN - 1 <= pos0) return;
+    constexpr unsigned kE = kExp | (unsigned)kExp << 16, kLow = F16 ? 0x04000400u : 0x00800080u;
+    unsigned hit = 0;   // exponent + its lowest bit carries into bit 15 iff all exponent bits are set
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) {
+      const auto w = __builtin_bit_cast(u32x4, st[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) hit |= (w[j] & kE) + kLow;
+    }
+    if (__builtin_expect(hit & 0x80008000u, 0)) {
+      odd_values = 1;
 #pragma unroll
       for (int i = 0; i < NLOAD; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) odd |= (stv[i][j] & kExp) == kExp;
-      if (odd) odd_tile[buf] = n0;
-    }
-#pragma unroll
-    for (int i = 0; i < NLOAD; ++i) {
-      const int rr = lrow + ROWS * i, o = rr * (D * 2) + swz<D>(rr, lch) * 16;
-      *reinterpret_cast<u16x8*>(kt + o) = stk[i];
-      *reinterpret_cast<u16x8*>(kt + TILE + o) = stv[i];
+        for (int j = 0; j < 8; ++j) st[i][j] = (st[i][j] & kExp) == kExp ? (unsigned short)0 : st[i][j];
     }
   };
 
@@ -226,142 +245,141 @@ __global__ __launch_bounds__(256, D > 128 ? 1 : 2) void chunk_kernel(Args a) {
   float m = -INFINITY, l = 0.f;
   const float sl2 = a.scale_log2;
   const int wave_rt0 = wv * 32 / a.G, wave_rt1 = min((wv * 32 + 31) / a.G, ntok - 1);
-  const int wave_first = pos0 + wave_rt0;                             // keys up to here are seen by all of its rows
+  const int wave_first = min(pos0 + wave_rt0, k1 - 1);                // keys up to here are seen by all of its rows
   const int wave_last = wave_rt0 < ntok ? pos0 + wave_rt1 : -1;       // and none past here by any
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kBN - 1) / kBN : 0;
-  if (tid < 2) odd_tile[tid] = -1;
-  __syncthreads();
+  if (tid == 0) odd_values = 0;
+  lds_barrier();
   if (ntiles > 0) {
     pages(k0);
-    gload(k0);
-    if (ntiles > 1) pages(k0 + kBN);
-    lstore(0, k0);
+    gload(a.k, k0);
+    lstore(smem);
+    gload(a.v, k0);
+    pages(k0 + kBN);
+    finite_only(k0);
+    lstore(smem + TILE);
   }
-  __syncthreads();
-  // V^T reads: rows 16 s + 8 (j >> 2) + 4 hh + qq of the tile, 16-byte chunks 4 dt + cbits
-  const int g = lane >> 4, qq = (lane & 15) >> 2, pp = lane & 3, hh = g >> 1, cbits = ((g & 1) << 1) | (pp >> 1);
+  lds_barrier();
 
-  for (int t = 0; t < ntiles; ++t) {
+  // Lane bases of the LDS reads; every read is one of them with a compile-time XOR:
+  //  K row kb * 32 + r, 16-byte chunk 2 ks + h;  V^T: rows 16 s + 8 (j >> 2) + 4 hh + qq, chunk 4 dt + cbits
+  const int g = lane >> 4, qq = (lane & 15) >> 2, pp = lane & 3, hh = g >> 1, cbits = ((g & 1) << 1) | (pp >> 1);
+  int o_k = r * (D * 2) + swz<D>(r, h) * 16;
+  int o_va = (4 * hh + qq) * (D * 2) + swz<D>(4 * hh + qq, cbits) * 16 + 8 * (pp & 1);
+  int o_vb = (4 * hh + qq + 8) * (D * 2) + swz<D>(4 * hh + qq + 8, cbits) * 16 + 8 * (pp & 1);
+
+  // One tile.  MASKED: some row of the wave does not see all of its keys (two bodies: as a branch in one, the masks
+  // were turned into selects on every tile).
+  auto tile_step = [&](auto MASKED_, int t) {
+    constexpr bool MASKED = decltype(MASKED_)::value;
     const int n0 = k0 + t * kBN;
     const char* kt = smem + (t & 1) * 2 * TILE;
     const char* vt = kt + TILE;
-    const bool next = t + 1 < ntiles;
-    if (n0 <= wave_last) {
-      f32x16 sc[2];
+    char* const nxt = smem + ((t + 1) & 1) * 2 * TILE;
+    asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
+    f32x16 sc[2];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        sc[kb] = f32x16{};
-        const int kr = kb * 32 + r;
+    for (int kb = 0; kb < 2; ++kb) {
+      sc[kb] = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(kt + kr * (D * 2) + swz<D>(kr, 2 * ks + h) * 16), qf[ks], sc[kb]);
-      }
-      if (next) gload(n0 + kBN);
-      if (n0 + kBN > k1 || n0 + kBN - 1 > wave_first) {
-        const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int c = kb * 32 + (i & 3) + 8 * (i >> 2);
-            sc[kb][i] = c >= lim ? -INFINITY : sc[kb][i];
-          }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int ks = 0; ks < KS; ++ks)
+        sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(kt + kb * 32 * (D * 2) + (o_k ^ (ks << 5))), qf[ks], sc[kb]);
+    }
+    gload(a.k, n0 + kBN);   // in flight under the softmax (past the last tile it reads zeros: no branch in the tile)
+    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
+    if constexpr (MASKED) {
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[kb][i]);
-      float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-      {
-        const unsigned mu = __builtin_bit_cast(unsigned, mt);
-        const auto sw = __builtin_amdgcn_permlane32_swap(mu, mu, false, false);
-        mt = fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1]));
+        for (int i = 0; i < 16; ++i) sc[kb][i] = kb * 32 + (i & 3) + 8 * (i >> 2) >= lim ? -INFINITY : sc[kb][i];
+    }
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[kb][i]);
+    float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    {
+      const unsigned mu = __builtin_bit_cast(unsigned, mt);
+      const auto sw = __builtin_amdgcn_permlane32_swap(mu, mu, false, false);
+      mt = fmaxf(__builtin_bit_cast(float, (unsigned)sw[0]), __builtin_bit_cast(float, (unsigned)sw[1]));
+    }
+    const float mc = fmaxf(m, mt * sl2);
+    if (__builtin_expect(__any(mc > m + kDefer), 0)) {
+      asm volatile("" ::: "memory");   // a branch, not selects: it is rare
+      const float alpha = __builtin_amdgcn_exp2f(m - (mc == -INFINITY ? 0.f : mc));
+      l *= alpha;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
+      m = mc;
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+    float ls[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], sl2, -base));
+        sc[kb][i] = p;
+        ls[i & 3] += p;
       }
-      const float mc = fmaxf(m, mt * sl2);
-      if (__builtin_expect(__any(mc > m + kDefer), 0)) {
-        asm volatile("" ::: "memory");
-        const float alpha = __builtin_amdgcn_exp2f(m - (mc == -INFINITY ? 0.f : mc));
-        l *= alpha;
+    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    lstore(nxt);
+    gload(a.v, n0 + kBN);   // in flight under P.V
+    pages(n0 + 2 * kBN);
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
-        m = mc;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      float ls[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], sl2, -base));
-          sc[kb][i] = p;
-          ls[i & 3] += p;
-        }
-      l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-      auto v_frag = [&](int kb, int ss, int dt) {
-        const int ra = kb * 32 + 16 * ss + 4 * hh + qq, rb = ra + 8;
-        const s16x4 lo = lds_tr(vt, ra * (D * 2) + swz<D>(ra, 4 * dt + cbits) * 16 + 8 * (pp & 1));
-        const s16x4 hi = lds_tr(vt, rb * (D * 2) + swz<D>(rb, 4 * dt + cbits) * 16 + 8 * (pp & 1));
-        return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-      };
-      if (__builtin_expect(n0 + kBN - 1 <= wave_first || odd_tile[t & 1] != n0, 1)) {
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int ss = 0; ss < 2; ++ss) {
-            const bf16x8 pb = pack8<F16>(sc[kb], ss);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, v_frag(kb, ss, dt)), pb, o[dt]);
-          }
-      } else {
-        const int lim = min(k1, pos + 1) - n0 - 4 * h;
-        bf16x8 pb[4], seen[4];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-          for (int ss = 0; ss < 2; ++ss) pb[2 * kb + ss] = pack8<F16>(sc[kb], ss);
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) sc[kb][i] = kb * 32 + (i & 3) + 8 * (i >> 2) < lim ? 1.f : 0.f;
-#pragma unroll
-          for (int ss = 0; ss < 2; ++ss) seen[2 * kb + ss] = pack8<F16>(sc[kb], ss);
-        }
-        constexpr short kOne = F16 ? 0x3c00 : 0x3f80;
+      for (int ss = 0; ss < 2; ++ss) {
+        const bf16x8 pb = pack8<F16>(sc[kb], ss);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          f32x16 up = f32x16{}, down = f32x16{};   // infinities of each sign seen by a row; NaN counts in both
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const s16x8 vv = v_frag(i >> 1, i & 1, dt);
-            s16x8 fin, pos_inf, neg_inf;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const unsigned short w = (unsigned short)vv[j], mag = w & 0x7fff;
-              fin[j] = mag >= kExp ? (short)0 : vv[j];
-              pos_inf[j] = (mag > kExp || w == kExp) ? kOne : (short)0;
-              neg_inf[j] = (mag > kExp || w == (kExp | 0x8000)) ? kOne : (short)0;
-            }
-            o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, fin), pb[i], o[dt]);
-            up = mfma<F16>(__builtin_bit_cast(bf16x8, pos_inf), seen[i], up);
-            down = mfma<F16>(__builtin_bit_cast(bf16x8, neg_inf), seen[i], down);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            o[dt][i] += up[i] > 0.f ? INFINITY : 0.f;
-            o[dt][i] += down[i] > 0.f ? -INFINITY : 0.f;
-          }
+          const char* vr = vt + (kb * 32 + 16 * ss) * (D * 2);
+          const s16x4 lo = lds_tr(vr, o_va ^ (dt << 6)), hi = lds_tr(vr, o_vb ^ (dt << 6));
+          const s16x8 vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, vv), pb, o[dt]);
         }
       }
-    } else if (next) {
-      gload(n0 + kBN);
+    finite_only(n0 + kBN);
+    lstore(nxt + TILE);
+    lds_barrier();
+  };
+  for (int t = 0; t < ntiles; ++t) {
+    const int n0 = k0 + t * kBN;
+    if (n0 > wave_last) {   // nothing to see for this wave: it helps to stage the next tile
+      char* const nxt = smem + ((t + 1) & 1) * 2 * TILE;
+      gload(a.k, n0 + kBN);
+      lstore(nxt);
+      gload(a.v, n0 + kBN);
+      pages(n0 + 2 * kBN);
+      finite_only(n0 + kBN);
+      lstore(nxt + TILE);
+      lds_barrier();
+    } else if (n0 + kBN - 1 > wave_first) {
+      tile_step(std::true_type{}, t);
+    } else {
+      tile_step(std::false_type{}, t);
     }
-    if (next) {
-      if (t + 2 < ntiles) pages(n0 + 2 * kBN);
-      lstore((t + 1) & 1, n0 + kBN);
+  }
+
+  if (__builtin_expect(odd_values, 0)) {
+    // what finite_only took out comes back, for the rows that see it
+    // (tiles whose last key lies past pos0; a tile begins at k0 + a multiple of kBN)
+    for (int j = k0 + max(pos0 - k0, 0) / kBN * kBN; j < k1; ++j) {
+      const int page = tab[block_of(j)];
+      if ((unsigned)page >= (unsigned)a.num_blocks || !live || j > pos) continue;
+      const unsigned short* vr = a.v + row_offset(page, j) + 4 * h - lch * 8;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned short w = vr[32 * dt + 8 * c + e];
+            if ((w & kExp) == kExp) o[dt][4 * c + e] += F16 ? h2f(w) : bf2f(w);
+          }
     }
-    __syncthreads();
   }
 
   // lane (row, half h) holds O[row][32 dt + 8 c + 4 h + e] in o[dt][4 c + e]
@@ -459,13 +477,18 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   if (T <= 0 || B <= 0) return 0;
   if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1) return -1;
   if (splits > 1 && (!part_o || !part_ml)) return -1;
+  // a page's span in 32 bits (its number times s_blk is taken in 64)
+  const long span = (long)(block - 1) * s_tok + (long)(Hk - 1) * s_head + D;
+  if (s_blk < 0 || s_tok < 0 || s_head < 0 || s_blk > 0x7fffffffL || s_tok > 0x7fffffffL || s_head > 0x7fffffffL ||
+      span > 0x7fffffffL)
+    return -3;
   ca::Args a;
   a.q = (const unsigned short*)q;
   a.k = (const unsigned short*)k;
   a.v = (const unsigned short*)v;
   a.out = (unsigned short*)out;
   a.sq_tok = sq_tok, a.sq_head = sq_head, a.so_tok = so_tok, a.so_head = so_head;
-  a.s_blk = s_blk, a.s_tok = s_tok, a.s_head = s_head;
+  a.s_blk = (int)s_blk, a.s_tok = (int)s_tok, a.s_head = (int)s_head;
   a.cu = cu, a.lens = lens, a.table = table;
   a.B = B, a.T = T, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk;
   a.max_blocks = max_blocks, a.num_blocks = num_blocks, a.block = block;
@@ -481,8 +504,13 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   hipStream_t st = (hipStream_t)stream;
 #define PD_CHUNK(DV)                                                                        \
   do {                                                                                      \
-    if (f16) ca::chunk_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);                  \
-    else ca::chunk_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);                     \
+    if (a.block_shift >= 0) {                                                               \
+      if (f16) ca::chunk_kernel<DV, true, true><<<(unsigned)wgs, 256, 0, st>>>(a);          \
+      else ca::chunk_kernel<DV, false, true><<<(unsigned)wgs, 256, 0, st>>>(a);             \
+    } else {                                                                                \
+      if (f16) ca::chunk_kernel<DV, true, false><<<(unsigned)wgs, 256, 0, st>>>(a);         \
+      else ca::chunk_kernel<DV, false, false><<<(unsigned)wgs, 256, 0, st>>>(a);            \
+    }                                                                                       \
     if (splits > 1) {                                                                       \
       if (f16) ca::join_kernel<DV, true><<<T, 256, 0, st>>>(a);                             \
       else ca::join_kernel<DV, false><<<T, 256, 0, st>>>(a);                                \
