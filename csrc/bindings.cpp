@@ -80,7 +80,8 @@ int pd_chunk_attn(int, const void*, long, long, const void*, const void*, long, 
                   void*);
 int pd_kv_copy(const uint64_t*, int, const int*, const int*, int, long, long, void*);
 int pd_sample(int, const void*, long, int, int, const float*, const float*, float, const int*, int, const float*, float,
-              const float*, float, int64_t*, void*);
+              const float*, float, int64_t*, void*, void*);
+long pd_sample_workspace(int, int);
 long pd_bn_workspace(int, long, int);
 int pd_wo_splits(int, int, int, int);
 int pd_dec_splits(int, int, int);
@@ -398,12 +399,13 @@ PYBIND11_MODULE(_C, m) {
   });
   m.def("sample", [](int dt, uintptr_t logits, long stride, int B, int V, uintptr_t uniform, uintptr_t temps, float temp,
                      uintptr_t top_ks, int top_k, uintptr_t top_ps, float top_p, uintptr_t min_ps, float min_p,
-                     uintptr_t out, uintptr_t st) {
+                     uintptr_t out, uintptr_t ws, uintptr_t st) {
     check(pd_sample(dt, P<const void*>(logits), stride, B, V, P<const float*>(uniform), P<const float*>(temps), temp,
                     P<const int*>(top_ks), top_k, P<const float*>(top_ps), top_p, P<const float*>(min_ps), min_p,
-                    P<int64_t*>(out), P<void*>(st)),
+                    P<int64_t*>(out), P<void*>(ws), P<void*>(st)),
           "sample");
   });
+  m.def("sample_workspace", &pd_sample_workspace);
   m.def("decode_attn", [](uintptr_t q, long sq_b, long sq_h, uintptr_t kc, uintptr_t vc, long s_blk, long s_tok,
                           long s_head, uintptr_t table, int max_blocks, int block_size, uintptr_t seq_lens, int max_len,
                           uintptr_t part_o, uintptr_t part_ml, uintptr_t out, long so_b, long so_h, int B, int Hq,

@@ -73,9 +73,12 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         if x.stride(1) != 1 and V > 1:
             x = x.contiguous()
         u = u.contiguous()
+        if B > 65535:
+            raise ValueError(f"sample_tokens: {B} rows (at most 65,535)")
         with _on(dev):
+            ws = torch.empty(N.native().sample_workspace(B, V), dtype=torch.uint8, device=dev)
             N.native().sample(N.DT_CODE[x.dtype], x.data_ptr(), x.stride(0), B, V, u.data_ptr(), N.ptr(t[0]), t[1],
-                              N.ptr(k[0]), k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), N.stream())
+                              N.ptr(k[0]), k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), ws.data_ptr(), N.stream())
     else:
         out.copy_(_reference(x, u, t, k, p, m))
     return Tensor._wrap(out) if wrap else out
