@@ -8,7 +8,7 @@
 // A choice next to a border turns on the last bits of these sums, so weights are computed in 64 bits and summed as
 // integers of 2^-shift (shift = 62 - bits of V): integer sums do not depend on the order they are taken in, so a row's
 // token is the same in every launch.  No sort.  Four launches; a row is cut into chunks of 512 logits (a wave's load)
-// and groups of 128:
+// and groups of 32 or 128:
 //   peaks_kernel   every group's largest logit;
 //   bins_kernel    knows the row's largest.  Without top-k and top-p: the kept mass of every chunk.  Top-p alone: masses
 //                  over 2,047 bins of 1/64 in log2 of the weight, and of the tail behind them;
@@ -24,8 +24,8 @@ namespace pd {
 namespace smp {
 
 typedef unsigned long long u64;
-constexpr int kThreads = 1024, kWaves = kThreads / 64, kChunk = 512, kMaxChunks = 2048;   // V <= 2^20
-constexpr int kGroup = 128, kBins = 2048, kList = 8192, kShort = 1024, kMaxK = 512, kTable = 256;
+constexpr int kChunk = 512, kMaxChunks = 2048;   // V <= 2^20
+constexpr int kBins = 2048, kList = 8192, kShort = 1024, kMaxK = 512, kWide = 8;
 
 // bits that order as the values do; NaN as -inf, -0 as +0
 __device__ __forceinline__ unsigned key_of(float x) {
@@ -36,19 +36,54 @@ __device__ __forceinline__ float value_of(unsigned k) {
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+// Lanes of a wave summed by data-parallel moves (row_shr 1, 2, 4, 8, then row_bcast 15 and 31): a fifth of the latency of
+// shuffles through LDS.  Lanes without a source add 0.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int old, int v) {
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved64(u64 v) {
+  const unsigned lo = (unsigned)moved<CTRL, ROWS>(0, (int)(unsigned)v), hi = (unsigned)moved<CTRL, ROWS>(0, (int)(v >> 32));
+  return ((u64)hi << 32) | lo;
 }
 // inclusive prefix over the lanes
-__device__ __forceinline__ u64 wave_scan64(u64 v, int lane) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 t = __shfl_up(v, o, 64);
-    if (lane >= o) v += t;
-  }
+__device__ __forceinline__ u64 wave_scan64(u64 v) {
+  v += moved64<0x111, 0xf>(v);
+  v += moved64<0x112, 0xf>(v);
+  v += moved64<0x114, 0xf>(v);
+  v += moved64<0x118, 0xf>(v);
+  v += moved64<0x142, 0xa>(v);
+  v += moved64<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ int wave_scan32(int v) {
+  v += moved<0x111, 0xf>(0, v);
+  v += moved<0x112, 0xf>(0, v);
+  v += moved<0x114, 0xf>(0, v);
+  v += moved<0x118, 0xf>(0, v);
+  v += moved<0x142, 0xa>(0, v);
+  v += moved<0x143, 0xc>(0, v);
+  return v;
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+  v = wave_scan64(v);
+  const unsigned lo = (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63);
+  return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), 63) << 32) | lo;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved_max(float v) {
+  const int i = __float_as_int(v);
+  return fmaxf(v, __int_as_float(moved<CTRL, ROWS>(i, i)));
+}
+__device__ __forceinline__ float wave_peak(float v) {
+  v = moved_max<0x111, 0xf>(v);
+  v = moved_max<0x112, 0xf>(v);
+  v = moved_max<0x114, 0xf>(v);
+  v = moved_max<0x118, 0xf>(v);
+  v = moved_max<0x142, 0xa>(v);
+  v = moved_max<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
 // 8 logits from index i; -inf past the row's end and for NaN.  Rows of odd lengths start at odd addresses: the copy
@@ -80,10 +115,49 @@ __device__ __forceinline__ double weight(const Row& r, float x) {
 }
 __device__ __forceinline__ u64 fixed(const Row& r, double w) { return (u64)(w * r.unit + 0.5); }
 
+// f(chunk, x) for those of the chunks c, c + step, c + 2 step .. < c1 that want(chunk) names, by one wave.  want is asked
+// by a lane per chunk; the loads of four chunks are in flight before the first is worked on (one at a time, the latency of
+// each was most of the time).
+template <typename T, typename Want, typename F>
+__device__ __forceinline__ void walk(const T* __restrict__ row, int V, int c, int c1, int step, Want want, F f) {
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int N = 4, Q = sizeof(T) / 2;   // 16-byte loads per lane and chunk
+  const int lane = threadIdx.x & 63;
+  for (; c < c1; c += 64 * step) {
+    u64 todo = __ballot(c + lane * step < c1 && want(c + lane * step));
+    while (todo) {
+      u32x4 raw[N][Q];
+      int at[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        at[n] = todo ? c + (__ffsll((long long)todo) - 1) * step : -1;
+        todo &= todo - 1;
+        if (at[n] >= 0 && (at[n] + 1) * kChunk <= V) __builtin_memcpy(raw[n], row + (long)at[n] * kChunk + lane * 8, 16 * Q);
+      }
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        if (at[n] < 0) break;
+        float x[8];
+        if ((at[n] + 1) * kChunk <= V) {
+          T t[8];
+          __builtin_memcpy(t, raw[n], sizeof(t));
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            x[j] = Elt<T>::ld(t + j);
+            x[j] = x[j] != x[j] ? -INFINITY : x[j];
+          }
+        } else {
+          load8(row, at[n] * kChunk + lane * 8, V, x);
+        }
+        f(at[n], x);
+      }
+    }
+  }
+}
+
 struct Setting {
   const float* p;   // one value per row, or null
   float v;
-  __device__ __forceinline__ float of(int b) const { return p ? p[b] : v; }
 };
 
 // Everything a launch needs; settings per row (pointers) or for all rows.
@@ -91,7 +165,7 @@ template <typename T>
 struct Args {
   const T* logits;
   long stride;
-  int V, chunks, groups, shift;
+  int V, chunks, groups, group_lanes, shift;   // a group: group_lanes x 8 logits
   const float* uniform;
   Setting temp, top_p, min_p;
   const int* top_ks;
@@ -102,19 +176,35 @@ struct Args {
   int* listed;     // [B] how many
   float* peaks;    // [B][groups] largest logit of a group
   int64_t* out;
-  __device__ __forceinline__ int k_of(int b) const {   // 0: off
-    const int k = top_ks ? top_ks[b] : top_k;
-    return k > 0 && k < V ? k : 0;
-  }
 };
+
+// a row's settings: loaded together, whichever of them are tensors (the others load their number's place holder)
+struct Of {
+  float t, p, m, u;
+  int k;   // 0: off
+};
+template <typename T>
+__device__ __forceinline__ Of row_of(const Args<T>& a, int b) {
+  const float u = a.uniform[b];
+  const float t = (a.temp.p ? a.temp.p : a.uniform)[b], p = (a.top_p.p ? a.top_p.p : a.uniform)[b];
+  const float m = (a.min_p.p ? a.min_p.p : a.uniform)[b];
+  const int k = (a.top_ks ? a.top_ks : reinterpret_cast<const int*>(a.uniform))[b];
+  Of r;
+  r.u = u;
+  r.t = a.temp.p ? t : a.temp.v;
+  r.p = a.top_p.p ? p : a.top_p.v;
+  r.m = a.min_p.p ? m : a.min_p.v;
+  r.k = a.top_ks ? k : a.top_k;
+  if (r.k <= 0 || r.k >= a.V) r.k = 0;
+  return r;
+}
 enum Kind { kGreedy, kPlain, kTopP, kShortK, kFromStart };
 template <typename T>
-__device__ __forceinline__ Kind kind_of(const Args<T>& a, int b, float top) {
-  if (!(a.temp.of(b) > 0.f) || top == -INFINITY) return kGreedy;
-  if (top == INFINITY || !(a.uniform[b] >= 9.094947e-13f)) return kFromStart;   // 2^-40
-  const int k = a.k_of(b);
-  if (k) return k <= a.groups / 2 && k <= kMaxK ? kShortK : kFromStart;
-  return a.top_p.of(b) < 1.f ? kTopP : kPlain;
+__device__ __forceinline__ Kind kind_of(const Args<T>& a, const Of& r, float top) {
+  if (!(r.t > 0.f) || top == -INFINITY) return kGreedy;
+  if (top == INFINITY || !(r.u >= 9.094947e-13f)) return kFromStart;   // 2^-40
+  if (r.k) return r.k <= a.groups / 2 && r.k <= kMaxK ? kShortK : kFromStart;
+  return r.p < 1.f ? kTopP : kPlain;
 }
 // least mass that top-p keeps of z
 __device__ __forceinline__ u64 share_of(float p, u64 z) {
@@ -122,23 +212,39 @@ __device__ __forceinline__ u64 share_of(float p, u64 z) {
   return n < 1 ? (u64)1 : n > z ? z : n;
 }
 
-// 2^y as an integer of 2^-shift, y = (x - top) / (T ln 2) <= 0: y = k / 256 + r, 2^(k / 256) from a table of 2^(j / 256),
-// 2^r by its series to r^4 (|r| <= 2^-9: 4e-17 off).  Adding 1.5 * 2^44 leaves k in the low word of the sum.
+// p * r + c with c left in its registers: the compiler's choice, the two-operand form, copies c first, a third more
+// instructions over the series below
+__device__ __forceinline__ double horner(double p, double r, double c) {
+  double d;
+  asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(p), "v"(r), "v"(c));
+  return d;
+}
+
+// 2^y as an integer of 2^-shift, y = (x - top) / (T ln 2) <= 0: y = k + r, |r| <= 1/2, 2^r by its series to r^10 (2e-13
+// off; tables of 2^(j / 256) in LDS took longer: their random reads share one pipe).  Adding 1.5 * 2^52 leaves k in the
+// low word of the sum.
 struct Weigher {
   float top;
-  double scale;         // 1 / (T ln 2)
-  float bin_scale;      // bins per unit of x
+  double scale;      // 1 / (T ln 2)
+  float bin_scale;   // bins per unit of x
   int shift;
-  const double* table;  // 2^(j / 256) in LDS
   __device__ __forceinline__ u64 operator()(float x) const {
-    const double y = ((double)x - (double)top) * scale;
-    if (!(y > -(double)(shift + 2))) return 0;   // also -inf
-    const double magic = 26388279066624.0, t = y + magic;
+    const double y0 = ((double)x - (double)top) * scale, y = fmax(y0, -64.0);   // below: 2^(50 - 64) rounds to 0
+    const double magic = 6755399441055744.0, t = y + magic;
     const int k = (int)(unsigned)__double_as_longlong(t);
     const double r = y - (t - magic);
-    const double p = fma(fma(fma(fma(0.009618129107628477, r, 0.055504108664821580), r, 0.24022650695910072), r,
-                             0.69314718055994531), r, 1.0);
-    const double w = ldexp(p * table[k & (kTable - 1)], (k >> 8) + shift);
+    double p = 7.0549116208011e-09;              // (ln 2)^n / n!, n = 10 .. 0
+    p = horner(p, r, 1.01780860092397e-07);
+    p = horner(p, r, 1.32154867901443e-06);
+    p = horner(p, r, 1.5252733804059840e-05);
+    p = horner(p, r, 1.5403530393381608e-04);
+    p = horner(p, r, 1.3333558146428443e-03);
+    p = horner(p, r, 9.6181291076284772e-03);
+    p = horner(p, r, 5.5504108664821580e-02);
+    p = horner(p, r, 2.4022650695910071e-01);
+    p = horner(p, r, 6.9314718055994531e-01);
+    p = fma(p, r, 1.0);
+    const double w = ldexp(p, k + shift);
     return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;   // w <= 2^50: rounded to an integer
   }
   // bin of a logit, not decreasing as x falls; the last one holds all the rest.  wide_bin: twice as wide, so that the
@@ -148,16 +254,12 @@ struct Weigher {
     return (int)fminf((top - x) * bin_scale * 0.5f, (float)(kBins - 1));
   }
 };
-__device__ __forceinline__ void fill_table(double* table) {
-  for (int j = threadIdx.x; j < kTable; j += blockDim.x) table[j] = exp2((double)j / kTable);
-}
-__device__ __forceinline__ Weigher weigher(float top, float t, int shift, const double* table) {
+__device__ __forceinline__ Weigher weigher(float top, float t, int shift) {
   Weigher w;
   w.top = top;
   w.scale = 1.4426950408889634 / (double)t;
   w.bin_scale = (float)fmin(w.scale * 64.0, 3e38);
   w.shift = shift;
-  w.table = table;
   return w;
 }
 // least weight that min-p keeps
@@ -172,40 +274,49 @@ __global__ __launch_bounds__(256) void peaks_kernel(Args<T> a) {
   const int b = blockIdx.y, lane = threadIdx.x & 63;
   const T* row = a.logits + (long)b * a.stride;
   const int per = (a.chunks + gridDim.x - 1) / gridDim.x, c0 = blockIdx.x * per, c1 = min(a.chunks, c0 + per);
-  for (int c = c0 + (threadIdx.x >> 6); c < c1; c += 4) {
-    float x[8];
-    load8(row, c * kChunk + lane * 8, a.V, x);
+  const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  walk(row, a.V, c0 + wv, c1, 4, [](int) { return true; }, [&](int c, const float (&x)[8]) {
     float m = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) m = fmaxf(m, x[j]);
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-    const int g = c * (kChunk / kGroup) + (lane >> 4);
-    if ((lane & 15) == 0 && g < a.groups) a.peaks[(long)b * a.groups + g] = m;
-  }
+    // the last lane of a group gets its largest (groups of 4 lanes or of a row of 16)
+    m = moved_max<0x111, 0xf>(m);
+    m = moved_max<0x112, 0xf>(m);
+    if (a.group_lanes == 16) {
+      m = moved_max<0x114, 0xf>(m);
+      m = moved_max<0x118, 0xf>(m);
+    }
+    const int g = (c * 64 + lane) / a.group_lanes;
+    if ((lane & (a.group_lanes - 1)) == a.group_lanes - 1 && g < a.groups) a.peaks[(long)b * a.groups + g] = m;
+  });
   for (int i = blockIdx.x * 256 + threadIdx.x; i < kBins; i += gridDim.x * 256) a.hist[(long)b * kBins + i] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) a.listed[b] = 0;
 }
 
 // the row's largest logit, from its groups', for every thread
+template <int WAVES>
 __device__ __forceinline__ float row_peak(const float* peaks, int groups, float* red) {
   float m = -INFINITY;
-  for (int g = threadIdx.x; g < groups; g += blockDim.x) m = fmaxf(m, peaks[g]);
-  m = wave_max(m);
+  for (int g = threadIdx.x; g < groups; g += WAVES * 64) m = fmaxf(m, peaks[g]);
+  m = wave_peak(m);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
   __syncthreads();
   m = red[0];
-  for (int i = 1; i < (int)blockDim.x / 64; ++i) m = fmaxf(m, red[i]);
+#pragma unroll
+  for (int i = 1; i < WAVES; ++i) m = fmaxf(m, red[i]);
   return m;
 }
-__device__ __forceinline__ float chunk_peak(const float* peaks, int c, int groups) {
+// the largest logit of a chunk, by one lane
+__device__ __forceinline__ float chunk_peak(const float* peaks, int c, int groups, int group_lanes) {
+  const int n = 64 / group_lanes, g0 = c * n;
   float m = -INFINITY;
+  for (int i = 0; i < n; i += 4)
 #pragma unroll
-  for (int g = 0; g < kChunk / kGroup; ++g) m = fmaxf(m, peaks[min(c * (kChunk / kGroup) + g, groups - 1)]);
+    for (int j = 0; j < 4; ++j) m = fmaxf(m, peaks[min(g0 + i + j, groups - 1)]);
   return m;
 }
 
-// sum of v over the workgroup, for every thread; WAVES of it
+// sum of v over the workgroup, for every thread
 template <int WAVES>
 __device__ __forceinline__ u64 group_sum(u64 v, u64* red) {
   v = wave_sum64(v);
@@ -218,81 +329,87 @@ __device__ __forceinline__ u64 group_sum(u64 v, u64* red) {
   return s;
 }
 
-// The first of n <= WAVES * 64 * 8 entries (in LDS, or global memory) at which the running sum passes `want`, and the sum
-// before it, in found[0], found[1]; the last entry where none does.  All threads take part.
-template <int WAVES>
-__device__ __forceinline__ void group_find(const u64* v, int n, u64 want, u64* red, u64* found) {
+// The first of n <= WAVES * 64 * PER entries (in LDS or global memory) at which the running sum passes want(total), the sum
+// before it, and want, in found[0 .. 2]; the last entry where none does.  All threads take part.
+template <int WAVES, int PER, typename Want>
+__device__ __forceinline__ void group_find(const u64* v, int n, u64* red, u64* found, Want want_of) {
   const int per = (n + WAVES * 64 - 1) / (WAVES * 64), i0 = threadIdx.x * per;
-  u64 x[8], s = 0;
+  u64 x[PER], s = 0;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
+  for (int j = 0; j < PER; ++j) {
     x[j] = j < per && i0 + j < n ? v[i0 + j] : 0;
     s += x[j];
   }
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-  u64 cum = wave_scan64(s, lane);
+  const int wv = threadIdx.x >> 6;
+  u64 cum = wave_scan64(s);
   __syncthreads();
-  if (lane == 63) red[wv] = cum;
-  if (threadIdx.x == 0) {
-    found[0] = n - 1;
-    found[1] = 0;
-  }
+  if ((threadIdx.x & 63) == 63) red[wv] = cum;
   __syncthreads();
+  u64 total = 0;
   cum -= s;
-  for (int i = 0; i < wv; ++i) cum += red[i];
-  if (cum <= want && want < cum + s) {
-    int at = -1;
-    u64 before = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (at < 0 && cum + x[j] > want) {
+  for (int i = 0; i < WAVES; ++i) {
+    cum += i < wv ? red[i] : 0;
+    total += red[i];
+  }
+  const u64 want = want_of(total);
+  if (want >= total ? threadIdx.x == 0 : cum <= want && want < cum + s) {
+    int at = n - 1;
+    u64 before = 0;
+    bool open = want < total;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      if (open && cum + x[j] > want) {
         at = i0 + j;
         before = cum;
+        open = false;
       }
       cum += x[j];
     }
     found[0] = at;
     found[1] = before;
+    found[2] = want;
   }
   __syncthreads();
 }
 
-// grid (slices, B), 256 threads
+// grid (slices, B).  Wide workgroups: every one adds its bins to the row's in global memory
 template <typename T>
-__global__ __launch_bounds__(256) void bins_kernel(Args<T> a) {
-  __shared__ u64 hist[kBins], red[4];
-  __shared__ double table[kTable];
-  __shared__ float redf[4];
+__global__ __launch_bounds__(kWide * 64) void bins_kernel(Args<T> a) {
+  __shared__ u64 hist[kBins], red[kWide];
+  __shared__ float redf[kWide];
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  if (!(a.temp.of(b) > 0.f) || a.k_of(b)) return;
+  const Of of = row_of(a, b);
+  if (!(of.t > 0.f) || of.k) return;
   const float* peaks = a.peaks + (long)b * a.groups;
-  fill_table(table);
-  for (int i = tid; i < kBins; i += 256) hist[i] = 0;
-  const float top = row_peak(peaks, a.groups, redf);   // (its barrier also publishes hist and table)
-  const Kind kind = kind_of(a, b, top);
+  if (of.p < 1.f)
+    for (int i = tid; i < kBins; i += kWide * 64) hist[i] = 0;
+  const float top = row_peak<kWide>(peaks, a.groups, redf);   // (its barrier also publishes hist)
+  const Kind kind = kind_of(a, of, top);
   if (kind != kPlain && kind != kTopP) return;
-  const Weigher weigh = weigher(top, a.temp.of(b), a.shift, table);
-  const u64 least = least_weight(a.min_p.of(b), a.shift);
+  const Weigher weigh = weigher(top, of.t, a.shift);
+  const u64 least = least_weight(of.m, a.shift);
   const T* row = a.logits + (long)b * a.stride;
   const int per = (a.chunks + gridDim.x - 1) / gridDim.x, c0 = blockIdx.x * per, c1 = min(a.chunks, c0 + per);
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   u64 tail = 0;
-  for (int c = c0 + (tid >> 6); c < c1; c += 4) {
-    const u64 most = weigh(chunk_peak(peaks, c, a.groups));
-    float x[8];
+  auto weighs = [&](int c) {   // (a chunk that does not: its mass is 0)
+    const u64 most = weigh(chunk_peak(peaks, c, a.groups, a.group_lanes));
+    const bool yes = most > 0 && (kind != kPlain || most >= least);
+    if (!yes && kind == kPlain) a.mass[(long)b * a.chunks + c] = 0;
+    return yes;
+  };
+  walk(row, a.V, c0 + wv, c1, kWide, weighs, [&](int c, const float (&x)[8]) {
     if (kind == kPlain) {
       u64 s = 0;
-      if (most > 0 && most >= least) {
-        load8(row, c * kChunk + lane * 8, a.V, x);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const u64 w = weigh(x[j]);
-          s += w >= least ? w : 0;
-        }
-        s = wave_sum64(s);
+      for (int j = 0; j < 8; ++j) {
+        const u64 w = weigh(x[j]);
+        s += w >= least ? w : 0;
       }
+      s = wave_sum64(s);
       if (lane == 0) a.mass[(long)b * a.chunks + c] = s;
-    } else if (most > 0) {
-      load8(row, c * kChunk + lane * 8, a.V, x);
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int n = weigh.bin(x[j]);
@@ -301,95 +418,86 @@ __global__ __launch_bounds__(256) void bins_kernel(Args<T> a) {
         else tail += w;
       }
     }
-  }
+  });
   if (kind == kPlain) return;
-  tail = group_sum<4>(tail, red);
+  tail = group_sum<kWide>(tail, red);
   if (tid == 0) hist[kBins - 1] = tail;
   __syncthreads();
-  for (int i = tid; i < kBins; i += 256)
+  for (int i = tid; i < kBins; i += kWide * 64)
     if (hist[i]) atomicAdd(&a.hist[(long)b * kBins + i], hist[i]);   // integers: any order gives the same sums
 }
 
-// What top-p alone keeps of a row: its share of the mass, the border's bin and the mass before it; false: the tail.
+// The bin of the border of what top-p alone keeps of a row, and the mass it keeps of that bin; false: in the tail.
 template <int WAVES>
 __device__ __forceinline__ bool border_bin(const u64* hist, float p, u64* red, u64* found, int& bin, u64& left) {
-  u64 z = 0;
-  for (int i = threadIdx.x; i < kBins; i += WAVES * 64) z += hist[i];
-  const u64 need = share_of(p, group_sum<WAVES>(z, red));
-  group_find<WAVES>(hist, kBins, need - 1, red, found);
+  group_find<WAVES, kBins / 64 / WAVES>(hist, kBins, red, found, [&](u64 z) { return share_of(p, z) - 1; });
   bin = (int)found[0];
-  left = need - found[1];
-  __syncthreads();
+  left = found[2] + 1 - found[1];
   return bin < kBins - 1;
 }
 
-// grid (slices, B), 256 threads; rows of top-p alone
+// grid (slices, B); rows of top-p alone
 template <typename T>
-__global__ __launch_bounds__(256) void sweep_kernel(Args<T> a) {
-  __shared__ u64 red[4], found[2];
-  __shared__ double table[kTable];
-  __shared__ float redf[4];
+__global__ __launch_bounds__(kWide * 64) void sweep_kernel(Args<T> a) {
+  constexpr int kPart = 4096;
+  __shared__ u64 red[kWide], found[3], list[kPart];
+  __shared__ float redf[kWide];
+  __shared__ int listed, place;
   const int b = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  if (!(a.temp.of(b) > 0.f) || a.k_of(b) || !(a.top_p.of(b) < 1.f)) return;
+  const Of of = row_of(a, b);
+  if (!(of.t > 0.f) || of.k || !(of.p < 1.f)) return;
+  if (tid == 0) listed = 0;
   const float* peaks = a.peaks + (long)b * a.groups;
-  fill_table(table);
-  const float top = row_peak(peaks, a.groups, redf);
-  if (kind_of(a, b, top) != kTopP) return;
+  const float top = row_peak<kWide>(peaks, a.groups, redf);
+  if (kind_of(a, of, top) != kTopP) return;
   int bin;
   u64 left;
-  if (!border_bin<4>(a.hist + (long)b * kBins, a.top_p.of(b), red, found, bin, left)) return;
-  const Weigher weigh = weigher(top, a.temp.of(b), a.shift, table);
-  const u64 least = least_weight(a.min_p.of(b), a.shift);
+  if (!border_bin<kWide>(a.hist + (long)b * kBins, of.p, red, found, bin, left)) return;
+  const Weigher weigh = weigher(top, of.t, a.shift);
+  const u64 least = least_weight(of.m, a.shift);
   const T* row = a.logits + (long)b * a.stride;
   const int per = (a.chunks + gridDim.x - 1) / gridDim.x, c0 = blockIdx.x * per, c1 = min(a.chunks, c0 + per);
-  for (int c = c0 + (tid >> 6); c < c1; c += 4) {
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto reaches = [&](int c) {
+    const bool yes = weigh.bin(chunk_peak(peaks, c, a.groups, a.group_lanes)) <= bin;
+    if (!yes) a.mass[(long)b * a.chunks + c] = 0;
+    return yes;
+  };
+  walk(row, a.V, c0 + wv, c1, kWide, reaches, [&](int c, const float (&x)[8]) {
     u64 s = 0;
-    if (weigh.bin(chunk_peak(peaks, c, a.groups)) <= bin) {
-      float x[8];
-      const int i = c * kChunk + lane * 8;
-      load8(row, i, a.V, x);
-      int mine = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int n = weigh.bin(x[j]);
-        if (n < bin) {
-          const u64 w = weigh(x[j]);
-          s += w >= least ? w : 0;
-        }
-        mine += n == bin;
-      }
-      s = wave_sum64(s);
-      if (__any(mine)) {   // room in the list for the whole wave at once
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-          const int t = __shfl_up(upto, o, 64);
-          if (lane >= o) upto += t;
-        }
-        int at = 0;
-        if (lane == 63) at = atomicAdd(&a.listed[b], upto);
-        at = __shfl(at, 63, 64) + upto - mine;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (weigh.bin(x[j]) == bin) {
-            if (at < kList) a.list[(long)b * kList + at] = ((u64)key_of(x[j]) << 32) | (unsigned)(i + j);
-            ++at;
-          }
+    for (int j = 0; j < 8; ++j) {
+      const int n = weigh.bin(x[j]);
+      if (n < bin) {
+        const u64 w = weigh(x[j]);
+        s += w >= least ? w : 0;
+      } else if (n == bin) {
+        const int at = atomicAdd(&listed, 1);
+        if (at < kPart) list[at] = ((u64)key_of(x[j]) << 32) | (unsigned)(c * kChunk + lane * 8 + j);
       }
     }
+    s = wave_sum64(s);
     if (lane == 0) a.mass[(long)b * a.chunks + c] = s;
-  }
+  });
+  // this workgroup's part of the list, in one piece; too long a one makes the row's count too long as well
+  __syncthreads();
+  const int n = listed;
+  if (n == 0) return;
+  if (tid == 0) place = atomicAdd(&a.listed[b], n <= kPart ? n : kList + 1);
+  __syncthreads();
+  if (n > kPart) return;
+  for (int i = tid; i < n; i += kWide * 64)
+    if (place + i < kList) a.list[(long)b * kList + place + i] = list[i];
 }
 
 struct Shared {   // of choose_kernel
-  u64 red[kWaves], found[4], part[kMaxChunks], hist[kBins], list[kList], weight[kShort];
-  double table[kTable];
+  u64 red[16], found[4], part[kMaxChunks], hist[kBins], list[kList], weight[kShort];
   int listed;
 };
 
 // ---- a row from the start, by radix selection
-template <typename T>
-__device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
+template <int kWaves, typename T>
+__device__ void choose_from_start(const Args<T>& a, const Of& of, int b, Shared& sh) {
   const int V = a.V;
   u64 *const red = sh.red, *const hist = sh.hist, *const part = sh.part, *const found = sh.found;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -420,7 +528,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
   for (int i = 0; i < kWaves; ++i) best = red[i] > best ? red[i] : best;
   Row r;
   r.top = value_of((unsigned)(best >> 32));
-  const float t = a.temp.of(b);
+  const float t = of.t;
   if (!(t > 0.f) || r.top == -INFINITY) {   // greedy; a row with no allowed token gives 0
     if (tid == 0) a.out[b] = (unsigned)~(unsigned)best;
     return;
@@ -435,7 +543,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
     unsigned prefix = 0;
     for (int sh = 24; sh >= 0; sh -= 8) {
       __syncthreads();
-      if (tid < 256) hist[tid] = 0;
+      for (int i = tid; i < 256; i += kWaves * 64) hist[i] = 0;
       __syncthreads();
       const unsigned himask = sh == 24 ? 0u : ~0u << (sh + 8);
       for (int c = wv; c < chunks; c += kWaves) {
@@ -457,7 +565,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
           h[j] = hist[255 - (lane * 4 + j)];
           s += h[j];
         }
-        const u64 incl = wave_scan64(s, lane);
+        const u64 incl = wave_scan64(s);
         const u64 hit = __ballot(incl >= need);
         const int first = hit ? __ffsll((long long)hit) - 1 : 63;
         if (lane == first) {
@@ -495,9 +603,9 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
     if (same > ties) same = ties;
     return s + (same ? same * fixed(r, weight(r, value_of(kmin))) : 0);
   };
-  const int k = a.k_of(b);
+  const int k = of.k;
   if (k) ties = select(false, (u64)k);
-  const float p = a.top_p.of(b);
+  const float p = of.p;
   if (p < 1.f) {
     const u64 z = kept_mass();
     u64 need = (u64)ceil(fmax((double)p, 0.0) * (double)z);
@@ -522,7 +630,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
     }
     __syncthreads();
     // the chunk that holds tie number `ties` (counted from 1), then the element
-    group_find<kWaves>(part, chunks, ties - 1, red, found);
+    group_find<kWaves, kMaxChunks / 64 / kWaves>(part, chunks, red, found, [&](u64) { return ties - 1; });
     const int at = (int)found[0];
     const u64 before = found[1];
     __syncthreads();
@@ -535,7 +643,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
         u64 same = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) same += i + j < V && key_of(x[j]) == kmin;
-        u64 n = before + wave_scan64(same, lane) - same;
+        u64 n = before + wave_scan64(same) - same;
         if (n < ties && n + same >= ties) {
           int at_j = 0;
 #pragma unroll
@@ -551,7 +659,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
   }
   // ---- kept mass per chunk, then the chunk, lane and element where the cumulative mass passes u * total
   // A number below 2^-40 draws the first kept token of any weight above 0, also one that is below the integers' unit.
-  const float mp = a.min_p.of(b), uf = a.uniform[b];
+  const float mp = of.m, uf = of.u;
   const bool first_kept = !(uf >= 9.094947e-13f);
   auto kept = [&](float x, int i) -> u64 {
     const unsigned ky = key_of(x);
@@ -575,7 +683,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
   const u64 total = group_sum<kWaves>(mine, red);
   u64 want = first_kept ? 0 : (u64)fmin((double)uf * (double)total, 9.0e18);
   if (want >= total) want = total - 1;
-  group_find<kWaves>(part, chunks, want, red, found);
+  group_find<kWaves, kMaxChunks / 64 / kWaves>(part, chunks, red, found, [&](u64) { return want; });
   if (wv == 0) {
     const int at = (int)found[0];
     const u64 before = found[1];
@@ -588,7 +696,7 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
       w[j] = kept(x[j], i + j);
       s += w[j];
     }
-    u64 cum = before + wave_scan64(s, lane) - s;
+    u64 cum = before + wave_scan64(s) - s;
     if (cum <= want && want < cum + s) {
       int token = i;
       bool open = true;
@@ -608,9 +716,10 @@ __device__ void choose_from_start(const Args<T>& a, int b, Shared& sh) {
 // Where the border lies among n <= kList listed logits (key << 32 | index, in any order; LDS): the entry at which those
 // before it in the order (larger key, then smaller index) hold less than `left` of the mass, and with it `left` or more.
 // The entries before it go to `keep(entry, weight)`.  The list is used up.
-template <typename Keep>
+template <int kWaves, typename Keep>
 __device__ __forceinline__ u64 resolve(Shared& sh, int n, u64 left, const Weigher& weigh, Keep keep) {
   constexpr u64 kFlip = 0xffffffffull;   // index reversed: the order is then that of falling numbers
+  constexpr int kThreads = kWaves * 64;
   const int tid = threadIdx.x;
   while (n > 256) {   // narrow down by the highest ten bits that differ
     u64 lo = ~0ull, hi = 0, e[kList / kThreads];
@@ -634,7 +743,7 @@ __device__ __forceinline__ u64 resolve(Shared& sh, int n, u64 left, const Weighe
       sh.red[tid >> 6] = lo;
       sh.hist[1024 + (tid >> 6)] = hi;
     }
-    if (tid < 1024) sh.hist[tid] = 0;
+    for (int i = tid; i < 1024; i += kThreads) sh.hist[i] = 0;
     if (tid == 0) sh.listed = 0;
     __syncthreads();
 #pragma unroll
@@ -653,7 +762,7 @@ __device__ __forceinline__ u64 resolve(Shared& sh, int n, u64 left, const Weighe
       }
     }
     __syncthreads();
-    group_find<kWaves>(sh.hist, 1024, left - 1, sh.red, sh.found);
+    group_find<kWaves, 1024 / 64 / kWaves>(sh.hist, 1024, sh.red, sh.found, [&](u64) { return left - 1; });
     const int digit = 1023 - (int)sh.found[0];
     left -= sh.found[1];
 #pragma unroll
@@ -674,25 +783,26 @@ __device__ __forceinline__ u64 resolve(Shared& sh, int n, u64 left, const Weighe
     u64 before = 0;
     for (int i = 0; i < n; ++i) before += (sh.list[i] ^ kFlip) > (mine ^ kFlip) ? sh.weight[i] : 0;
     if (before < left) {
-      if (before + w >= left) sh.found[2] = mine;
+      if (before + w >= left) sh.found[3] = mine;
       else keep(mine, w);
     }
   }
   __syncthreads();
-  return sh.found[2];
+  return sh.found[3];
 }
 
 // grid B, one row each
-template <typename T>
-__global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
+template <typename T, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
+  constexpr int kThreads = kWaves * 64;
   __shared__ Shared sh;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, V = a.V, chunks = a.chunks;
   const T* row = a.logits + (long)b * a.stride;
   const float* peaks = a.peaks + (long)b * a.groups;
-  fill_table(sh.table);
+  const Of of = row_of(a, b);
   if (tid == 0) sh.listed = 0;
-  const float top = row_peak(peaks, a.groups, reinterpret_cast<float*>(sh.red));
-  const Kind kind = kind_of(a, b, top);
+  const float top = row_peak<kWaves>(peaks, a.groups, reinterpret_cast<float*>(sh.red));
+  const Kind kind = kind_of(a, of, top);
   if (kind == kGreedy) {   // the lowest index of the largest logit; 0 where no token is allowed
     int g = a.groups;
     for (int i = tid; i < a.groups; i += kThreads)
@@ -709,37 +819,35 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) g = min(g, __shfl_xor(g, o, 64));
       float x[8];
-      const int i = g * kGroup + (lane & 15) * 8;
+      const int i = g * a.group_lanes * 8 + (lane & (a.group_lanes - 1)) * 8;
       load8(row, i, V, x);
       int first = 8;
 #pragma unroll
       for (int j = 7; j >= 0; --j) first = x[j] == top ? j : first;
-      const u64 hit = __ballot(first < 8 && lane < 16);
+      const u64 hit = __ballot(first < 8 && lane < a.group_lanes);
       if (lane == (hit ? __ffsll((long long)hit) - 1 : 0)) a.out[b] = hit && top > -INFINITY ? i + first : 0;
     }
     return;
   }
   if (kind == kFromStart) {
-    choose_from_start(a, b, sh);
+    choose_from_start<kWaves>(a, of, b, sh);
     return;
   }
-  const float uf = a.uniform[b];
-  const Weigher weigh = weigher(top, a.temp.of(b), a.shift, sh.table);
-  const u64 least = least_weight(a.min_p.of(b), a.shift);
+  const Weigher weigh = weigher(top, of.t, a.shift);
+  const u64 least = least_weight(of.m, a.shift);
   auto target = [&](u64 total) {
-    const u64 want = (u64)fmin((double)uf * (double)total, 9.0e18);
+    const u64 want = (u64)fmin((double)of.u * (double)total, 9.0e18);
     return want >= total ? total - 1 : want;
   };
   if (kind == kShortK) {
     // the bound: the first bin at which k groups have their largest logit (or all that weighs anything)
-    const int k = a.k_of(b);
     for (int i = tid; i < kBins; i += kThreads) sh.hist[i] = 0;
     __syncthreads();
     for (int g = tid; g < a.groups; g += kThreads) atomicAdd(&sh.hist[weigh.wide_bin(peaks[g])], 1ull);
     __syncthreads();
-    group_find<kWaves>(sh.hist, kBins, (u64)k - 1, sh.red, sh.found);
+    group_find<kWaves, kBins / 64 / kWaves>(sh.hist, kBins, sh.red, sh.found, [&](u64) { return (u64)of.k - 1; });
     const int bound = min((int)sh.found[0], kBins - 2);
-    // the groups at or above it, then their logits at or above it; 16 lanes take a group
+    // the groups at or above it, then their logits at or above it; group_lanes lanes take a group
     int* groups = reinterpret_cast<int*>(sh.hist);
     __syncthreads();
     for (int g = tid; g < a.groups; g += kThreads)
@@ -753,9 +861,9 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
     if (tid == 0) sh.listed = 0;
     __syncthreads();
     const bool ok = n_groups <= 2 * kBins;
-    for (int at = tid >> 4; ok && at < n_groups; at += kThreads / 16) {
+    for (int at = tid / a.group_lanes; ok && at < n_groups; at += kThreads / a.group_lanes) {
       float x[8];
-      const int i = groups[at] * kGroup + (tid & 15) * 8;
+      const int i = (groups[at] * a.group_lanes + (tid & (a.group_lanes - 1))) * 8;
       load8(row, i, V, x);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -768,35 +876,61 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
     const int n = sh.listed;
     if (!ok || n > kShort) {
       __syncthreads();
-      choose_from_start(a, b, sh);
+      choose_from_start<kWaves>(a, of, b, sh);
       return;
     }
-    u64 mine = 0, w = 0, before = 0;
-    int rank = 0;
-    if (tid < n) {
-      mine = sh.list[tid] ^ 0xffffffffull;
-      w = weigh(value_of((unsigned)(mine >> 32)));
-      sh.weight[tid] = w;
-    }
+    // All against all, `parts` threads to an entry where there are fewer entries than threads: rank and mass before it,
+    // then the kept mass at smaller indexes
+    constexpr u64 kFlip = 0xffffffffull;
+    u64 *const before = sh.part, *const weight = sh.weight;
+    int* const rank = reinterpret_cast<int*>(sh.hist);
+    int step = 64;
+    while (step < n && step < kThreads) step *= 2;
+    const int part = tid / step, parts = kThreads / step, first = tid & (step - 1);
     __syncthreads();
-    if (tid < n)
-      for (int i = 0; i < n; ++i) {
-        const bool ahead = (sh.list[i] ^ 0xffffffffull) > mine;
-        rank += ahead;
-        before += ahead ? sh.weight[i] : 0;
+    for (int at = tid; at < kShort; at += kThreads) {
+      if (at < n) {
+        sh.list[at] ^= kFlip;
+        weight[at] = weigh(value_of((unsigned)(sh.list[at] >> 32)));
       }
-    bool kept = tid < n && rank < k;
-    const u64 z = group_sum<kWaves>(kept ? w : 0, sh.red);
-    const float p = a.top_p.of(b);
-    kept = kept && !(p < 1.f && before >= share_of(p, z)) && w >= least;
-    const u64 want = target(group_sum<kWaves>(kept ? w : 0, sh.red));
-    if (tid < n) sh.weight[tid] = kept ? w : 0;
-    __syncthreads();
-    if (kept) {
-      u64 c = 0;
-      for (int i = 0; i < n; ++i) c += (unsigned)sh.list[i] < ~(unsigned)mine ? sh.weight[i] : 0;
-      if (c <= want && want < c + w) a.out[b] = (int64_t)(unsigned)~(unsigned)mine;
+      before[at] = 0, rank[at] = 0;
     }
+    __syncthreads();
+    for (int at = first; at < n; at += step) {
+      const u64 mine = sh.list[at];
+      u64 sum = 0;
+      int ahead = 0;
+#pragma unroll 4
+      for (int i = part; i < n; i += parts) {
+        const bool is = sh.list[i] > mine;
+        ahead += is;
+        sum += is ? weight[i] : 0;
+      }
+      if (parts == 1) before[at] = sum, rank[at] = ahead;
+      else if (ahead) atomicAdd(&before[at], sum), atomicAdd(&rank[at], ahead);
+    }
+    __syncthreads();
+    u64 in_k = 0, in_all = 0;
+    for (int at = tid; at < n; at += kThreads) in_k += rank[at] < of.k ? weight[at] : 0;
+    const u64 share = of.p < 1.f ? share_of(of.p, group_sum<kWaves>(in_k, sh.red)) : ~0ull;
+    for (int at = tid; at < n; at += kThreads) {
+      const bool kept = rank[at] < of.k && before[at] < share && weight[at] >= least;
+      if (!kept) weight[at] = 0;
+      in_all += weight[at];
+      before[at] = 0;
+    }
+    const u64 want = target(group_sum<kWaves>(in_all, sh.red));   // (its barriers publish the kept weights)
+    for (int at = first; at < n; at += step) {
+      const unsigned mine = (unsigned)sh.list[at];   // the index, flipped
+      u64 sum = 0;
+#pragma unroll 4
+      for (int i = part; i < n; i += parts) sum += (unsigned)sh.list[i] > mine ? weight[i] : 0;
+      if (parts == 1) before[at] = sum;
+      else if (sum) atomicAdd(&before[at], sum);
+    }
+    __syncthreads();
+    for (int at = tid; at < n; at += kThreads)
+      if (weight[at] && before[at] <= want && want < before[at] + weight[at]) a.out[b] = (int64_t)(unsigned)~(unsigned)sh.list[at];
     return;
   }
   // a logit is kept when its key is above kmin, or equals it at an index up to last, and its weight is `least` or more
@@ -807,8 +941,8 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
     int bin = 0;
     u64 left = 0;
     const int n = a.listed[b];
-    if (!border_bin<kWaves>(a.hist + (long)b * kBins, a.top_p.of(b), sh.red, sh.found, bin, left) || n > kList) {
-      choose_from_start(a, b, sh);
+    if (!border_bin<kWaves>(a.hist + (long)b * kBins, of.p, sh.red, sh.found, bin, left) || n > kList) {
+      choose_from_start<kWaves>(a, of, b, sh);
       return;
     }
     for (int i = tid; i < n; i += kThreads) sh.list[i] = a.list[(long)b * kList + i];
@@ -816,17 +950,14 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
     auto keep = [&](u64 e, u64 w) {
       if (w >= least) atomicAdd(&sh.part[(unsigned)e / kChunk], w);
     };
-    const u64 edge = resolve(sh, n, left, weigh, keep);
+    const u64 edge = resolve<kWaves>(sh, n, left, weigh, keep);
     kmin = (unsigned)(edge >> 32);
     last = (int)(unsigned)edge;
     if (tid == 0) keep(edge, weigh(value_of(kmin)));
   }
   __syncthreads();
-  u64 total = 0;
-  for (int c = tid; c < chunks; c += kThreads) total += sh.part[c];
-  total = group_sum<kWaves>(total, sh.red);
-  const u64 want = target(total);
-  group_find<kWaves>(sh.part, chunks, want, sh.red, sh.found);
+  group_find<kWaves, kMaxChunks / 64 / kWaves>(sh.part, chunks, sh.red, sh.found, target);
+  const u64 want = sh.found[2];
   if (wv == 0) {
     float x[8];
     const int i = (int)sh.found[0] * kChunk + lane * 8;
@@ -839,7 +970,7 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
       w[j] = w[j] >= least ? w[j] : 0;
       s += w[j];
     }
-    u64 cum = sh.found[1] + wave_scan64(s, lane) - s;
+    u64 cum = sh.found[1] + wave_scan64(s) - s;
     if (cum <= want && want < cum + s) {
       int token = i;
       bool open = true;
@@ -861,9 +992,12 @@ __global__ __launch_bounds__(kThreads) void choose_kernel(Args<T> a) {
 
 using namespace pd;
 
+// logits per group: small ones allow a larger top-k (half the groups), large ones keep the list of their peaks short
+static int sample_group(int V) { return V <= 65536 ? 32 : 128; }
+
 // bytes of scratch for B rows of V logits
 extern "C" long pd_sample_workspace(int B, int V) {
-  const long chunks = (V + smp::kChunk - 1) / smp::kChunk, groups = (V + smp::kGroup - 1) / smp::kGroup;
+  const long chunks = (V + smp::kChunk - 1) / smp::kChunk, per = sample_group(V), groups = (V + per - 1) / per;
   return (long)B * (8 * (chunks + smp::kBins + smp::kList) + 4 * (groups + 1));
 }
 
@@ -875,11 +1009,13 @@ extern "C" int pd_sample(int dt, const void* logits, long stride, int B, int V, 
   int bits = 0;
   while ((1L << bits) < V) ++bits;
   const int shift = 62 - bits < 50 ? 62 - bits : 50;   // V weights of at most 2^shift stay under 2^62
-  const int chunks = (V + smp::kChunk - 1) / smp::kChunk, groups = (V + smp::kGroup - 1) / smp::kGroup;
-  // workgroups of four waves per row: a chunk a wave at most, about eight workgroups a CU in all
-  int slices = (chunks + 3) / 4;
-  const int enough = (2048 + B - 1) / B;
-  if (slices > enough) slices = enough;
+  const int chunks = (V + smp::kChunk - 1) / smp::kChunk, per = sample_group(V), groups = (V + per - 1) / per;
+  // workgroups per row: a chunk a wave, but about two thousand narrow (four waves) or a thousand wide ones in all
+  auto slices_of = [&](int waves, int all) {
+    const int most = (chunks + waves - 1) / waves, enough = (all + B - 1) / B;
+    return most < enough ? most : enough;
+  };
+  const dim3 narrow(slices_of(4, 2048), B), wide(slices_of(smp::kWide, 1024), B);
   hipStream_t st = (hipStream_t)stream;
   smp::u64* const mass = (smp::u64*)workspace;
   smp::u64* const hist = mass + (long)B * chunks;
@@ -891,12 +1027,13 @@ extern "C" int pd_sample(int dt, const void* logits, long stride, int B, int V, 
   const bool maybe_short = top_ks || (top_k > 0 && top_k < V), always_k = !top_ks && maybe_short;
   const bool maybe_p = maybe_warm && !always_k && (top_ps || top_p < 1.f);
   PD_DISPATCH_FLOAT(dt, T, {
-    const smp::Args<T> a{(const T*)logits, stride, V, chunks, groups, shift, uniform, {temps, temp}, {top_ps, top_p},
+    const smp::Args<T> a{(const T*)logits, stride, V, chunks, groups, per / 8, shift, uniform, {temps, temp}, {top_ps, top_p},
                          {min_ps, min_p}, top_ks, top_k, mass, hist, list, listed, peaks, out};
-    smp::peaks_kernel<T><<<dim3(slices, B), 256, 0, st>>>(a);
-    if (maybe_warm && !always_k) smp::bins_kernel<T><<<dim3(slices, B), 256, 0, st>>>(a);
-    if (maybe_p) smp::sweep_kernel<T><<<dim3(slices, B), 256, 0, st>>>(a);
-    smp::choose_kernel<T><<<B, smp::kThreads, 0, st>>>(a);
+    smp::peaks_kernel<T><<<narrow, 256, 0, st>>>(a);
+    if (maybe_warm && !always_k) smp::bins_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
+    if (maybe_p) smp::sweep_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
+    if (V <= 65536) smp::choose_kernel<T, 8><<<B, 512, 0, st>>>(a);
+    else smp::choose_kernel<T, 16><<<B, 1024, 0, st>>>(a);
   });
   return (int)hipGetLastError();
 }
