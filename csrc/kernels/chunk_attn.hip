@@ -48,10 +48,12 @@ struct Args {
   int s_blk, s_tok, s_head;
   const int *cu, *lens, *table;
   int B, T, Hq, Hk, G;
-  int max_blocks, num_blocks, block, block_shift;   // block_shift < 0: block is no power of two
+  int max_blocks, num_blocks, block, block_shift;
+  unsigned block_mul;                               // key / block = key * block_mul >> block_shift, for keys < 2^31
   int tiles, splits, min_keys;                      // tiles: upper bound over the batch
   float scale_log2;
   float *part_o, *part_ml;                          // [splits][T][Hq][D], [splits][T][Hq][2]
+  int* pieces;                                      // [T] into how many a token's keys were split
 };
 
 struct Seq {
@@ -149,14 +151,93 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-template <int D, bool F16, bool POW2>
-__global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
-  constexpr int NCH = D / 8, KS = D / 16, DT = D / 32, TILE = kBN * D * 2;
+__device__ __forceinline__ int block_of(const Args& a, int key) {
+  return (int)(((unsigned long long)(unsigned)key * a.block_mul) >> a.block_shift);
+}
+
+// A K or V tile on its way from the pages to LDS: a thread loads chunk tid % NCH of rows tid / NCH + ROWS * i.
+// UNI: the block size is a multiple of the RW rows that one wave's load covers, so a wave's rows of a load lie in one page.
+// Lane i works out load i's page, byte offset and extent, and the load is a buffer load from a scalar base whose extent
+// ends with the valid rows (past it, and for page numbers outside the pool, it reads zeros): K and V share all of that.
+// Otherwise every thread looks up its own rows' pages and points the missing ones at a block of zeros.
+template <int D, bool UNI>
+struct Stage {
+  static constexpr int NCH = D / 8, NLOAD = kBN * NCH / 256, ROWS = 256 / NCH, RW = 64 / NCH;
+  const Args& a;
+  const int* tab;
+  int k1, first_row, o_st, voff;
+  int page[UNI ? 1 : NLOAD], rest[UNI ? 1 : NLOAD], extent;   // of the tile to come
+  u16x8 st[NLOAD];
+  __device__ __forceinline__ Stage(const Args& a_, const Seq& s, int hk, int tid, int k1_) : a(a_) {
+    tab = a.table + (long)s.b * a.max_blocks;
+    k1 = k1_;
+    const int lrow = tid / NCH, lch = tid % NCH;
+    // (the swizzle has the row's lowest 4 bits, which ROWS leaves alone)
+    o_st = lrow * (D * 2) + swz<D>(lrow, lch) * 16;
+    if constexpr (UNI) {
+      first_row = (tid >> 6) * RW + ROWS * (tid & (NLOAD - 1));
+      voff = (lrow % RW) * a.s_tok * 2 + (hk * a.s_head + lch * 8) * 2;
+    } else {
+      first_row = lrow;
+      voff = hk * a.s_head + lch * 8;
+    }
+  }
+  // look up the pages of the tile at n0
+  __device__ __forceinline__ void pages(int n0) {
+#pragma unroll
+    for (int i = 0; i < (UNI ? 1 : NLOAD); ++i) {
+      const int key = n0 + first_row + ROWS * i, blk = block_of(a, min(key, k1 - 1));
+      page[i] = tab[blk];
+      rest[i] = (key - blk * a.block) * a.s_tok;
+      if constexpr (UNI) extent = min(max(k1 - key, 0), RW);
+      else rest[i] = key < k1 ? rest[i] : -1;
+    }
+  }
+  // where they lie, once they have arrived: K and V alike
+  unsigned lo, hi;
+  __device__ __forceinline__ void locate(int hk) {
+    if constexpr (UNI) {
+      const unsigned long long off = ((unsigned long long)(unsigned)page[0] * (unsigned)a.s_blk + (unsigned)rest[0]) * 2;
+      lo = (unsigned)off, hi = (unsigned)(off >> 32);
+      // (rows of other heads may lie between: the extent reaches to the end of the last row's head)
+      extent = (unsigned)page[0] < (unsigned)a.num_blocks && extent > 0 ? ((extent - 1) * a.s_tok + hk * a.s_head + D) * 2 : 0;
+    }
+  }
+  __device__ __forceinline__ void load(const unsigned short* cache) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) {
+      if constexpr (UNI) {
+        const unsigned long long off = (unsigned)__builtin_amdgcn_readlane((int)lo, i) |
+                                       (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, i) << 32;
+        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
+            (void*)((unsigned long long)cache + off), (short)0, __builtin_amdgcn_readlane(extent, i), 0x00020000);
+        st[i] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, voff, 0, 0));
+      } else {
+        const bool ok = rest[i] >= 0 && (unsigned)page[i] < (unsigned)a.num_blocks;
+        const unsigned short* p = cache + (long)page[i] * a.s_blk + (unsigned)(rest[i] + voff);
+        st[i] = *(ok ? reinterpret_cast<const u16x8*>(p) : &kZeros);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(char* dst) const {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) *reinterpret_cast<u16x8*>(dst + o_st + i * ROWS * (D * 2)) = st[i];
+  }
+};
+
+// KG groups of four waves: each takes every KG-th 64-key tile of the same 128 rows, and the groups' (m, l, O) are joined
+// through LDS.  KG = 2 has one workgroup on a CU where KG = 1 has two.
+template <int D, bool F16, bool UNI, int KG>
+__global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a) {
   constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;         // exponent bits: all set in infinities and NaN
-  constexpr int NLOAD = kBN * NCH / 256, ROWS = 256 / NCH;   // loads per thread and tile; rows between them
-  __shared__ __attribute__((aligned(16))) char smem[4 * TILE];
+  constexpr int KS = D / 16, DT = D / 32, TILE = kBN * D * 2;
+  using St = Stage<D, UNI>;
+  constexpr int NLOAD = St::NLOAD;
+  __shared__ __attribute__((aligned(16))) char lds[KG * 4 * TILE];
   __shared__ int odd_values;   // finite_only took something out
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tid = threadIdx.x & 255, wv = wave & 3, group = wave >> 2;
+  char* const smem = lds + group * 4 * TILE;
   const int r = lane & 31, h = lane >> 5;
   const int tile_tokens = kBM / a.G;
 
@@ -171,6 +252,8 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
   const int piece = piece_of(a, keys);
   const int k0 = sp * piece, k1 = min(keys, k0 + piece);
   const bool whole = piece >= keys;
+  if (a.splits > 1 && sp == 0 && hk == 0)
+    for (int i = threadIdx.x; i < ntok; i += 256 * KG) a.pieces[s.q0 + tok0 + i] = whole ? 1 : (keys + piece - 1) / piece;
   if (sp > 0 && k0 >= keys) return;
 
   const int row = wv * 32 + r;                                  // this lane's row: token row / G, head row % G
@@ -188,37 +271,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
     }
   }
 
-  // page numbers, then rows, of the tile's 64 keys; a thread loads chunk tid % NCH of rows tid / NCH + ROWS * i
-  const int lrow = tid / NCH, lch = tid % NCH;
-  const int* tab = a.table + (long)s.b * a.max_blocks;
-  const int head_off = hk * a.s_head + lch * 8;
-  auto block_of = [&](int key) { return POW2 ? key >> a.block_shift : key / a.block; };
-  auto row_offset = [&](int page, int key) {   // in elements, for this thread's 8; the part within the page fits 32 bits
-    const int in_page = POW2 ? key & (a.block - 1) : key % a.block;
-    return (long)page * a.s_blk + (unsigned)(in_page * a.s_tok + head_off);
-  };
-  int pid[NLOAD];
-  auto pages = [&](int n0) {
-#pragma unroll
-    for (int i = 0; i < NLOAD; ++i) pid[i] = tab[block_of(min(n0 + lrow + ROWS * i, k1 - 1))];
-  };
-  u16x8 st[NLOAD];
-  auto gload = [&](const unsigned short* cache, int n0) {
-#pragma unroll
-    for (int i = 0; i < NLOAD; ++i) {
-      const int key = n0 + lrow + ROWS * i;
-      const bool ok = key < k1 && (unsigned)pid[i] < (unsigned)a.num_blocks;
-      const unsigned short* p = cache + row_offset(pid[i], key);
-      st[i] = *(ok ? reinterpret_cast<const u16x8*>(p) : &kZeros);
-    }
-  };
-  // (the swizzle has the row's lowest 4 bits, which ROWS leaves alone)
-  const int o_st = lrow * (D * 2) + swz<D>(lrow, lch) * 16;
-  auto lstore = [&](char* dst) {
-#pragma unroll
-    for (int i = 0; i < NLOAD; ++i) *reinterpret_cast<u16x8*>(dst + o_st + i * ROWS * (D * 2)) = st[i];
-  };
-
+  St stage(a, s, hk, tid, k1);
   // V rows in registers, of a tile that some row does not see in full: values that are not finite become 0 (rare)
   auto finite_only = [&](int n0) {
     if (n0 + kBN - 1 <= pos0) return;
@@ -226,7 +279,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
     unsigned hit = 0;   // exponent + its lowest bit carries into bit 15 iff all exponent bits are set
 #pragma unroll
     for (int i = 0; i < NLOAD; ++i) {
-      const auto w = __builtin_bit_cast(u32x4, st[i]);
+      const auto w = __builtin_bit_cast(u32x4, stage.st[i]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) hit |= (w[j] & kE) + kLow;
     }
@@ -235,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
 #pragma unroll
       for (int i = 0; i < NLOAD; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) st[i][j] = (st[i][j] & kExp) == kExp ? (unsigned short)0 : st[i][j];
+        for (int j = 0; j < 8; ++j) stage.st[i][j] = (stage.st[i][j] & kExp) == kExp ? (unsigned short)0 : stage.st[i][j];
     }
   };
 
@@ -245,38 +298,40 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
   float m = -INFINITY, l = 0.f;
   const float sl2 = a.scale_log2;
   const int wave_rt0 = wv * 32 / a.G, wave_rt1 = min((wv * 32 + 31) / a.G, ntok - 1);
-  const int wave_first = min(pos0 + wave_rt0, k1 - 1);                // keys up to here are seen by all of its rows
-  const int wave_last = wave_rt0 < ntok ? pos0 + wave_rt1 : -1;       // and none past here by any
+  const int wave_last = wave_rt0 < ntok ? pos0 + wave_rt1 : -1;   // the last key that some row of the wave sees
 
   const int ntiles = k1 > k0 ? (k1 - k0 + kBN - 1) / kBN : 0;
-  if (tid == 0) odd_values = 0;
+  constexpr int kStep = KG * kBN;       // from one tile of a group to its next
+  const int kg = k0 + group * kBN;      // the group's first
+  if (threadIdx.x == 0) odd_values = 0;
   lds_barrier();
   if (ntiles > 0) {
-    pages(k0);
-    gload(a.k, k0);
-    lstore(smem);
-    gload(a.v, k0);
-    pages(k0 + kBN);
-    finite_only(k0);
-    lstore(smem + TILE);
+    stage.pages(kg);
+    stage.locate(hk);
+    stage.load(a.k);
+    stage.store(smem);
+    stage.load(a.v);
+    stage.pages(kg + kStep);
+    finite_only(kg);
+    stage.store(smem + TILE);
   }
   lds_barrier();
 
-  // Lane bases of the LDS reads; every read is one of them with a compile-time XOR:
+  // Lane bases of the LDS reads, in the stage being read; every read is one of them with a compile-time XOR and offset:
   //  K row kb * 32 + r, 16-byte chunk 2 ks + h;  V^T: rows 16 s + 8 (j >> 2) + 4 hh + qq, chunk 4 dt + cbits
   const int g = lane >> 4, qq = (lane & 15) >> 2, pp = lane & 3, hh = g >> 1, cbits = ((g & 1) << 1) | (pp >> 1);
   int o_k = r * (D * 2) + swz<D>(r, h) * 16;
   int o_va = (4 * hh + qq) * (D * 2) + swz<D>(4 * hh + qq, cbits) * 16 + 8 * (pp & 1);
   int o_vb = (4 * hh + qq + 8) * (D * 2) + swz<D>(4 * hh + qq + 8, cbits) * 16 + 8 * (pp & 1);
+  int buf = 0;   // byte offset of the stage being read
 
-  // One tile.  MASKED: some row of the wave does not see all of its keys (two bodies: as a branch in one, the masks
-  // were turned into selects on every tile).
-  auto tile_step = [&](auto MASKED_, int t) {
-    constexpr bool MASKED = decltype(MASKED_)::value;
-    const int n0 = k0 + t * kBN;
-    const char* kt = smem + (t & 1) * 2 * TILE;
-    const char* vt = kt + TILE;
-    char* const nxt = smem + ((t + 1) & 1) * 2 * TILE;
+  // One tile.  EDGE: some row may not see all of its keys, or of the next tile's (two loops, one body each: with both
+  // bodies in one loop O was copied between registers at their joint, 64 moves a tile).
+  auto tile_step = [&](auto EDGE_, int n0) {
+    constexpr bool EDGE = decltype(EDGE_)::value;
+    const char* const kt = smem;
+    const char* const vt = smem + TILE;
+    char* const nxt = smem + (buf ^ (2 * TILE));
     asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
     f32x16 sc[2];
 #pragma unroll
@@ -286,9 +341,10 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
       for (int ks = 0; ks < KS; ++ks)
         sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(kt + kb * 32 * (D * 2) + (o_k ^ (ks << 5))), qf[ks], sc[kb]);
     }
-    gload(a.k, n0 + kBN);   // in flight under the softmax (past the last tile it reads zeros: no branch in the tile)
-    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
-    if constexpr (MASKED) {
+    stage.locate(hk);
+    stage.load(a.k);   // in flight under the softmax (past the last tile it reads zeros: no branch in the tile)
+    if constexpr (EDGE) {
+      const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -325,9 +381,9 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
         ls[i & 3] += p;
       }
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    lstore(nxt);
-    gload(a.v, n0 + kBN);   // in flight under P.V
-    pages(n0 + 2 * kBN);
+    stage.store(nxt);
+    stage.load(a.v);   // in flight under P.V
+    stage.pages(n0 + 2 * kStep);
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
@@ -341,35 +397,71 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
           o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, vv), pb, o[dt]);
         }
       }
-    finite_only(n0 + kBN);
-    lstore(nxt + TILE);
+    if constexpr (EDGE) finite_only(n0 + kStep);
+    stage.store(nxt + TILE);
     lds_barrier();
   };
-  for (int t = 0; t < ntiles; ++t) {
-    const int n0 = k0 + t * kBN;
-    if (n0 > wave_last) {   // nothing to see for this wave: it helps to stage the next tile
-      char* const nxt = smem + ((t + 1) & 1) * 2 * TILE;
-      gload(a.k, n0 + kBN);
-      lstore(nxt);
-      gload(a.v, n0 + kBN);
-      pages(n0 + 2 * kBN);
-      finite_only(n0 + kBN);
-      lstore(nxt + TILE);
-      lds_barrier();
-    } else if (n0 + kBN - 1 > wave_first) {
-      tile_step(std::true_type{}, t);
-    } else {
-      tile_step(std::false_type{}, t);
+  auto stage_only = [&](int n0) {   // a wave with nothing to see helps to stage the next tile
+    char* const nxt = smem + (buf ^ (2 * TILE));
+    stage.locate(hk);
+    stage.load(a.k);
+    stage.store(nxt);
+    stage.load(a.v);
+    stage.pages(n0 + 2 * kStep);
+    finite_only(n0 + kStep);
+    stage.store(nxt + TILE);
+    lds_barrier();
+  };
+  auto turn = [&]() {
+    const int d = buf ? -2 * TILE : 2 * TILE;
+    buf ^= 2 * TILE;
+    o_k += d, o_va += d, o_vb += d;
+  };
+  // tiles that every row sees in full, and whose next one too; the same for every wave, as are all tiles' count: the
+  // barriers are shared
+  const int rounds = (ntiles + KG - 1) / KG, seen = (min(pos0 + 1, k1) - k0) / kBN;
+  const int inner = max(0, min(rounds, seen / KG - 1));
+  int n0 = kg;
+  if (wave_last < 0) {
+    for (int t = 0; t < rounds; ++t, n0 += kStep, turn()) stage_only(n0);
+  } else {
+    for (int t = 0; t < inner; ++t, n0 += kStep, turn()) tile_step(std::false_type{}, n0);
+    for (int t = inner; t < rounds; ++t, n0 += kStep, turn()) {
+      if (n0 > wave_last || n0 >= k1) stage_only(n0);
+      else tile_step(std::true_type{}, n0);
     }
+  }
+
+  if constexpr (KG == 2) {
+    // group 1 hands its rows to the same lanes of group 0: m, l, then O register by register
+    float* const x = reinterpret_cast<float*>(lds);
+    if (group == 1) {
+      x[tid] = m;
+      x[256 + tid] = l;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[(2 + dt * 16 + i) * 256 + tid] = o[dt][i];
+    }
+    lds_barrier();
+    if (group == 1) return;
+    const float m1 = x[tid], both = fmaxf(m, m1), base = both == -INFINITY ? 0.f : both;
+    const float w0 = __builtin_amdgcn_exp2f(m - base), w1 = __builtin_amdgcn_exp2f(m1 - base);
+    m = both;
+    l = l * w0 + x[256 + tid] * w1;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] = o[dt][i] * w0 + x[(2 + dt * 16 + i) * 256 + tid] * w1;
   }
 
   if (__builtin_expect(odd_values, 0)) {
     // what finite_only took out comes back, for the rows that see it
     // (tiles whose last key lies past pos0; a tile begins at k0 + a multiple of kBN)
     for (int j = k0 + max(pos0 - k0, 0) / kBN * kBN; j < k1; ++j) {
-      const int page = tab[block_of(j)];
+      const int blk = block_of(a, j), page = stage.tab[blk];
       if ((unsigned)page >= (unsigned)a.num_blocks || !live || j > pos) continue;
-      const unsigned short* vr = a.v + row_offset(page, j) + 4 * h - lch * 8;
+      const unsigned short* vr = a.v + (long)page * a.s_blk + (unsigned)((j - blk * a.block) * a.s_tok + hk * a.s_head) + 4 * h;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -418,44 +510,50 @@ __global__ __launch_bounds__(256, 2) void chunk_kernel(Args a) {
   }
 }
 
-// joins the pieces of every row that was split: one workgroup per token, D / 4 lanes per query head
+// joins the pieces of every row that was split: grid (tokens, groups of heads), D / 4 lanes per query head
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
   constexpr int LANES = D / 4, HEADS = 256 / LANES;
-  const int tok = blockIdx.x;
-  // the sequence of this token: the last b with cu[b] <= tok
-  int lo = 0, hi = a.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (a.cu[mid] <= tok) lo = mid;
-    else hi = mid - 1;
-  }
-  int q0, n;
-  bounds_of(a, lo, q0, n);
-  if (tok < q0 || tok >= q0 + n) return;
-  const int tile_tokens = kBM / a.G, tok0 = (tok - q0) / tile_tokens * tile_tokens;
-  const int keys = max(len_of(a, lo) - n + min(tok0 + tile_tokens, n), 0);
-  const int piece = piece_of(a, keys);
-  if (piece >= keys) return;
-  const int pieces = (keys + piece - 1) / piece;
-  const int d = (threadIdx.x % LANES) * 4;
-  for (int hq = threadIdx.x / LANES; hq < a.Hq; hq += HEADS) {
-    float M = -INFINITY;
-    for (int p = 0; p < pieces; ++p) M = fmaxf(M, a.part_ml[(((long)p * a.T + tok) * a.Hq + hq) * 2]);
-    const float base = M == -INFINITY ? 0.f : M;
-    float L = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < pieces; ++p) {
-      const long pi = ((long)p * a.T + tok) * a.Hq + hq;
-      const float w = __builtin_amdgcn_exp2f(a.part_ml[pi * 2] - base);
-      L += a.part_ml[pi * 2 + 1] * w;
-      acc += *reinterpret_cast<const f32x4*>(a.part_o + pi * D + d) * w;
-    }
-    const float inv = L != 0.f ? 1.f / L : 0.f;
-    unsigned short* op = a.out + (long)tok * a.so_tok + (long)hq * a.so_head + d;
+  const int tok = blockIdx.x, hq = blockIdx.y * HEADS + threadIdx.x / LANES, d = (threadIdx.x % LANES) * 4;
+  const int pieces = min(a.pieces[tok], a.splits);
+  // (a row of no sequence has no count)
+  if (tok < a.cu[0] || tok >= a.cu[a.B] || pieces <= 1 || hq >= a.Hq) return;
+  float M = -INFINITY, L = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < pieces; p0 += 4) {   // four pieces' loads together; past the last one m is -inf
+    float m[4], l[4];
+    f32x4 o[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) op[e] = cvt16<F16>(acc[e] * inv);
+    for (int i = 0; i < 4; ++i) {
+      const long pi = ((long)min(p0 + i, pieces - 1) * a.T + tok) * a.Hq + hq;
+      m[i] = a.part_ml[pi * 2];
+      l[i] = a.part_ml[pi * 2 + 1];
+      o[i] = *reinterpret_cast<const f32x4*>(a.part_o + pi * D + d);
+    }
+    float top = M;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (p0 + i >= pieces) m[i] = -INFINITY;
+      top = fmaxf(top, m[i]);
+    }
+    const float base = top == -INFINITY ? 0.f : top, w = __builtin_amdgcn_exp2f(M - base);
+    L *= w;
+    acc *= w;
+    M = top;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (p0 + i < pieces) {
+        const float wi = __builtin_amdgcn_exp2f(m[i] - base);
+        L += l[i] * wi;
+        acc += o[i] * wi;
+      }
   }
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+  u16x4 w;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w[e] = cvt16<F16>(acc[e] * inv);
+  *reinterpret_cast<u16x4*>(a.out + (long)tok * a.so_tok + (long)hq * a.so_head + d) = w;
 }
 
 }  // namespace ca
@@ -472,11 +570,11 @@ extern "C" int pd_chunk_attn_tiles(int T, int B, int G) {
 extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, const void* k, const void* v, long s_blk,
                              long s_tok, long s_head, const int* table, int max_blocks, int num_blocks, int block,
                              const int* cu, const int* lens, void* out, long so_tok, long so_head, int B, int T, int Hq,
-                             int Hk, int D, int splits, int min_keys, float scale, float* part_o, float* part_ml,
-                             void* stream) {
+                             int Hk, int D, int splits, int min_keys, float scale, int groups, float* part_o,
+                             float* part_ml, int* pieces, void* stream) {
   if (T <= 0 || B <= 0) return 0;
   if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1) return -1;
-  if (splits > 1 && (!part_o || !part_ml)) return -1;
+  if (splits > 1 && (!part_o || !part_ml || !pieces)) return -1;
   // a page's span in 32 bits (its number times s_blk is taken in 64)
   const long span = (long)(block - 1) * s_tok + (long)(Hk - 1) * s_head + D;
   if (s_blk < 0 || s_tok < 0 || s_head < 0 || s_blk > 0x7fffffffL || s_tok > 0x7fffffffL || s_head > 0x7fffffffL ||
@@ -492,33 +590,42 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   a.cu = cu, a.lens = lens, a.table = table;
   a.B = B, a.T = T, a.Hq = Hq, a.Hk = Hk, a.G = Hq / Hk;
   a.max_blocks = max_blocks, a.num_blocks = num_blocks, a.block = block;
-  a.block_shift = -1;
-  for (int s = 0; s < 31; ++s)
-    if ((1 << s) == block) a.block_shift = s;
+  // key / block as a product: m = ceil(2^(31 + L) / block), L = ceil(log2 block); the excess key * (m block - 2^(31 + L)) /
+  // (block 2^(31 + L)) stays below 2^-L <= 1 / block for keys < 2^31
+  int L = 0;
+  while ((1L << L) < block) ++L;
+  a.block_shift = block == 1 ? 0 : 31 + L;
+  a.block_mul = block == 1 ? 1u : (unsigned)(((1UL << (31 + L)) + block - 1) / block);
   a.tiles = pd_chunk_attn_tiles(T, B, a.G);
   a.splits = splits, a.min_keys = min_keys < ca::kBN ? ca::kBN : min_keys;
   a.scale_log2 = scale * ca::kLog2e;
-  a.part_o = part_o, a.part_ml = part_ml;
+  a.part_o = part_o, a.part_ml = part_ml, a.pieces = pieces;
   const long wgs = (long)a.tiles * Hk * splits;
   if (wgs > 0x7fffffffL) return -1;
   hipStream_t st = (hipStream_t)stream;
+  // (a wave's load covers 512 / D rows: see Stage)
+  const bool uni = block % (512 / D) == 0 && s_tok >= D && span + 8 * s_tok < 1L << 30;
+#define PD_CHUNK3(DV, F, U)                                                                 \
+  do {                                                                                      \
+    if (groups == 2) ca::chunk_kernel<DV, F, U, 2><<<(unsigned)wgs, 512, 0, st>>>(a);       \
+    else ca::chunk_kernel<DV, F, U, 1><<<(unsigned)wgs, 256, 0, st>>>(a);                   \
+  } while (0)
 #define PD_CHUNK(DV)                                                                        \
   do {                                                                                      \
-    if (a.block_shift >= 0) {                                                               \
-      if (f16) ca::chunk_kernel<DV, true, true><<<(unsigned)wgs, 256, 0, st>>>(a);          \
-      else ca::chunk_kernel<DV, false, true><<<(unsigned)wgs, 256, 0, st>>>(a);             \
-    } else {                                                                                \
-      if (f16) ca::chunk_kernel<DV, true, false><<<(unsigned)wgs, 256, 0, st>>>(a);         \
-      else ca::chunk_kernel<DV, false, false><<<(unsigned)wgs, 256, 0, st>>>(a);            \
-    }                                                                                       \
+    if (f16 && uni) PD_CHUNK3(DV, true, true);                                              \
+    else if (f16) PD_CHUNK3(DV, true, false);                                               \
+    else if (uni) PD_CHUNK3(DV, false, true);                                               \
+    else PD_CHUNK3(DV, false, false);                                                       \
     if (splits > 1) {                                                                       \
-      if (f16) ca::join_kernel<DV, true><<<T, 256, 0, st>>>(a);                             \
-      else ca::join_kernel<DV, false><<<T, 256, 0, st>>>(a);                                \
+      const dim3 jg(T, (Hq * DV / 4 + 255) / 256);                                          \
+      if (f16) ca::join_kernel<DV, true><<<jg, 256, 0, st>>>(a);                            \
+      else ca::join_kernel<DV, false><<<jg, 256, 0, st>>>(a);                               \
     }                                                                                       \
   } while (0)
   if (D == 64) PD_CHUNK(64);
   else if (D == 128) PD_CHUNK(128);
   else return -2;
 #undef PD_CHUNK
+#undef PD_CHUNK3
   return (int)hipGetLastError();
 }

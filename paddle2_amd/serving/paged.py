@@ -17,6 +17,7 @@ _HEAD_DIMS = (64, 128)
 # split of a tile's keys over workgroups: enough of them to fill the chip, each with at least this many keys
 _CHUNK_WG_TARGET = 512
 _CHUNK_MIN_KEYS = 256
+_CHUNK_GROUPS = int(__import__('os').environ.get('CG', '1'))
 
 
 def _u(x):
@@ -119,14 +120,15 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     wgs = m.chunk_attn_tiles(T, B, Hq // Hk) * Hk
     splits = max(1, min(-(-_CHUNK_WG_TARGET // wgs), max_blocks * bs // _CHUNK_MIN_KEYS, 64))
     with _on(q.device):
-        po = pm = None
+        po = pm = pc = None
         if splits > 1:
+            pc = torch.empty(T, dtype=torch.int32, device=q.device)
             po = torch.empty(splits * T * Hq * D, dtype=torch.float32, device=q.device)
             pm = torch.empty(splits * T * Hq * 2, dtype=torch.float32, device=q.device)
         m.chunk_attn(int(q.dtype == torch.float16), q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
                      kc.stride(0), kc.stride(tok), kc.stride(head), table.data_ptr(), max_blocks, kc.shape[0], bs,
                      cu.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), B, T, Hq, Hk, D,
-                     splits, _CHUNK_MIN_KEYS, scale, N.ptr(po), N.ptr(pm), N.stream())
+                     splits, _CHUNK_MIN_KEYS, scale, _CHUNK_GROUPS, N.ptr(po), N.ptr(pm), N.ptr(pc), N.stream())
 
 
 def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):
