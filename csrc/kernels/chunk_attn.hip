@@ -39,7 +39,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kDefer = 8.f;   // the running maximum moves only when a row outgrows it by 2^8
 constexpr int kBM = 128, kBN = 64;
 
-__device__ const u16x8 kZeros = {0, 0, 0, 0, 0, 0, 0, 0};
+__device__ const u16x8 kZeros[16] = {};   // a row of D = 128
+// p, or a row of zeros.  (Both are named global: chosen as plain pointers they gave flat loads, which count as LDS
+// operations too and made every LDS wait one for memory.)
+typedef __attribute__((address_space(1))) const u16x8 global_u16x8;
+__device__ __forceinline__ global_u16x8* row_or_zeros(bool ok, const unsigned short* p) {
+  return ok ? (global_u16x8*)p : (global_u16x8*)kZeros;
+}
 
 struct Args {
   const unsigned short *q, *k, *v;
@@ -50,7 +56,7 @@ struct Args {
   int B, T, Hq, Hk, G;
   int max_blocks, num_blocks, block, block_shift;
   unsigned block_mul;                               // key / block = key * block_mul >> block_shift, for keys < 2^31
-  int tiles, splits, min_keys;                      // tiles: upper bound over the batch
+  int tiles, splits, min_keys, grain;               // tiles: upper bound over the batch; a piece: a multiple of grain keys
   float scale_log2;
   float *part_o, *part_ml;                          // [splits][T][Hq][D], [splits][T][Hq][2]
   int* pieces;                                      // [T] into how many a token's keys were split
@@ -72,8 +78,11 @@ __device__ __forceinline__ int len_of(const Args& a, int b) {
 __device__ __forceinline__ Seq find_tile(const Args& a, int tile, int tile_tokens, int lane) {
   int base = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    int q0 = 0, n = 0;
-    if (b0 + lane < a.B) bounds_of(a, b0 + lane, q0, n);
+    const int b = min(b0 + lane, a.B - 1);
+    int q0, n;
+    bounds_of(a, b, q0, n);
+    const int len = len_of(a, b);   // (here, so that it is under way with cu)
+    if (b0 + lane >= a.B) n = 0;
     const int mine = (n + tile_tokens - 1) / tile_tokens;
     int incl = mine;
 #pragma unroll
@@ -83,27 +92,26 @@ __device__ __forceinline__ Seq find_tile(const Args& a, int tile, int tile_token
     }
     const unsigned long long hit = __ballot(base + incl > tile);
     if (hit) {
-      const int l = __ffsll((long long)hit) - 1;
+      const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1);
       Seq s;
-      s.b = __builtin_amdgcn_readfirstlane(b0 + l);
-      s.q0 = __builtin_amdgcn_readfirstlane(__shfl(q0, l, 64));
-      s.n = __builtin_amdgcn_readfirstlane(__shfl(n, l, 64));
+      s.b = b0 + l;
+      s.q0 = __builtin_amdgcn_readlane(q0, l);
+      s.n = __builtin_amdgcn_readlane(n, l);
+      s.len = __builtin_amdgcn_readlane(len, l);
       // the tile that sees the most keys first
-      const int in_seq = __shfl(mine, l, 64) - 1 - (tile - (base + __shfl(incl - mine, l, 64)));
-      s.tile = __builtin_amdgcn_readfirstlane(in_seq);
-      s.len = len_of(a, s.b);
+      s.tile = __builtin_amdgcn_readlane(incl, l) - 1 - (tile - base);
       return s;
     }
-    base += __shfl(incl, 63, 64);
+    base += __builtin_amdgcn_readlane(incl, 63);
   }
   return Seq{0, 0, 0, 0, -1};
 }
 
-// keys per piece of a tile that sees `keys` keys: whole 64-key tiles, at least min_keys, at most `splits` pieces
+// keys per piece of a tile that sees `keys` keys: whole grains, at least min_keys, at most `splits` pieces
 __device__ __forceinline__ int piece_of(const Args& a, int keys) {
   const int pieces = max(1, min(a.splits, (keys + a.min_keys - 1) / a.min_keys));
   const int per = (keys + pieces - 1) / pieces;
-  return max((per + kBN - 1) / kBN * kBN, kBN);
+  return max((per + a.grain - 1) / a.grain * a.grain, a.grain);
 }
 
 template <int D>
@@ -215,7 +223,7 @@ struct Stage {
       } else {
         const bool ok = rest[i] >= 0 && (unsigned)page[i] < (unsigned)a.num_blocks;
         const unsigned short* p = cache + (long)page[i] * a.s_blk + (unsigned)(rest[i] + voff);
-        st[i] = *(ok ? reinterpret_cast<const u16x8*>(p) : &kZeros);
+        st[i] = *row_or_zeros(ok, p);
       }
     }
   }
@@ -309,9 +317,10 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
     stage.pages(kg);
     stage.locate(hk);
     stage.load(a.k);
-    stage.store(smem);
+    St first(stage);      // (K and V on their way together)
     stage.load(a.v);
     stage.pages(kg + kStep);
+    first.store(smem);
     finite_only(kg);
     stage.store(smem + TILE);
   }
@@ -510,6 +519,232 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   }
 }
 
+// Few rows (decoding, drafted tokens): 16 rows of one (sequence, kv head) per workgroup, bound by the reads of K and V.
+// Each of the four waves takes every fourth 32-key tile of the piece on its own, with no barrier in the loop:
+//  * S^T = K . Q^T on 16x16x32 MFMA; a lane loads its K operands (16 bytes of a key's row) straight into registers, V goes
+//    through a wave's own LDS image for the transposed reads;
+//  * two register sets in turn: 32 loads of 16 bytes a lane are in flight (D = 128), page numbers one tile further ahead;
+//  * the waves' (m, l, O) are joined through LDS at the end.
+// The tiled kernel above needs 20 us for 8 x 4 drafted tokens over 350 - 700 keys, most of it the latency of its steps.
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+constexpr int kFewRows = 16, kFewKeys = 32;
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
+  constexpr int KC = D / 32, DT = D / 16;
+  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kFewKeys * D * 2];   // the waves' V images, then their O
+  __shared__ float ml[4][kFewRows][2];
+  __shared__ int odd_values;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, h = lane >> 4;
+  const int tile_tokens = kFewRows / a.G;
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int hk = id % a.Hk, sp = id / a.Hk % a.splits, tile = id / (a.Hk * a.splits);   // the heads of a token together
+  const Seq s = find_tile(a, tile, tile_tokens, lane);
+  if (s.tile < 0) return;
+  const int tok0 = s.tile * tile_tokens, ntok = min(tile_tokens, s.n - tok0);
+  const int pos0 = s.len - s.n + tok0, keys = max(pos0 + ntok, 0);
+  const int piece = piece_of(a, keys), k0 = sp * piece, k1 = min(keys, k0 + piece);
+  const bool whole = piece >= keys;
+  if (a.splits > 1 && sp == 0 && hk == 0 && tid < ntok) a.pieces[s.q0 + tok0 + tid] = whole ? 1 : (keys + piece - 1) / piece;
+  if (sp > 0 && k0 >= keys) return;
+  if (tid == 0) odd_values = 0;
+  lds_barrier();
+
+  const int rt = c16 / a.G, rh = hk * a.G + c16 % a.G, pos = pos0 + rt;
+  const bool live = rt < ntok;
+  bf16x8 qf[KC];
+  {
+    const unsigned short* qp = a.q + (long)(s.q0 + tok0 + (live ? rt : 0)) * a.sq_tok + (long)(live ? rh : 0) * a.sq_head + 8 * h;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      qf[c] = *reinterpret_cast<const bf16x8*>(qp + 32 * c);
+      if (!live) qf[c] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  const int* tab = a.table + (long)s.b * a.max_blocks;
+  const unsigned head_off = hk * a.s_head + 8 * h;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kFewKeys - 1) / kFewKeys : 0;
+  auto pages = [&](int t, int (&pg)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) pg[u] = tab[block_of(a, min(k0 + kFewKeys * t + 16 * u + c16, k1 - 1))];
+  };
+  auto load = [&](int t, const int (&pg)[2], u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = k0 + kFewKeys * t + 16 * u + c16, blk = block_of(a, key);
+      const bool ok = key < k1 && (unsigned)pg[u] < (unsigned)a.num_blocks;
+      const long off = (long)pg[u] * a.s_blk + (unsigned)((key - blk * a.block) * a.s_tok + head_off);
+      global_u16x8 *pk = row_or_zeros(ok, a.k + off), *pv = row_or_zeros(ok, a.v + off);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        kk[u][c] = pk[4 * c];
+        vv[u][c] = pv[4 * c];
+      }
+    }
+  };
+  f32x4 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const float sl2 = a.scale_log2;
+  char* const vl = lds + w * (kFewKeys * D * 2);
+  const int qq = c16 >> 2, pp = c16 & 3;
+  auto compute = [&](int t, const u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
+    const int n0 = k0 + kFewKeys * t;
+    if (n0 + kFewKeys - 1 > pos0) {   // some row does not see all of it: values that are not finite are put in at the end
+      constexpr unsigned kE = kExp | (unsigned)kExp << 16, kLow = F16 ? 0x04000400u : 0x00800080u;
+      unsigned hit = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const auto x = __builtin_bit_cast(u32x4, vv[u][c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) hit |= (x[j] & kE) + kLow;
+        }
+      if (__builtin_expect(hit & 0x80008000u, 0)) {
+        odd_values = 1;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vv[u][c][j] = (vv[u][c][j] & kExp) == kExp ? (unsigned short)0 : vv[u][c][j];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        *reinterpret_cast<u16x8*>(vl + (16 * u + c16) * (D * 2) + 16 * swz<D>(16 * u + c16, 4 * c + h)) = vv[u][c];
+    f32x4 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) sc[u] = mfma16<F16>(__builtin_bit_cast(bf16x8, kk[u][c]), qf[c], sc[u]);
+    }
+    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 16 u + 4 h + e is hidden iff 16 u + e >= lim
+    float mt = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[u][e] = 16 * u + e >= lim ? -INFINITY : sc[u][e] * sl2;
+        mt = fmaxf(mt, sc[u][e]);
+      }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);
+    m = mn;
+    bf16x8 pf;
+    float ps = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(sc[u][e] - base);
+        ps += p;
+        pf[4 * u + e] = __builtin_bit_cast(__bf16, cvt16<F16>(p));
+      }
+    l = l * alpha + ps;
+    float ar[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ar[e] = __shfl(alpha, 4 * h + e, 64);   // O's row 4 h + e has its state in that lane
+#pragma unroll
+    for (int t2 = 0; t2 < DT; ++t2) {
+      const s16x4 lo = lds_tr(vl, (4 * h + qq) * (D * 2) + 16 * swz<D>(4 * h + qq, 2 * t2 + (pp >> 1)) + 8 * (pp & 1));
+      const s16x4 hi = lds_tr(vl, (16 + 4 * h + qq) * (D * 2) + 16 * swz<D>(16 + 4 * h + qq, 2 * t2 + (pp >> 1)) + 8 * (pp & 1));
+      const s16x8 v8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t2][e] *= ar[e];
+      o[t2] = mfma16<F16>(pf, __builtin_bit_cast(bf16x8, v8), o[t2]);
+    }
+  };
+  // Two tiles a turn without an exit between them; past the last tile keys are hidden and loads read zeros
+  u16x8 ka[2][KC], va[2][KC], kb[2][KC], vb[2][KC];
+  if (w < ntiles) {
+    int pa[2], pb[2];
+    pages(w, pa);
+    pages(w + 4, pb);
+    load(w, pa, ka, va);
+    for (int t = w; t < ntiles; t += 8) {
+      pages(t + 8, pa);
+      load(t + 4, pb, kb, vb);
+      __builtin_amdgcn_sched_barrier(0);   // the loads stay ahead of the work
+      compute(t, ka, va);
+      pages(t + 12, pb);
+      load(t + 8, pa, ka, va);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(t + 4, kb, vb);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  __syncthreads();   // every wave is done with its V image
+  float* const ow = reinterpret_cast<float*>(lds);   // [4][16][D]
+  if (h == 0) {
+    ml[w][c16][0] = m;
+    ml[w][c16][1] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ow[(w * kFewRows + 4 * h + e) * D + 16 * t + c16] = o[t][e];
+  __syncthreads();
+  const int rows = ntok * a.G;
+  for (int i = tid; i < rows * (D / 4); i += 256) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) M = fmaxf(M, ml[x][row][0]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const float wt = __builtin_amdgcn_exp2f(ml[x][row][0] - base);
+      L += ml[x][row][1] * wt;
+      acc += *reinterpret_cast<const f32x4*>(ow + (x * kFewRows + row) * D + d) * wt;
+    }
+    const int tok = row / a.G, hq = hk * a.G + row % a.G;
+    if (__builtin_expect(odd_values, 0)) {   // the values that were taken out, where this row sees them
+      for (int j = k0 + max(pos0 - k0, 0) / kFewKeys * kFewKeys; j < k1 && j <= pos0 + tok; ++j) {
+        const int blk = block_of(a, j), page = tab[blk];
+        if ((unsigned)page >= (unsigned)a.num_blocks) continue;
+        const unsigned short* vr = a.v + (long)page * a.s_blk + (unsigned)((j - blk * a.block) * a.s_tok + hk * a.s_head) + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((vr[e] & kExp) == kExp) acc[e] += F16 ? h2f(vr[e]) : bf2f(vr[e]);
+      }
+    }
+    const long trow = s.q0 + tok0 + tok;
+    if (whole) {
+      const float inv = L != 0.f ? 1.f / L : 0.f;
+      typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+      u16x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = cvt16<F16>(acc[e] * inv);
+      *reinterpret_cast<u16x4*>(a.out + trow * a.so_tok + (long)hq * a.so_head + d) = r;
+    } else {
+      const long pi = ((long)sp * a.T + trow) * a.Hq + hq;
+      *reinterpret_cast<f32x4*>(a.part_o + pi * D + d) = acc;
+      if (d == 0) {
+        a.part_ml[pi * 2] = M;
+        a.part_ml[pi * 2 + 1] = L;
+      }
+    }
+  }
+}
+
 // joins the pieces of every row that was split: grid (tokens, groups of heads), D / 4 lanes per query head
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
@@ -562,18 +797,20 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 using namespace pd;
 
 // upper bound of the batch's row tiles: every sequence may end in a part of one
-extern "C" int pd_chunk_attn_tiles(int T, int B, int G) {
-  const int tt = ca::kBM / G, some = B < T ? B : T;
+extern "C" int pd_chunk_attn_tiles(int T, int B, int G, int few) {
+  const int tt = (few ? ca::kFewRows : ca::kBM) / G, some = B < T ? B : T;
   return (int)((T + (long)some * (tt - 1)) / tt);
 }
 
 extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, const void* k, const void* v, long s_blk,
                              long s_tok, long s_head, const int* table, int max_blocks, int num_blocks, int block,
                              const int* cu, const int* lens, void* out, long so_tok, long so_head, int B, int T, int Hq,
-                             int Hk, int D, int splits, int min_keys, float scale, int groups, float* part_o,
+                             int Hk, int D, int splits, int min_keys, float scale, int few, int groups, float* part_o,
                              float* part_ml, int* pieces, void* stream) {
   if (T <= 0 || B <= 0) return 0;
-  if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1) return -1;
+  if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1 ||
+      (few && Hq / Hk > ca::kFewRows))
+    return -1;
   if (splits > 1 && (!part_o || !part_ml || !pieces)) return -1;
   // a page's span in 32 bits (its number times s_blk is taken in 64)
   const long span = (long)(block - 1) * s_tok + (long)(Hk - 1) * s_head + D;
@@ -596,8 +833,9 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   while ((1L << L) < block) ++L;
   a.block_shift = block == 1 ? 0 : 31 + L;
   a.block_mul = block == 1 ? 1u : (unsigned)(((1UL << (31 + L)) + block - 1) / block);
-  a.tiles = pd_chunk_attn_tiles(T, B, a.G);
-  a.splits = splits, a.min_keys = min_keys < ca::kBN ? ca::kBN : min_keys;
+  a.tiles = pd_chunk_attn_tiles(T, B, a.G, few);
+  a.grain = few ? 4 * ca::kFewKeys : ca::kBN;
+  a.splits = splits, a.min_keys = min_keys < a.grain ? a.grain : min_keys;
   a.scale_log2 = scale * ca::kLog2e;
   a.part_o = part_o, a.part_ml = part_ml, a.pieces = pieces;
   const long wgs = (long)a.tiles * Hk * splits;
@@ -612,7 +850,9 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   } while (0)
 #define PD_CHUNK(DV)                                                                        \
   do {                                                                                      \
-    if (f16 && uni) PD_CHUNK3(DV, true, true);                                              \
+    if (few && f16) ca::few_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);             \
+    else if (few) ca::few_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);              \
+    else if (f16 && uni) PD_CHUNK3(DV, true, true);                                            \
     else if (f16) PD_CHUNK3(DV, true, false);                                               \
     else if (uni) PD_CHUNK3(DV, false, true);                                               \
     else PD_CHUNK3(DV, false, false);                                                       \

@@ -5,7 +5,6 @@ same definitions run in PyTorch.  Inference only: nothing here records a gradien
 """
 from __future__ import annotations
 
-import contextlib
 import math
 
 import torch
@@ -17,6 +16,9 @@ _HEAD_DIMS = (64, 128)
 # split of a tile's keys over workgroups: enough of them to fill the chip, each with at least this many keys
 _CHUNK_WG_TARGET = 512
 _CHUNK_MIN_KEYS = 256
+_FEW_ROWS = int(__import__('os').environ.get('FR', '16'))
+_FEW_WG_TARGET = int(__import__('os').environ.get('FT', '1024'))
+_FEW_MIN_KEYS = int(__import__('os').environ.get('FM', '256'))
 _CHUNK_GROUPS = int(__import__('os').environ.get('CG', '1'))
 
 
@@ -24,24 +26,32 @@ def _u(x):
     return x._t if isinstance(x, Tensor) else x
 
 
-def _on(dev):
-    """The device of the operands as the current one, for the launch and its stream."""
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on ``dev``: its current stream, and it the current device meanwhile."""
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
+    if dev.index == torch.cuda.current_device():
+        fn(*args, stream)
+    else:
+        with torch.cuda.device(dev):
+            fn(*args, stream)
 
 
-def _ints(t, name, size, dev):
-    """A 1-D or 2-D int tensor on ``dev`` as contiguous int32."""
+_INTS = (torch.int32, torch.int64, torch.int16, torch.uint8, torch.int8)
+
+
+def _ints(t, name, rows, cols, dev):
+    """An int tensor [rows] or (cols given) [rows, any] on ``dev`` as contiguous int32."""
     t = _u(t)
-    if not torch.is_tensor(t) or t.is_floating_point() or t.dtype == torch.bool:
+    if not torch.is_tensor(t) or t.dtype not in _INTS:
         raise TypeError(f"chunk_attention: {name} must be an integer tensor")
     if t.device != dev:
         raise ValueError(f"chunk_attention: {name} is on {t.device}, the queries on {dev}")
-    if t.dim() != len(size) or any(s is not None and s != n for s, n in zip(size, t.shape)):
-        raise ValueError(f"chunk_attention: {name} has shape {tuple(t.shape)}, expected {size}")
-    return t.to(torch.int32).contiguous()
+    shape = t.shape
+    if len(shape) != (2 if cols else 1) or (rows is not None and shape[0] != rows):
+        raise ValueError(f"chunk_attention: {name} has shape {tuple(shape)}, expected ({rows or 'B'}{', pages' if cols else ''})")
+    return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 
-@torch.no_grad()
 def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=None, layout="paged", scale=None, out=None):
     """Attention of the new tokens of a ragged batch over a paged KV cache.
 
@@ -60,75 +70,83 @@ def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=Non
     16-byte aligned.  Returns out [T, Hq, D]."""
     wrap = isinstance(q, Tensor)
     q, k_cache, v_cache, out = _u(q), _u(k_cache), _u(v_cache), _u(out)
-    dev = q.device
-    if q.dim() != 3 or k_cache.dim() != 4 or k_cache.shape != v_cache.shape:
-        raise ValueError(f"chunk_attention: q {tuple(q.shape)}, caches {tuple(k_cache.shape)}, {tuple(v_cache.shape)}")
-    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise TypeError(f"chunk_attention: q {q.dtype}, caches {k_cache.dtype}, {v_cache.dtype}")
+    dev, dt, qs, ks = q.device, q.dtype, q.shape, k_cache.shape
+    if len(qs) != 3 or len(ks) != 4 or ks != v_cache.shape:
+        raise ValueError(f"chunk_attention: q {tuple(qs)}, caches {tuple(ks)}, {tuple(v_cache.shape)}")
+    if k_cache.dtype is not dt or v_cache.dtype is not dt:
+        raise TypeError(f"chunk_attention: q {dt}, caches {k_cache.dtype}, {v_cache.dtype}")
     if k_cache.device != dev or v_cache.device != dev:
         raise ValueError(f"chunk_attention: q on {dev}, caches on {k_cache.device}, {v_cache.device}")
-    T, Hq, D = q.shape
-    tok, head = {"paged": (1, 2), "paddle_block": (2, 1), "bhsd": (2, 1)}.get(layout, (None, None))
-    if tok is None:
+    T, Hq, D = qs
+    if layout == "paged":
+        tok, head = 1, 2
+    elif layout in ("paddle_block", "bhsd"):
+        tok, head = 2, 1
+    else:
         raise ValueError(f"chunk_attention: layout {layout!r}")
-    bs, Hk = k_cache.shape[tok], k_cache.shape[head]
-    if k_cache.shape[3] != D or Hk == 0 or bs == 0 or Hq % Hk:
-        raise ValueError(f"chunk_attention: q {tuple(q.shape)} does not fit the {layout} cache {tuple(k_cache.shape)}")
-    lens = _ints(seq_lens, "seq_lens", (None,), dev)
+    bs, Hk = ks[tok], ks[head]
+    if ks[3] != D or Hk == 0 or bs == 0 or Hq % Hk:
+        raise ValueError(f"chunk_attention: q {tuple(qs)} does not fit the {layout} cache {tuple(ks)}")
+    lens = _ints(seq_lens, "seq_lens", None, False, dev)
     B = lens.shape[0]
-    cu = _ints(cu_seqlens_q, "cu_seqlens_q", (B + 1,), dev)
+    cu = _ints(cu_seqlens_q, "cu_seqlens_q", B + 1, False, dev)
     if layout == "bhsd":
-        if k_cache.shape[0] < B:
-            raise ValueError(f"chunk_attention: {B} sequences, caches for {k_cache.shape[0]}")
+        if ks[0] < B:
+            raise ValueError(f"chunk_attention: {B} sequences, caches for {ks[0]}")
         table = torch.arange(B, dtype=torch.int32, device=dev)[:, None]
     elif block_table is None:
         raise ValueError(f"chunk_attention: layout {layout!r} needs a block_table")
     else:
-        table = _ints(block_table, "block_table", (B, None), dev)
+        table = _ints(block_table, "block_table", B, True, dev)
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"chunk_attention: scale {scale}")
     if out is None:
-        out = torch.empty(T, Hq, D, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev:
+        out = torch.empty(qs, dtype=dt, device=dev)
+    elif out.shape != qs or out.dtype is not dt or out.device != dev:
         raise ValueError(f"chunk_attention: out {tuple(out.shape)} {out.dtype} on {out.device}")
-    if T and B and table.shape[1] and k_cache.shape[0]:
+    if T and B:
         if dev.type == "cuda" and N.use_native(q):
             _chunk_native(q, k_cache, v_cache, cu, lens, table, tok, head, scale, out)
         else:
-            _chunk_reference(q, k_cache, v_cache, cu, lens, table, tok, scale, out)
-    elif T and B:   # an empty cache: no row sees a key
-        out[:int(cu[-1])] = 0
+            with torch.no_grad():
+                _chunk_reference(q, k_cache, v_cache, cu, lens, table, tok, scale, out)
     return Tensor._wrap(out) if wrap else out
 
 
 def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     T, Hq, D = q.shape
     B, max_blocks = table.shape
-    bs, Hk = kc.shape[tok], kc.shape[head]
-    if q.dtype not in (torch.bfloat16, torch.float16) or D not in _HEAD_DIMS or Hq // Hk > 128:
-        raise ValueError(f"chunk_attention: {q.dtype} with head dim {D} and {Hq // Hk} query heads per kv head (bfloat16 or "
-                         f"float16, {_HEAD_DIMS}, at most 128)")
-    if kc.stride() != vc.stride():
+    ks, sk, so = kc.shape, kc.stride(), out.stride()
+    bs, Hk = ks[tok], ks[head]
+    G = Hq // Hk
+    if q.dtype not in (torch.bfloat16, torch.float16) or D not in _HEAD_DIMS or G > 128:
+        raise ValueError(f"chunk_attention: {q.dtype} with head dim {D} and {G} query heads per kv head (bfloat16 or float16, "
+                         f"{_HEAD_DIMS}, at most 128)")
+    if not max_blocks or not ks[0]:
+        raise ValueError("chunk_attention: a cache or a block table without pages")
+    if sk != vc.stride():
         raise ValueError("chunk_attention: the K and V caches have different strides")
-    if q.stride(2) != 1 or (q.data_ptr() | (q.stride(0) * 2) | (q.stride(1) * 2)) & 15:
-        q = q.clone(memory_format=torch.contiguous_format)
-    for name, t in (("k_cache", kc), ("v_cache", vc), ("out", out)):
-        if t.stride(-1) != 1 or any((s * 2) & 15 for s in t.stride()[:-1]) or t.data_ptr() & 15:
-            raise ValueError(f"chunk_attention: {name} needs contiguous, 16-byte aligned rows")
+    sq = q.stride()
+    if sq[2] != 1 or (q.data_ptr() | sq[0] * 2 | sq[1] * 2) & 15:
+        with torch.no_grad():
+            q = q.clone(memory_format=torch.contiguous_format)
+        sq = q.stride()
+    pq, pk, pv, po = q.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr()
+    if sk[3] != 1 or so[2] != 1 or ((sk[0] | sk[1] | sk[2] | so[0] | so[1]) * 2 | pk | pv | po) & 15:
+        raise ValueError("chunk_attention: the caches and out need contiguous, 16-byte aligned rows")
     m = N.native()
-    wgs = m.chunk_attn_tiles(T, B, Hq // Hk) * Hk
-    splits = max(1, min(-(-_CHUNK_WG_TARGET // wgs), max_blocks * bs // _CHUNK_MIN_KEYS, 64))
-    with _on(q.device):
-        po = pm = pc = None
-        if splits > 1:
-            pc = torch.empty(T, dtype=torch.int32, device=q.device)
-            po = torch.empty(splits * T * Hq * D, dtype=torch.float32, device=q.device)
-            pm = torch.empty(splits * T * Hq * 2, dtype=torch.float32, device=q.device)
-        m.chunk_attn(int(q.dtype == torch.float16), q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(),
-                     kc.stride(0), kc.stride(tok), kc.stride(head), table.data_ptr(), max_blocks, kc.shape[0], bs,
-                     cu.data_ptr(), lens.data_ptr(), out.data_ptr(), out.stride(0), out.stride(1), B, T, Hq, Hk, D,
-                     splits, _CHUNK_MIN_KEYS, scale, _CHUNK_GROUPS, N.ptr(po), N.ptr(pm), N.ptr(pc), N.stream())
+    few = G <= 16 and T * G <= _FEW_ROWS * B
+    wgs = m.chunk_attn_tiles(T, B, G, few) * Hk
+    target, least = (_FEW_WG_TARGET, _FEW_MIN_KEYS) if few else (_CHUNK_WG_TARGET, _CHUNK_MIN_KEYS)
+    splits = max(1, min(-(-target // wgs), max_blocks * bs // least, 64))
+    # scratch of a split: the pieces' O, their (maximum, sum), and into how many a token's keys were split
+    ws = torch.empty(splits * T * Hq * (D + 2) + T, dtype=torch.float32, device=q.device) if splits > 1 else None
+    w0 = 0 if ws is None else ws.data_ptr()
+    w1 = w0 + 4 * splits * T * Hq * D
+    _launch(q.device, m.chunk_attn, int(q.dtype is torch.float16), pq, sq[0], sq[1], pk, pv, sk[0], sk[tok], sk[head],
+            table.data_ptr(), max_blocks, ks[0], bs, cu.data_ptr(), lens.data_ptr(), po, so[0], so[1], B, T, Hq, Hk, D,
+            splits, least, scale, int(few), _CHUNK_GROUPS, w0, w1, w1 + 8 * splits * T * Hq)
 
 
 def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):
@@ -186,15 +204,14 @@ class KVBlockCopier:
         self._bytes = (a.numel() // max(a.shape[0], 1)) * a.element_size()
         self._stride = a.stride(0) * a.element_size()
         self._native = self._dev.type == "cuda" and N.use_native(a)
-        self._ptrs = [t.data_ptr() for t in pools] if self._native else None
+        if self._native:
+            self._ptrs, self._copy = [t.data_ptr() for t in pools], N.native().kv_copy
 
-    @torch.no_grad()
     def copy(self, src, dst):
         """Page src[i] -> page dst[i] in every pool, on the current stream.  ``src`` / ``dst``: host integers.  A page may be
         a source many times, a destination once, and never both; ValueError otherwise, with nothing copied."""
         if self._native:
-            with _on(self._dev):
-                N.native().kv_copy(self._ptrs, src, dst, self._blocks, self._bytes, self._stride, N.stream())
+            _launch(self._dev, self._copy, self._ptrs, src, dst, self._blocks, self._bytes, self._stride)
             return
         src, dst = [int(i) for i in src], [int(i) for i in dst]
         if len(src) != len(dst):
@@ -208,8 +225,9 @@ class KVBlockCopier:
             raise ValueError("a page is both a source and a destination")
         if src:
             s, d = (torch.tensor(i, device=self._dev) for i in (src, dst))
-            for t in self.pools:
-                t[d] = t[s]
+            with torch.no_grad():
+                for t in self.pools:
+                    t[d] = t[s]
 
 
 def copy_kv_blocks(k_caches, v_caches, src, dst):

@@ -8,29 +8,32 @@ import torch
 
 from ..framework.tensor import Tensor
 from ..ops import _native as N
-from .paged import _on, _u
+from .paged import _launch, _u
 
-_MAX_VOCAB = 1 << 20
+_MAX_VOCAB, _MAX_ROWS = 1 << 20, 65535
 
 
 def _setting(v, name, rows, dev, dtype, lo, hi):
     """(tensor or None, number): one value per row, or one for all, checked where the host can see it."""
-    v = _u(v)
-    if torch.is_tensor(v):
-        if v.shape != (rows,) or v.device != dev:
-            raise ValueError(f"sample_tokens: {name} {tuple(v.shape)} on {v.device}, expected ({rows},) on {dev}")
-        if dtype == torch.int32:
-            if v.is_floating_point() or v.dtype == torch.bool:
-                raise TypeError(f"sample_tokens: {name} must hold integers")
-            if v.dtype == torch.int64:
-                v = v.clamp(-1, 2 ** 31 - 1)
-        return v.to(dtype).contiguous(), 0
-    if not isinstance(v, numbers.Real) or not lo <= v <= hi or (dtype == torch.int32 and v != int(v)):
+    if v.__class__ is float or v.__class__ is int:
+        number = True
+    else:
+        v = _u(v)
+        number = isinstance(v, numbers.Real)
+    if number and lo <= v <= hi and (dtype is not torch.int32 or v == int(v)):
+        return None, int(min(v, 2 ** 31 - 1)) if dtype is torch.int32 else float(v)
+    if not torch.is_tensor(v):
         raise ValueError(f"sample_tokens: {name} = {v!r} (a number in [{lo}, {hi}] or a tensor of one per row)")
-    return None, int(min(v, 2 ** 31 - 1)) if dtype == torch.int32 else float(v)
+    if v.shape != (rows,) or v.device != dev:
+        raise ValueError(f"sample_tokens: {name} {tuple(v.shape)} on {v.device}, expected ({rows},) on {dev}")
+    if dtype is torch.int32:
+        if v.is_floating_point() or v.dtype is torch.bool:
+            raise TypeError(f"sample_tokens: {name} must hold integers")
+        if v.dtype is torch.int64:
+            v = v.clamp(-1, 2 ** 31 - 1)
+    return (v if v.dtype is dtype and v.is_contiguous() else v.detach().to(dtype).contiguous()), 0
 
 
-@torch.no_grad()
 def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
     """Draw one token per row: logits [B, V] (float32, bfloat16, float16) and a random number per row,
     ``uniform`` [B] float32 in [0, 1) -> int64 [B].
@@ -50,11 +53,11 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     same in every launch, batch and graph.  V is at most 1,048,576 on the GPU."""
     wrap = isinstance(logits, Tensor)
     x, u, out = _u(logits), _u(uniform), _u(out)
-    if x.dim() != 2 or x.shape[1] < 1 or not x.is_floating_point():
-        raise ValueError(f"sample_tokens: logits {tuple(x.shape)} {x.dtype}")
-    B, V = x.shape
-    dev = x.device
-    if u.shape != (B,) or u.dtype != torch.float32 or u.device != dev:
+    shape, dev, dt = x.shape, x.device, x.dtype
+    if len(shape) != 2 or shape[1] < 1 or not dt.is_floating_point:
+        raise ValueError(f"sample_tokens: logits {tuple(shape)} {dt}")
+    B, V = shape
+    if u.shape != (B,) or u.dtype is not torch.float32 or u.device != dev:
         raise ValueError(f"sample_tokens: uniform {tuple(u.shape)} {u.dtype} on {u.device}, expected ({B},) float32 on {dev}")
     t = _setting(temperature, "temperature", B, dev, torch.float32, 0.0, 1e30)
     k = _setting(top_k, "top_k", B, dev, torch.int32, -1, math.inf)
@@ -62,25 +65,25 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     m = _setting(min_p, "min_p", B, dev, torch.float32, 0.0, 1.0)
     if out is None:
         out = torch.empty(B, dtype=torch.int64, device=dev)
-    elif out.shape != (B,) or out.dtype != torch.int64 or out.device != dev or not out.is_contiguous():
+    elif out.shape != (B,) or out.dtype is not torch.int64 or out.device != dev or not out.is_contiguous():
         raise ValueError(f"sample_tokens: out {tuple(out.shape)} {out.dtype} on {out.device}")
     if B == 0:
         pass
     elif dev.type == "cuda" and N.use_native(x):
-        if x.dtype not in N.DT_CODE or V > _MAX_VOCAB:
-            raise ValueError(f"sample_tokens: {x.dtype} logits over {V} tokens (float32, bfloat16 or float16, at most "
-                             f"{_MAX_VOCAB})")
-        if x.stride(1) != 1 and V > 1:
-            x = x.contiguous()
-        u = u.contiguous()
-        if B > 65535:
-            raise ValueError(f"sample_tokens: {B} rows (at most 65,535)")
-        with _on(dev):
-            ws = torch.empty(N.native().sample_workspace(B, V), dtype=torch.uint8, device=dev)
-            N.native().sample(N.DT_CODE[x.dtype], x.data_ptr(), x.stride(0), B, V, u.data_ptr(), N.ptr(t[0]), t[1],
-                              N.ptr(k[0]), k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), ws.data_ptr(), N.stream())
+        if dt not in N.DT_CODE or V > _MAX_VOCAB or B > _MAX_ROWS:
+            raise ValueError(f"sample_tokens: {B} rows of {dt} logits over {V} tokens (float32, bfloat16 or float16, at most "
+                             f"{_MAX_ROWS} rows and {_MAX_VOCAB} tokens)")
+        if V > 1 and x.stride(1) != 1:
+            x = x.detach().contiguous()
+        if not u.is_contiguous():
+            u = u.detach().contiguous()
+        n = N.native()
+        ws = torch.empty(n.sample_workspace(B, V), dtype=torch.uint8, device=dev)
+        _launch(dev, n.sample, N.DT_CODE[dt], x.data_ptr(), x.stride(0), B, V, u.data_ptr(), N.ptr(t[0]), t[1], N.ptr(k[0]),
+                k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), ws.data_ptr())
     else:
-        out.copy_(_reference(x, u, t, k, p, m))
+        with torch.no_grad():
+            out.copy_(_reference(x, u, t, k, p, m))
     return Tensor._wrap(out) if wrap else out
 
 

@@ -118,6 +118,34 @@ def test_chunk_attention_long_gpu(new, held, Hq, Hk, D):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 10 ** 6])
+@pytest.mark.parametrize("splits", [1, 10 ** 6])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_chunk_attention_every_kernel_gpu(rows, splits, dtype, monkeypatch):
+    """The kernels for few rows and for many, with the keys in one piece and in as many as possible, on the same batches."""
+    from paddle2_amd.serving import paged
+
+    monkeypatch.setattr(paged, "_FEW_ROWS", rows)
+    for name in ("_CHUNK_WG_TARGET", "_FEW_WG_TARGET"):
+        monkeypatch.setattr(paged, name, splits)
+    for D in (64, 128):
+        _check_attn("cuda", dtype, [1, 0, 40, 3], [1000, 50, 700, 0], 8, 2, D, 16)
+        _check_attn("cuda", dtype, [2, 17], [129, 400], 4, 4, D, 32, seed=1)
+        _check_attn("cuda", dtype, [9, 1], [127, 255], 6, 2, D, 12, seed=2)
+        _check_attn("cuda", dtype, [5, 4], [300, 31], 16, 1, D, 7, seed=3)
+        q, kc, vc, cu, lens, table = _batch("cuda", dtype, [10, 4], [0, 600], 4, 1, D, 16, seed=4)
+        lens[0] = 4
+        assert (serving.chunk_attention(q, kc, vc, cu, lens, table)[:6] == 0).all()
+        for bad in (float("nan"), float("inf")):      # behind token 2 of sequence 1: its last token alone sees it
+            good = serving.chunk_attention(q, kc, vc, cu, lens, table)
+            vc[table[1, 603 // 16].long(), 603 % 16] = bad
+            out = serving.chunk_attention(q, kc, vc, cu, lens, table)
+            torch.testing.assert_close(out[:13], good[:13], rtol=2 ** -7, atol=1e-3)
+            assert not torch.isfinite(out[13]).any()
+            vc[table[1, 603 // 16].long(), 603 % 16] = 1.0
+
+
+@pytest.mark.gpu
 def test_chunk_attention_many_sequences_gpu():
     """More sequences than a wave has lanes, lengths of zero among them."""
     new = [(i * 7) % 5 for i in range(150)]
@@ -311,8 +339,17 @@ def test_chunk_attention_refusals_cpu():
     _refused("cpu", torch.float32)
     m = N.native()
     with pytest.raises(ValueError):
-        m.chunk_attn_tiles(4, 1, 129)
-    assert m.chunk_attn_tiles(2048, 1, 1) == 16 and m.chunk_attn_tiles(3, 64, 1) == 3 and m.chunk_attn_tiles(5, 2, 128) == 5
+        m.chunk_attn_tiles(4, 1, 129, 0)
+    with pytest.raises(ValueError):
+        m.chunk_attn_tiles(4, 1, 17, 1)
+    # enough tiles for every split of T rows over B sequences
+    for T in (1, 5, 2048):
+        for B in (1, 3, 64):
+            for rows, few, Gs in ((128, 0, (1, 3, 128)), (16, 1, (1, 3, 16))):
+                for G in Gs:
+                    per, some = rows // G, min(B, T)
+                    most = some + (T - some) // per        # `some` sequences of one row, the rest in full tiles
+                    assert most <= m.chunk_attn_tiles(T, B, G, few) <= most + some
 
 
 @pytest.mark.gpu
