@@ -56,7 +56,7 @@ struct Args {
   int B, T, Hq, Hk, G;
   int max_blocks, num_blocks, block, block_shift;
   unsigned block_mul;                               // key / block = key * block_mul >> block_shift, for keys < 2^31
-  int tiles, splits, min_keys, grain;               // tiles: upper bound over the batch; a piece: a multiple of grain keys
+  int splits, min_keys, grain;                      // a piece of the keys: a multiple of grain
   float scale_log2;
   float *part_o, *part_ml;                          // [splits][T][Hq][D], [splits][T][Hq][2]
   int* pieces;                                      // [T] into how many a token's keys were split
@@ -74,37 +74,64 @@ __device__ __forceinline__ int len_of(const Args& a, int b) {
   return (int)min((long)max(a.lens[b], 0), (long)a.max_blocks * a.block);
 }
 
-// the sequence that holds tile `tile` of the batch; every wave computes it for itself
-__device__ __forceinline__ Seq find_tile(const Args& a, int tile, int tile_tokens, int lane) {
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int b = min(b0 + lane, a.B - 1);
-    int q0, n;
-    bounds_of(a, b, q0, n);
-    const int len = len_of(a, b);   // (here, so that it is under way with cu)
-    if (b0 + lane >= a.B) n = 0;
-    const int mine = (n + tile_tokens - 1) / tile_tokens;
-    int incl = mine;
+__device__ __forceinline__ int xcd_remap(int bid, int n) {
+  const int q = n / 8, r = n % 8, xcd = bid % 8;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
+}
+
+// 64 sequences from b0, one a lane: where its queries begin, how many, its keys, and the row tiles up to and with it
+struct Lanes {
+  int q0, n, len, upto;
+};
+__device__ __forceinline__ Lanes sequences(const Args& a, int b0, int tile_tokens, int lane) {
+  Lanes s;
+  const int b = min(b0 + lane, a.B - 1);
+  bounds_of(a, b, s.q0, s.n);
+  s.len = len_of(a, b);
+  if (b0 + lane >= a.B) s.n = 0;
+  s.upto = (s.n + tile_tokens - 1) / tile_tokens;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int t = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += t;
-    }
-    const unsigned long long hit = __ballot(base + incl > tile);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(s.upto, o, 64);
+    if (lane >= o) s.upto += t;
+  }
+  return s;
+}
+
+// This workgroup's part of the batch: a row tile, a kv head and a piece of the keys; every wave works it out for itself.
+// The grid is an upper bound.  The parts there really are go to the XCDs in eight equal stretches (with the bound's, the
+// last XCDs had nothing to do: 16 x 3 tokens over 3,000 keys 45 us instead of 33).  HEADS_FIRST: neighbours in a stretch
+// are the kv heads of the same keys, whose rows lie side by side; otherwise the tiles of one head, which share their keys.
+template <bool HEADS_FIRST>
+__device__ __forceinline__ Seq find_part(const Args& a, int tile_tokens, int lane, int& hk, int& sp) {
+  Lanes s = sequences(a, 0, tile_tokens, lane);
+  int total = __builtin_amdgcn_readlane(s.upto, 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(sequences(a, b0, tile_tokens, lane).upto, 63);
+  const int parts = total * a.Hk * a.splits;
+  if ((int)blockIdx.x >= parts) return Seq{0, 0, 0, 0, -1};
+  const int id = xcd_remap(blockIdx.x, parts);
+  int tile;
+  if (HEADS_FIRST) hk = id % a.Hk, sp = id / a.Hk % a.splits, tile = id / (a.Hk * a.splits);
+  else sp = id % a.splits, tile = id / a.splits % total, hk = id / (a.splits * total);
+  int base = 0, b0 = 0;
+  for (;;) {
+    const unsigned long long hit = __ballot(base + s.upto > tile);   // some lane, tile < total
     if (hit) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1);
-      Seq s;
-      s.b = b0 + l;
-      s.q0 = __builtin_amdgcn_readlane(q0, l);
-      s.n = __builtin_amdgcn_readlane(n, l);
-      s.len = __builtin_amdgcn_readlane(len, l);
+      Seq r;
+      r.b = b0 + l;
+      r.q0 = __builtin_amdgcn_readlane(s.q0, l);
+      r.n = __builtin_amdgcn_readlane(s.n, l);
+      r.len = __builtin_amdgcn_readlane(s.len, l);
       // the tile that sees the most keys first
-      s.tile = __builtin_amdgcn_readlane(incl, l) - 1 - (tile - base);
-      return s;
+      r.tile = __builtin_amdgcn_readlane(s.upto, l) - 1 - (tile - base);
+      return r;
     }
-    base += __builtin_amdgcn_readlane(incl, 63);
+    base += __builtin_amdgcn_readlane(s.upto, 63);
+    b0 += 64;
+    if (b0 >= a.B) return Seq{0, 0, 0, 0, -1};
+    s = sequences(a, b0, tile_tokens, lane);
   }
-  return Seq{0, 0, 0, 0, -1};
 }
 
 // keys per piece of a tile that sees `keys` keys: whole grains, at least min_keys, at most `splits` pieces
@@ -146,11 +173,6 @@ __device__ __forceinline__ bf16x8 pack8(const f32x16& acc, int s) {
     return r;
   }
 }
-__device__ __forceinline__ int xcd_remap(int bid, int n) {
-  const int q = n / 8, r = n % 8, xcd = bid % 8;
-  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
-}
-
 // Barrier for LDS hand-offs: this wave's LDS operations are done, its global loads may stay in flight (__syncthreads
 // would wait for them too)
 __device__ __forceinline__ void lds_barrier() {
@@ -249,9 +271,8 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   const int r = lane & 31, h = lane >> 5;
   const int tile_tokens = kBM / a.G;
 
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int sp = id % a.splits, tile = (id / a.splits) % a.tiles, hk = id / (a.splits * a.tiles);
-  const Seq s = find_tile(a, tile, tile_tokens, lane);
+  int hk, sp;
+  const Seq s = find_part<false>(a, tile_tokens, lane, hk, sp);
   if (s.tile < 0) return;
   const int tok0 = s.tile * tile_tokens;                        // first token of the tile within the sequence
   const int ntok = min(tile_tokens, s.n - tok0);
@@ -545,9 +566,8 @@ __global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int c16 = lane & 15, h = lane >> 4;
   const int tile_tokens = kFewRows / a.G;
-  const int id = xcd_remap(blockIdx.x, gridDim.x);
-  const int hk = id % a.Hk, sp = id / a.Hk % a.splits, tile = id / (a.Hk * a.splits);   // the heads of a token together
-  const Seq s = find_tile(a, tile, tile_tokens, lane);
+  int hk, sp;
+  const Seq s = find_part<true>(a, tile_tokens, lane, hk, sp);
   if (s.tile < 0) return;
   const int tok0 = s.tile * tile_tokens, ntok = min(tile_tokens, s.n - tok0);
   const int pos0 = s.len - s.n + tok0, keys = max(pos0 + ntok, 0);
@@ -833,12 +853,11 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   while ((1L << L) < block) ++L;
   a.block_shift = block == 1 ? 0 : 31 + L;
   a.block_mul = block == 1 ? 1u : (unsigned)(((1UL << (31 + L)) + block - 1) / block);
-  a.tiles = pd_chunk_attn_tiles(T, B, a.G, few);
   a.grain = few ? 4 * ca::kFewKeys : ca::kBN;
   a.splits = splits, a.min_keys = min_keys < a.grain ? a.grain : min_keys;
   a.scale_log2 = scale * ca::kLog2e;
   a.part_o = part_o, a.part_ml = part_ml, a.pieces = pieces;
-  const long wgs = (long)a.tiles * Hk * splits;
+  const long wgs = (long)pd_chunk_attn_tiles(T, B, a.G, few) * Hk * splits;
   if (wgs > 0x7fffffffL) return -1;
   hipStream_t st = (hipStream_t)stream;
   // (a wave's load covers 512 / D rows: see Stage)

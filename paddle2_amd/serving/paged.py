@@ -13,13 +13,10 @@ from ..framework.tensor import Tensor
 from ..ops import _native as N
 
 _HEAD_DIMS = (64, 128)
-# split of a tile's keys over workgroups: enough of them to fill the chip, each with at least this many keys
-_CHUNK_WG_TARGET = 512
-_CHUNK_MIN_KEYS = 256
-_FEW_ROWS = int(__import__('os').environ.get('FR', '16'))
-_FEW_WG_TARGET = int(__import__('os').environ.get('FT', '1024'))
-_FEW_MIN_KEYS = int(__import__('os').environ.get('FM', '256'))
-_CHUNK_GROUPS = int(__import__('os').environ.get('CG', '1'))
+_CHUNK_WGS = 512        # workgroups that fit the chip at once
+_CHUNK_MIN_KEYS = 256   # keys of a piece at least (128: the join costs more than the shorter pieces give)
+_FEW_ROWS = 16          # rows (query heads of a kv head times new tokens) per sequence up to which they are few, on average
+_CHUNK_GROUPS = 1
 
 
 def _u(x):
@@ -137,16 +134,19 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
         raise ValueError("chunk_attention: the caches and out need contiguous, 16-byte aligned rows")
     m = N.native()
     few = G <= 16 and T * G <= _FEW_ROWS * B
-    wgs = m.chunk_attn_tiles(T, B, G, few) * Hk
-    target, least = (_FEW_WG_TARGET, _FEW_MIN_KEYS) if few else (_CHUNK_WG_TARGET, _CHUNK_MIN_KEYS)
-    splits = max(1, min(-(-target // wgs), max_blocks * bs // least, 64))
+    # Pieces of a tile's keys.  Two workgroups fit a CU: as many pieces as fit the chip at once.  Few rows over many
+    # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
+    # are left whole, their pieces' O costs more than it evens out.
+    tiles = max(min(B, T), -(-T // ((16 if few else 128) // G))) * Hk
+    splits = _CHUNK_WGS // tiles if tiles < _CHUNK_WGS or not few else 4 * _CHUNK_WGS // tiles
+    splits = max(1, min(splits, max_blocks * bs // _CHUNK_MIN_KEYS, 64))
     # scratch of a split: the pieces' O, their (maximum, sum), and into how many a token's keys were split
     ws = torch.empty(splits * T * Hq * (D + 2) + T, dtype=torch.float32, device=q.device) if splits > 1 else None
     w0 = 0 if ws is None else ws.data_ptr()
     w1 = w0 + 4 * splits * T * Hq * D
     _launch(q.device, m.chunk_attn, int(q.dtype is torch.float16), pq, sq[0], sq[1], pk, pv, sk[0], sk[tok], sk[head],
             table.data_ptr(), max_blocks, ks[0], bs, cu.data_ptr(), lens.data_ptr(), po, so[0], so[1], B, T, Hq, Hk, D,
-            splits, least, scale, int(few), _CHUNK_GROUPS, w0, w1, w1 + 8 * splits * T * Hq)
+            splits, _CHUNK_MIN_KEYS, scale, int(few), _CHUNK_GROUPS, w0, w1, w1 + 8 * splits * T * Hq)
 
 
 def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):

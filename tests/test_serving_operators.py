@@ -126,8 +126,7 @@ def test_chunk_attention_every_kernel_gpu(rows, splits, dtype, monkeypatch):
     from paddle2_amd.serving import paged
 
     monkeypatch.setattr(paged, "_FEW_ROWS", rows)
-    for name in ("_CHUNK_WG_TARGET", "_FEW_WG_TARGET"):
-        monkeypatch.setattr(paged, name, splits)
+    monkeypatch.setattr(paged, "_CHUNK_WGS", splits)
     for D in (64, 128):
         _check_attn("cuda", dtype, [1, 0, 40, 3], [1000, 50, 700, 0], 8, 2, D, 16)
         _check_attn("cuda", dtype, [2, 17], [129, 400], 4, 4, D, 32, seed=1)
