@@ -99,20 +99,31 @@ __device__ __forceinline__ Lanes sequences(const Args& a, int b0, int tile_token
 }
 
 // This workgroup's part of the batch: a row tile, a kv head and a piece of the keys; every wave works it out for itself.
-// The grid is an upper bound.  The parts there really are go to the XCDs in eight equal stretches (with the bound's, the
-// last XCDs had nothing to do: 16 x 3 tokens over 3,000 keys 45 us instead of 33).  HEADS_FIRST: neighbours in a stretch
-// are the kv heads of the same keys, whose rows lie side by side; otherwise the tiles of one head, which share their keys.
-template <bool HEADS_FIRST>
+// The grid is an upper bound of the parts there are; neighbours are the kv heads of one tile, and a sequence's tiles go
+// from the one that sees the most keys to the one that sees the fewest.
+//  STRETCHES (few rows): each XCD takes an eighth of the parts, side by side, so that the heads' rows of one key, which
+//  share lines and pages, are read by one XCD.
+//  Otherwise workgroup i has part i, and an XCD every eighth: with eight heads or a multiple each has its own heads'
+//  keys in its L2, and the tiles' lengths are spread evenly.  Two workgroups share a CU, and the second of each is
+//  dispatched after the first of all: the second 32 of an XCD go from light to heavy, so that a heavy one has a light
+//  one beside it (2,048 tokens, 32 heads, nothing cached: 74 us without, all that a CU did was one weight).
+template <bool STRETCHES>
 __device__ __forceinline__ Seq find_part(const Args& a, int tile_tokens, int lane, int& hk, int& sp) {
   Lanes s = sequences(a, 0, tile_tokens, lane);
   int total = __builtin_amdgcn_readlane(s.upto, 63);
   for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(sequences(a, b0, tile_tokens, lane).upto, 63);
   const int parts = total * a.Hk * a.splits;
-  if ((int)blockIdx.x >= parts) return Seq{0, 0, 0, 0, -1};
-  const int id = xcd_remap(blockIdx.x, parts);
-  int tile;
-  if (HEADS_FIRST) hk = id % a.Hk, sp = id / a.Hk % a.splits, tile = id / (a.Hk * a.splits);
-  else sp = id % a.splits, tile = id / a.splits % total, hk = id / (a.splits * total);
+  int id = blockIdx.x;
+  if (id >= parts) return Seq{0, 0, 0, 0, -1};
+  if (STRETCHES) {
+    id = xcd_remap(id, parts);
+  } else {
+    const int per = parts / 8;   // (full rows of eight)
+    const int j = id / 8, last = min(per, 64) - 1;
+    if (j >= 32 && j <= last) id = (32 + last - j) * 8 + id % 8;
+  }
+  hk = id % a.Hk, sp = id / a.Hk % a.splits;
+  const int tile = id / (a.Hk * a.splits);
   int base = 0, b0 = 0;
   for (;;) {
     const unsigned long long hit = __ballot(base + s.upto > tile);   // some lane, tile < total
