@@ -345,15 +345,20 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   const int kg = k0 + group * kBN;      // the group's first
   if (threadIdx.x == 0) odd_values = 0;
   lds_barrier();
+  // The tiles run one ahead: S of the next tile is multiplied while the present one is exponentiated, so K is staged two
+  // tiles ahead and V one (K and V have two stages each: a stage is written in the round after its last read).
   if (ntiles > 0) {
     stage.pages(kg);
     stage.locate(hk);
     stage.load(a.k);
-    St first(stage);      // (K and V on their way together)
+    St first(stage);   // (K and V on their way together)
     stage.load(a.v);
     stage.pages(kg + kStep);
     first.store(smem);
     finite_only(kg);
+    stage.store(smem + 2 * TILE);
+    stage.locate(hk);
+    stage.load(a.k);
     stage.store(smem + TILE);
   }
   lds_barrier();
@@ -362,41 +367,28 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   //  K row kb * 32 + r, 16-byte chunk 2 ks + h;  V^T: rows 16 s + 8 (j >> 2) + 4 hh + qq, chunk 4 dt + cbits
   const int g = lane >> 4, qq = (lane & 15) >> 2, pp = lane & 3, hh = g >> 1, cbits = ((g & 1) << 1) | (pp >> 1);
   int o_k = r * (D * 2) + swz<D>(r, h) * 16;
-  int o_va = (4 * hh + qq) * (D * 2) + swz<D>(4 * hh + qq, cbits) * 16 + 8 * (pp & 1);
-  int o_vb = (4 * hh + qq + 8) * (D * 2) + swz<D>(4 * hh + qq + 8, cbits) * 16 + 8 * (pp & 1);
-  int buf = 0;   // byte offset of the stage being read
+  int o_va = 2 * TILE + (4 * hh + qq) * (D * 2) + swz<D>(4 * hh + qq, cbits) * 16 + 8 * (pp & 1);
+  int o_vb = 2 * TILE + (4 * hh + qq + 8) * (D * 2) + swz<D>(4 * hh + qq + 8, cbits) * 16 + 8 * (pp & 1);
+  int buf = 0;   // the present tile's stage: 0 or TILE
 
-  // One tile.  EDGE: some row may not see all of its keys, or of the next tile's (two loops, one body each: with both
-  // bodies in one loop O was copied between registers at their joint, 64 moves a tile).
-  auto tile_step = [&](auto EDGE_, int n0) {
-    constexpr bool EDGE = decltype(EDGE_)::value;
-    const char* const kt = smem;
-    const char* const vt = smem + TILE;
-    char* const nxt = smem + (buf ^ (2 * TILE));
-    asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
-    f32x16 sc[2];
+  auto scores = [&](f32x16 (&sc)[2], int at) {   // of the K stage at byte `at`
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       sc[kb] = f32x16{};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
-        sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(kt + kb * 32 * (D * 2) + (o_k ^ (ks << 5))), qf[ks], sc[kb]);
+        sc[kb] = mfma<F16>(*reinterpret_cast<const bf16x8*>(smem + kb * 32 * (D * 2) + (at ^ (ks << 5))), qf[ks], sc[kb]);
     }
-    stage.locate(hk);
-    stage.load(a.k);   // in flight under the softmax (past the last tile it reads zeros: no branch in the tile)
-    if constexpr (EDGE) {
-      const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sc[kb][i] = kb * 32 + (i & 3) + 8 * (i >> 2) >= lim ? -INFINITY : sc[kb][i];
-    }
-    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+  };
+  auto hide = [&](f32x16 (&sc)[2], int n0) {
+    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 4 h + c is hidden iff c >= lim
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[kb][i]);
-    float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      for (int i = 0; i < 16; ++i) sc[kb][i] = kb * 32 + (i & 3) + 8 * (i >> 2) >= lim ? -INFINITY : sc[kb][i];
+  };
+  // the running maximum takes in the largest of a lane's scores; l and O follow
+  auto raise = [&](float mt) {
     {
       const unsigned mu = __builtin_bit_cast(unsigned, mt);
       const auto sw = __builtin_amdgcn_permlane32_swap(mu, mu, false, false);
@@ -411,65 +403,143 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
       for (int dt = 0; dt < DT; ++dt) o[dt] *= alpha;
       m = mc;
     }
+  };
+  auto largest = [&](const f32x16 (&sc)[2]) {
+    float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mx[i & 3] = fmaxf(mx[i & 3], sc[kb][i]);
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  };
+  auto v_frag = [&](int i, int dt) {   // 16 keys from 16 i, 32 columns from 32 dt
+    const char* vr = smem + 16 * i * (D * 2);
+    const s16x4 lo = lds_tr(vr, o_va ^ (dt << 6)), hi = lds_tr(vr, o_vb ^ (dt << 6));
+    const s16x8 vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(bf16x8, vv);
+  };
+  // One tile, whose scores are in cur, the next one's in nxt at the end.  EDGE: some row may not see all keys of the next
+  // tile (two loops, one body each: with both in one loop O was copied between registers at their joint).
+  // The order of the inner body is written down step by step: an LDS read for a later product, a product, and a share of
+  // the exponentials or maxima, which take the time of the product.  Left to itself the compiler issues the 16 products
+  // first and the 32 exponentials after them.
+  auto tile_step = [&](auto EDGE_, int n0, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
+    constexpr bool EDGE = decltype(EDGE_)::value;
+    asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
+    stage.load(a.v);              // V of the next tile (stage still points at it), in flight under the exponentials
+    stage.pages(n0 + 2 * kStep);
+    const int next = o_k + (buf ? -TILE : TILE);
     const float base = m == -INFINITY ? 0.f : m;
     float ls[4] = {0.f, 0.f, 0.f, 0.f};
+    auto weight = [&](int i) {    // of the lane's score i
+      float p = __builtin_amdgcn_exp2f(fmaf(cur[i >> 4][i & 15], sl2, -base));
+      if constexpr (!EDGE) asm volatile("" : "+v"(p));   // (holds it to its step: scheduling barriers bind no arithmetic)
+      cur[i >> 4][i & 15] = p;
+      ls[i & 3] += p;
+    };
+    if constexpr (EDGE) {
+      scores(nxt, next);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+      for (int i = 0; i < 32; ++i) weight(i);
+    } else {
+      constexpr int AHEAD = 3, N = 2 * KS;
+      auto k_frag = [&](int i) {
+        return *reinterpret_cast<const bf16x8*>(smem + (i / KS) * 32 * (D * 2) + (next ^ ((i % KS) << 5)));
+      };
+      bf16x8 f[AHEAD + 1];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(sc[kb][i], sl2, -base));
-        sc[kb][i] = p;
-        ls[i & 3] += p;
+      for (int i = 0; i < AHEAD; ++i) f[i] = k_frag(i);
+      nxt[0] = f32x16{}, nxt[1] = f32x16{};
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = k_frag(i + AHEAD);
+        nxt[i / KS] = mfma<F16>(f[i % (AHEAD + 1)], qf[i % KS], nxt[i / KS]);
+#pragma unroll
+        for (int j = 32 * i / N; j < 32 * (i + 1) / N; ++j) weight(j);
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    stage.store(nxt);
-    stage.load(a.v);   // in flight under P.V
-    stage.pages(n0 + 2 * kStep);
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int ss = 0; ss < 2; ++ss) {
-        const bf16x8 pb = pack8<F16>(sc[kb], ss);
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const char* vr = vt + (kb * 32 + 16 * ss) * (D * 2);
-          const s16x4 lo = lds_tr(vr, o_va ^ (dt << 6)), hi = lds_tr(vr, o_vb ^ (dt << 6));
-          const s16x8 vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          o[dt] = mfma<F16>(__builtin_bit_cast(bf16x8, vv), pb, o[dt]);
-        }
-      }
     if constexpr (EDGE) finite_only(n0 + kStep);
-    stage.store(nxt + TILE);
+    stage.store(smem + 2 * TILE + (buf ^ TILE));
+    stage.locate(hk);
+    stage.load(a.k);              // K of the tile after it, in flight under P.V
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bf16x8 pb = pack8<F16>(cur[i >> 1], i & 1);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) o[dt] = mfma<F16>(v_frag(i, dt), pb, o[dt]);
+      }
+      hide(nxt, n0 + kStep);
+      raise(largest(nxt));
+    } else {
+      constexpr int AHEAD = 2, N = 4 * DT;
+      bf16x8 f[AHEAD + 1], pb[2];
+#pragma unroll
+      for (int i = 0; i < AHEAD; ++i) f[i] = v_frag(i / DT, i % DT);
+      pb[0] = pack8<F16>(cur[0], 0);
+      float mx[2] = {-INFINITY, -INFINITY};
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = v_frag((i + AHEAD) / DT, (i + AHEAD) % DT);
+        o[i % DT] = mfma<F16>(f[i % (AHEAD + 1)], pb[i / DT & 1], o[i % DT]);
+        if (i % DT == 0 && i / DT < 3) pb[i / DT + 1 & 1] = pack8<F16>(cur[(i / DT + 1) >> 1], (i / DT + 1) & 1);
+#pragma unroll
+        for (int j = 32 * i / N; j < 32 * (i + 1) / N; j += 2)
+          mx[j >> 1 & 1] = fmaxf(fmaxf(mx[j >> 1 & 1], nxt[j >> 4][j & 15]), nxt[j >> 4][(j & 15) + 1]);
+        asm volatile("" : "+v"(mx[0]), "+v"(mx[1]));
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      raise(fmaxf(mx[0], mx[1]));
+    }
+    stage.store(smem + buf);
     lds_barrier();
   };
-  auto stage_only = [&](int n0) {   // a wave with nothing to see helps to stage the next tile
-    char* const nxt = smem + (buf ^ (2 * TILE));
-    stage.locate(hk);
-    stage.load(a.k);
-    stage.store(nxt);
+  auto stage_only = [&](int n0) {   // a wave with nothing to see helps to stage
     stage.load(a.v);
     stage.pages(n0 + 2 * kStep);
     finite_only(n0 + kStep);
-    stage.store(nxt + TILE);
+    stage.store(smem + 2 * TILE + (buf ^ TILE));
+    stage.locate(hk);
+    stage.load(a.k);
+    stage.store(smem + buf);
     lds_barrier();
   };
   auto turn = [&]() {
-    const int d = buf ? -2 * TILE : 2 * TILE;
-    buf ^= 2 * TILE;
+    const int d = buf ? -TILE : TILE;
+    buf ^= TILE;
     o_k += d, o_va += d, o_vb += d;
   };
   // tiles that every row sees in full, and whose next one too; the same for every wave, as are all tiles' count: the
   // barriers are shared
   const int rounds = (ntiles + KG - 1) / KG, seen = (min(pos0 + 1, k1) - k0) / kBN;
   const int inner = max(0, min(rounds, seen / KG - 1));
-  int n0 = kg;
+  int n0 = kg, t = 0;
   if (wave_last < 0) {
-    for (int t = 0; t < rounds; ++t, n0 += kStep, turn()) stage_only(n0);
-  } else {
-    for (int t = 0; t < inner; ++t, n0 += kStep, turn()) tile_step(std::false_type{}, n0);
-    for (int t = inner; t < rounds; ++t, n0 += kStep, turn()) {
-      if (n0 > wave_last || n0 >= k1) stage_only(n0);
-      else tile_step(std::true_type{}, n0);
+    if (rounds > 0) lds_barrier();
+    for (; t < rounds; ++t, n0 += kStep, turn()) stage_only(n0);
+  } else if (rounds > 0) {
+    f32x16 s0[2], s1[2];
+    scores(s0, o_k);
+    hide(s0, n0);
+    raise(largest(s0));
+    lds_barrier();   // the first K stage is read: it may be written
+    for (; t + 2 <= inner; t += 2) {   // two a turn: the scores change places
+      tile_step(std::false_type{}, n0, s0, s1);
+      n0 += kStep, turn();
+      tile_step(std::false_type{}, n0, s1, s0);
+      n0 += kStep, turn();
+    }
+    for (; t < rounds; ++t, n0 += kStep, turn()) {
+      if (n0 > wave_last || n0 >= k1) {
+        stage_only(n0);
+      } else {
+        tile_step(std::true_type{}, n0, s0, s1);
+        s0[0] = s1[0], s0[1] = s1[1];
+      }
     }
   }
 
