@@ -16,7 +16,9 @@ _HEAD_DIMS = (64, 128)
 _CHUNK_WGS = 512        # workgroups that fit the chip at once
 _CHUNK_MIN_KEYS = 256   # keys of a piece at least (128: the join costs more than the shorter pieces give)
 _FEW_ROWS = 16          # rows (query heads of a kv head times new tokens) per sequence up to which they are few, on average
-_CHUNK_GROUPS = 1
+_PAIR_TILES = 256       # tiles (of 128 rows) up to which two groups of waves share one,
+_PAIR_ROWS = 64         # if the sequences have that many rows, on average
+_MAX_KEYS = 2**31 - 2**14   # positions are 32-bit, and a tile's loads reach past its last key
 
 
 def _u(x):
@@ -122,6 +124,8 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
                          f"{_HEAD_DIMS}, at most 128)")
     if not max_blocks or not ks[0]:
         raise ValueError("chunk_attention: a cache or a block table without pages")
+    if max_blocks * bs > _MAX_KEYS:
+        raise ValueError(f"chunk_attention: a block table for {max_blocks * bs} tokens (at most {_MAX_KEYS})")
     if sk != vc.stride():
         raise ValueError("chunk_attention: the K and V caches have different strides")
     sq = q.stride()
@@ -138,7 +142,12 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
     # are left whole, their pieces' O costs more than it evens out.
     tiles = max(min(B, T), -(-T // ((16 if few else 128) // G))) * Hk
-    splits = _CHUNK_WGS // tiles if tiles < _CHUNK_WGS or not few else 4 * _CHUNK_WGS // tiles
+    # No more tiles than CUs: two groups of waves per tile, whose halves of the keys are joined through LDS (700 tokens, 32
+    # heads: 21 us, with one 30; 1,000 over 3,000, 32 heads on 8: 77 and 81; 128 over 16,000, 16 on 4: 36 and 40; the other
+    # way 2 x 2,000 over 10,000, 8 on 1: 194 and 181).  With 512 tiles it is 67 and 60, with few rows 31 and 29.
+    groups = 2 if not few and tiles <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
+    slots = _CHUNK_WGS // groups
+    splits = slots // tiles if tiles < slots or not few else 4 * slots // tiles
     splits = max(1, min(splits, max_blocks * bs // _CHUNK_MIN_KEYS, 64))
     # scratch of a split: the pieces' O, their (maximum, sum), and into how many a token's keys were split
     ws = torch.empty(splits * T * Hq * (D + 2) + T, dtype=torch.float32, device=q.device) if splits > 1 else None
@@ -146,7 +155,7 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     w1 = w0 + 4 * splits * T * Hq * D
     _launch(q.device, m.chunk_attn, int(q.dtype is torch.float16), pq, sq[0], sq[1], pk, pv, sk[0], sk[tok], sk[head],
             table.data_ptr(), max_blocks, ks[0], bs, cu.data_ptr(), lens.data_ptr(), po, so[0], so[1], B, T, Hq, Hk, D,
-            splits, _CHUNK_MIN_KEYS, scale, int(few), _CHUNK_GROUPS, w0, w1, w1 + 8 * splits * T * Hq)
+            splits, _CHUNK_MIN_KEYS, scale, int(few), groups, w0, w1, w1 + 8 * splits * T * Hq)
 
 
 def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):
