@@ -141,11 +141,14 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     # Pieces of a tile's keys.  Two workgroups fit a CU: as many pieces as fit the chip at once.  Few rows over many
     # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
     # are left whole, their pieces' O costs more than it evens out.
-    tiles = max(min(B, T), -(-T // ((16 if few else 128) // G))) * Hk
-    # No more tiles than CUs: two groups of waves per tile, whose halves of the keys are joined through LDS (700 tokens, 32
-    # heads: 21 us, with one 30; 1,000 over 3,000, 32 heads on 8: 77 and 81; 128 over 16,000, 16 on 4: 36 and 40; the other
-    # way 2 x 2,000 over 10,000, 8 on 1: 194 and 181).  With 512 tiles it is 67 and 60, with few rows 31 and 29.
-    groups = 2 if not few and tiles <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
+    per = (16 if few else 128) // G   # tokens of a tile
+    tiles = max(min(B, T), -(-T // per)) * Hk
+    # No more tiles than CUs, parts of tiles at the sequences' ends counted: two groups of waves per tile, whose halves of
+    # the keys are joined through LDS (700 tokens, 32 heads: 21 us, with one 30; 1,000 over 3,000, 32 heads on 8: 77 and 81;
+    # 128 over 16,000, 16 on 4: 36 and 40; the other way 2 x 2,000 over 10,000, 8 on 1: 194 and 181).  With 512 tiles it is
+    # 67 and 60, with mostly single tokens 56 and 45, with 64 rows per sequence no difference.
+    most = (T + min(B, T) * (per - 1)) // per * Hk
+    groups = 2 if not few and most <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
     slots = _CHUNK_WGS // groups
     splits = slots // tiles if tiles < slots or not few else 4 * slots // tiles
     splits = max(1, min(splits, max_blocks * bs // _CHUNK_MIN_KEYS, 64))
