@@ -74,9 +74,9 @@ int pd_decode_attn(const void*, long, long, const void*, const void*, long, long
                    const int*, int, float*, float*, void*, long, long, int, int, int, int, int, float, int, void*);
 int pd_cache_write(const void*, const void*, long, long, void*, void*, long, long, long, const int*, int, int,
                    const int*, const int*, int, int, int, void*);
-int pd_chunk_attn_tiles(int, int, int, int);
+long pd_chunk_attn_tiles(int, int, int, int);
 int pd_chunk_attn(int, const void*, long, long, const void*, const void*, long, long, long, const int*, int, int, int,
-                  const int*, const int*, void*, long, long, int, int, int, int, int, int, int, float, int, int,
+                  const int*, const int*, void*, long, long, int, int, int, int, int, int, int, int, int, float,
                   float*, float*, int*, void*);
 int pd_kv_copy(const uint64_t*, int, const int*, const int*, int, long, long, void*);
 int pd_sample(int, const void*, long, int, int, const float*, const float*, float, const int*, int, const float*, float,
@@ -368,19 +368,20 @@ PYBIND11_MODULE(_C, m) {
                               fmax.data(), mp2.data(), P<void*>(st)),
           "fp8_update_scale");
   });
-  m.def("chunk_attn_tiles", [](int T, int B, int G, int few) {
-    if (T < 0 || B < 0 || G < 1 || G > (few ? 16 : 128)) throw std::invalid_argument("chunk_attn_tiles: bad sizes");
-    return pd_chunk_attn_tiles(T, B, G, few);
+  m.def("chunk_attn_tiles", [](int T, int B, int G, int rows) {
+    if (T < 0 || B < 0 || G < 1 || (rows != 16 && rows != 128) || G > rows)
+      throw std::invalid_argument("chunk_attn_tiles: bad sizes");
+    return pd_chunk_attn_tiles(T, B, G, rows);
   });
   m.def("chunk_attn", [](int f16, uintptr_t q, long sq_tok, long sq_head, uintptr_t k, uintptr_t v, long s_blk,
                          long s_tok, long s_head, uintptr_t table, int max_blocks, int num_blocks, int block,
                          uintptr_t cu, uintptr_t lens, uintptr_t out, long so_tok, long so_head, int B, int T, int Hq,
-                         int Hk, int D, int splits, int min_keys, float scale, int few, int groups, uintptr_t part_o,
-                         uintptr_t part_ml, uintptr_t pieces, uintptr_t st) {
+                         int Hk, int D, int rows, int groups, int splits, int min_keys, float scale,
+                         uintptr_t part_o, uintptr_t part_ml, uintptr_t pieces, uintptr_t st) {
     check(pd_chunk_attn(f16, P<const void*>(q), sq_tok, sq_head, P<const void*>(k), P<const void*>(v), s_blk, s_tok,
                         s_head, P<const int*>(table), max_blocks, num_blocks, block, P<const int*>(cu),
-                        P<const int*>(lens), P<void*>(out), so_tok, so_head, B, T, Hq, Hk, D, splits, min_keys, scale, few, groups,
-                        P<float*>(part_o), P<float*>(part_ml), P<int*>(pieces), P<void*>(st)),
+                        P<const int*>(lens), P<void*>(out), so_tok, so_head, B, T, Hq, Hk, D, rows,
+                        groups, splits, min_keys, scale, P<float*>(part_o), P<float*>(part_ml), P<int*>(pieces), P<void*>(st)),
           "chunk_attn");
   });
   // src / dst: page numbers; every page inside the pool, no destination twice, none also a source (std::invalid_argument

@@ -5,20 +5,25 @@
 //   o = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),   s_j = scale * q . k_j
 // Token t of sequence b lives at page(b, t) * s_blk + (t % block) * s_tok + kv_head * s_head, in 64 bits.
 //
-//  * A workgroup (4 waves) owns 128 rows of one (sequence, kv head): rows are (token, query head of the group), so a
-//    K / V tile read once serves the whole group.  Its sequence is found from cu by a prefix sum over the lanes: the
-//    host never reads lengths, and the launch is the same for every batch of a shape (it can be captured).
+//  * A workgroup (4 waves, or two groups of 4) owns 128 rows of one (sequence, kv head): rows are (token, query head of
+//    the group), so a K / V tile read once serves the whole group; where a sequence has no more it owns 16 (few_rows).  Its
+//    sequence is found from cu by a prefix sum over the lanes: the host never reads lengths, and the launch is the same
+//    for every batch of a shape (it can be captured).
 //  * S^T = K . Q^T on 32x32x16 MFMA: a lane owns one row's scores, the softmax needs one exchange between lane
 //    halves, and the bf16 / fp16 P is the next product's operand as it stands.  P is rounded to 16 bits because the
 //    matrix unit takes 16-bit operands; each P is off by half a step of a value <= 2^8 relative to the row's sum,
 //    which averages out below the rounding of the output.  Scores, maxima, sums and O stay in 32 bits.
-//  * 64-key tiles go global -> registers -> LDS, two stages, page numbers one tile further ahead.  Keys past the
-//    rows' reach and pages outside the pool are read from a block of zeros, so stale pages (NaN among them) never
-//    reach a product.
+//  * 64-key tiles lie in LDS in two stages, page numbers are looked up one tile further ahead.  Where one page holds the
+//    rows of a wave's load the tiles go there straight from memory, else through registers.  Keys past the rows' reach and
+//    pages outside the pool give zeros, so stale pages (NaN among them) never reach a product.
 //  * A hidden key has P = 0, but 0 * inf is NaN: in tiles that some row does not see in full, values that are not
 //    finite enter the product as 0 and are added at the end to the rows that see them.
-//  * Few rows over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
+//  * Few tiles over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
 //    second kernel.  How often is decided per tile, from its own length.
+//
+// Measured (bf16, D = 128, 32 heads on 8, pages of 64): 2,048 tokens over 30,720 take 1,000 - 1,060 us, 1.0 PFLOP/s, bound by
+// the exponentials and maxima beside the products (two waves per SIMD: the matrix unit is busy half the time); 64 single
+// tokens over 4,000 - 8,000 take 310 us, 5.1 TB/s, the rate of a large copy.
 #include "common.h"
 
 #include <type_traits>
@@ -32,6 +37,7 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((address_space(3))) char lds_char;
 
@@ -56,7 +62,7 @@ struct Args {
   int B, T, Hq, Hk, G;
   int max_blocks, num_blocks, block, block_shift;
   unsigned block_mul;                               // key / block = key * block_mul >> block_shift, for keys < 2^31
-  int splits, min_keys, grain;                      // a piece of the keys: a multiple of grain
+  int splits, min_keys;                             // pieces of a tile's keys at most, keys of one at least
   float scale_log2;
   float *part_o, *part_ml;                          // [splits][T][Hq][D], [splits][T][Hq][2]
   int* pieces;                                      // [T] into how many a token's keys were split
@@ -65,6 +71,7 @@ struct Args {
 struct Seq {
   int b, q0, n, len, tile;   // first query row, new tokens, keys, tile within the sequence (-1: none)
 };
+constexpr int kFewRows = 16, kFewKeys = 32;   // few rows: the rows of a tile, the keys of one wave's step
 
 __device__ __forceinline__ void bounds_of(const Args& a, int b, int& q0, int& n) {
   q0 = min(max(a.cu[b], 0), a.T);
@@ -79,21 +86,29 @@ __device__ __forceinline__ int xcd_remap(int bid, int n) {
   return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + bid / 8;
 }
 
-// 64 sequences from b0, one a lane: where its queries begin, how many, its keys, and the row tiles up to and with it
+// 64 sequences from b0, one a lane: where its queries begin, how many, its keys, and the row tiles up to and with it: all of
+// 16 rows (FEW), or of 128, and beside them one of 16 for each sequence that has no more
 struct Lanes {
-  int q0, n, len, upto;
+  int q0, n, len, upto, few_upto;
 };
-__device__ __forceinline__ Lanes sequences(const Args& a, int b0, int tile_tokens, int lane) {
+template <bool FEW>
+__device__ __forceinline__ Lanes sequences(const Args& a, int b0, int lane) {
   Lanes s;
-  const int b = min(b0 + lane, a.B - 1);
+  const int b = min(b0 + lane, a.B - 1), tile_tokens = (FEW ? kFewRows : kBM) / a.G;
   bounds_of(a, b, s.q0, s.n);
   s.len = len_of(a, b);
   if (b0 + lane >= a.B) s.n = 0;
-  s.upto = (s.n + tile_tokens - 1) / tile_tokens;
+  const bool few = !FEW && s.n > 0 && s.n <= kFewRows / a.G;
+  s.upto = few ? 0 : (s.n + tile_tokens - 1) / tile_tokens;
+  s.few_upto = few ? 1 : 0;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
     const int t = __shfl_up(s.upto, o, 64);
     if (lane >= o) s.upto += t;
+    if constexpr (!FEW) {
+      const int f = __shfl_up(s.few_upto, o, 64);
+      if (lane >= o) s.few_upto += f;
+    }
   }
   return s;
 }
@@ -101,21 +116,32 @@ __device__ __forceinline__ Lanes sequences(const Args& a, int b0, int tile_token
 // This workgroup's part of the batch: a row tile, a kv head and a piece of the keys; every wave works it out for itself.
 // The grid is an upper bound of the parts there are; neighbours are the kv heads of one tile, and a sequence's tiles go
 // from the one that sees the most keys to the one that sees the fewest.
-//  STRETCHES (few rows): each XCD takes an eighth of the parts, side by side, so that the heads' rows of one key, which
-//  share lines and pages, are read by one XCD.
-//  Otherwise workgroup i has part i, and an XCD every eighth: with eight heads or a multiple each has its own heads'
+//  Few rows: each XCD takes an eighth of the parts, side by side, so that the heads' rows of one key, which share lines
+//  and pages, are read by one XCD.
+//  Many: workgroup i has part i, and an XCD every eighth: with eight heads or a multiple each has its own heads'
 //  keys in its L2, and the tiles' lengths are spread evenly.  Two workgroups share a CU, and the second of each is
 //  dispatched after the first of all: the second 32 of an XCD go from light to heavy, so that a heavy one has a light
 //  one beside it (2,048 tokens, 32 heads, nothing cached: 74 us without, all that a CU did was one weight).
-template <bool STRETCHES>
-__device__ __forceinline__ Seq find_part(const Args& a, int tile_tokens, int lane, int& hk, int& sp) {
-  Lanes s = sequences(a, 0, tile_tokens, lane);
-  int total = __builtin_amdgcn_readlane(s.upto, 63);
-  for (int b0 = 64; b0 < a.B; b0 += 64) total += __builtin_amdgcn_readlane(sequences(a, b0, tile_tokens, lane).upto, 63);
-  const int parts = total * a.Hk * a.splits;
+//  The tiles of many rows come first, those of few after them.
+template <bool FEW>
+__device__ __forceinline__ Seq find_part(const Args& a, int lane, int& hk, int& sp, bool& few) {
+  Lanes s = sequences<FEW>(a, 0, lane);
+  int total = __builtin_amdgcn_readlane(s.upto, 63), few_total = __builtin_amdgcn_readlane(s.few_upto, 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) {
+    const Lanes t = sequences<FEW>(a, b0, lane);
+    total += __builtin_amdgcn_readlane(t.upto, 63);
+    few_total += __builtin_amdgcn_readlane(t.few_upto, 63);
+  }
+  int parts = total * a.Hk * a.splits;
   int id = blockIdx.x;
+  few = FEW;
+  if (!FEW && id >= parts) {
+    id -= parts;
+    few = true;
+    parts = few_total * a.Hk * a.splits;
+  }
   if (id >= parts) return Seq{0, 0, 0, 0, -1};
-  if (STRETCHES) {
+  if (few) {
     id = xcd_remap(id, parts);
   } else {
     const int per = parts / 8;   // (full rows of eight)
@@ -126,7 +152,8 @@ __device__ __forceinline__ Seq find_part(const Args& a, int tile_tokens, int lan
   const int tile = id / (a.Hk * a.splits);
   int base = 0, b0 = 0;
   for (;;) {
-    const unsigned long long hit = __ballot(base + s.upto > tile);   // some lane, tile < total
+    const int upto = !FEW && few ? s.few_upto : s.upto;
+    const unsigned long long hit = __ballot(base + upto > tile);   // some lane, tile < total
     if (hit) {
       const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)hit) - 1);
       Seq r;
@@ -135,21 +162,21 @@ __device__ __forceinline__ Seq find_part(const Args& a, int tile_tokens, int lan
       r.n = __builtin_amdgcn_readlane(s.n, l);
       r.len = __builtin_amdgcn_readlane(s.len, l);
       // the tile that sees the most keys first
-      r.tile = __builtin_amdgcn_readlane(s.upto, l) - 1 - (tile - base);
+      r.tile = __builtin_amdgcn_readlane(upto, l) - 1 - (tile - base);
       return r;
     }
-    base += __builtin_amdgcn_readlane(s.upto, 63);
+    base += __builtin_amdgcn_readlane(upto, 63);
     b0 += 64;
     if (b0 >= a.B) return Seq{0, 0, 0, 0, -1};
-    s = sequences(a, b0, tile_tokens, lane);
+    s = sequences<FEW>(a, b0, lane);
   }
 }
 
 // keys per piece of a tile that sees `keys` keys: whole grains, at least min_keys, at most `splits` pieces
-__device__ __forceinline__ int piece_of(const Args& a, int keys) {
+__device__ __forceinline__ int piece_of(const Args& a, int keys, int grain) {
   const int pieces = max(1, min(a.splits, (keys + a.min_keys - 1) / a.min_keys));
   const int per = (keys + pieces - 1) / pieces;
-  return max((per + a.grain - 1) / a.grain * a.grain, a.grain);
+  return max((per + grain - 1) / grain * grain, grain);
 }
 
 template <int D>
@@ -196,29 +223,270 @@ __device__ __forceinline__ int block_of(const Args& a, int key) {
   return (int)(((unsigned long long)(unsigned)key * a.block_mul) >> a.block_shift);
 }
 
-// A K or V tile on its way from the pages to LDS: a thread loads chunk tid % NCH of rows tid / NCH + ROWS * i.
+// Few rows (decoding, drafted tokens): 16 rows of one (sequence, kv head) per workgroup, bound by the reads of K and V.
+// Each of the W waves takes every W-th 32-key tile of the piece on its own, with no barrier in the loop:
+//  * S^T = K . Q^T on 16x16x32 MFMA; a lane loads its K operands (16 bytes of a key's row) straight into registers, V goes
+//    through a wave's own LDS image for the transposed reads;
+//  * two register sets in turn: 32 loads of 16 bytes a lane are in flight (D = 128), page numbers one tile further ahead;
+//  * the waves' (m, l, O) are joined through LDS at the end.
+// A step that mixes single tokens with pieces of prompts has both kinds of tiles in one launch: 45 sequences over 1,250 -
+// 2,500 keys, 33 of them single tokens, take 44 us, with 128-row tiles for all of them 48 (D = 64, 16 heads on 4).  Where
+// few rows are all there is, a kernel of their own with a quarter of the LDS and smaller pieces: 64 single tokens over 4,000
+// - 8,000 keys take 311 us in it, 338 in the other; 8 x 4 drafted tokens over 350 - 700 take 22 in both.
+
+template <bool F16>
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+template <int D, bool F16, int W>
+__device__ __forceinline__ void few_rows(const Args& a, const Seq& s, int hk, int sp, char* lds) {
+  constexpr int KC = D / 32, DT = D / 16;
+  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;
+  // lds: W * kFewKeys * D * 2 bytes, the waves' V images, then their O
+  __shared__ float ml[W][kFewRows][2];
+  __shared__ int odd_values;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c16 = lane & 15, h = lane >> 4;
+  const int tile_tokens = kFewRows / a.G;
+  const int tok0 = s.tile * tile_tokens, ntok = min(tile_tokens, s.n - tok0);
+  const int pos0 = s.len - s.n + tok0, keys = max(pos0 + ntok, 0);
+  const int piece = piece_of(a, keys, W * kFewKeys), k0 = sp * piece, k1 = min(keys, k0 + piece);
+  const bool whole = piece >= keys;
+  if (a.splits > 1 && sp == 0 && hk == 0 && tid < ntok) a.pieces[s.q0 + tok0 + tid] = whole ? 1 : (keys + piece - 1) / piece;
+  if (sp > 0 && k0 >= keys) return;
+  if (tid == 0) odd_values = 0;
+  lds_barrier();
+
+  const int rt = c16 / a.G, rh = hk * a.G + c16 % a.G, pos = pos0 + rt;
+  const bool live = rt < ntok;
+  bf16x8 qf[KC];
+  {
+    const unsigned short* qp = a.q + (long)(s.q0 + tok0 + (live ? rt : 0)) * a.sq_tok + (long)(live ? rh : 0) * a.sq_head + 8 * h;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      qf[c] = *reinterpret_cast<const bf16x8*>(qp + 32 * c);
+      if (!live) qf[c] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    }
+  }
+  const int* tab = a.table + (long)s.b * a.max_blocks;
+  const unsigned head_off = hk * a.s_head + 8 * h;
+  const int ntiles = k1 > k0 ? (k1 - k0 + kFewKeys - 1) / kFewKeys : 0;
+  auto pages = [&](int t, int (&pg)[2]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) pg[u] = tab[block_of(a, min(k0 + kFewKeys * t + 16 * u + c16, k1 - 1))];
+  };
+  auto load = [&](int t, const int (&pg)[2], u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = k0 + kFewKeys * t + 16 * u + c16, blk = block_of(a, key);
+      const bool ok = key < k1 && (unsigned)pg[u] < (unsigned)a.num_blocks;
+      const long off = (long)pg[u] * a.s_blk + (unsigned)((key - blk * a.block) * a.s_tok + head_off);
+      global_u16x8 *pk = row_or_zeros(ok, a.k + off), *pv = row_or_zeros(ok, a.v + off);
+#pragma unroll
+      for (int c = 0; c < KC; ++c) {
+        kk[u][c] = pk[4 * c];
+        vv[u][c] = pv[4 * c];
+      }
+    }
+  };
+  f32x4 o[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  const float sl2 = a.scale_log2;
+  char* const vl = lds + w * (kFewKeys * D * 2);
+  const int qq = c16 >> 2, pp = c16 & 3;
+  // (16 rows further down the swizzle is the same, and a chunk is an XOR)
+  int o_w = c16 * (D * 2) + 16 * swz<D>(c16, h);
+  int o_r = (4 * h + qq) * (D * 2) + 16 * swz<D>(4 * h + qq, pp >> 1) + 8 * (pp & 1);
+  auto compute = [&](int t, const u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
+    const int n0 = k0 + kFewKeys * t;
+    asm volatile("" : "+v"(o_w), "+v"(o_r));   // the XORs stay in the loop: hoisted they spilled
+    if (n0 + kFewKeys - 1 > pos0) {   // some row does not see all of it: values that are not finite are put in at the end
+      constexpr unsigned kE = kExp | (unsigned)kExp << 16, kLow = F16 ? 0x04000400u : 0x00800080u;
+      unsigned hit = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const auto x = __builtin_bit_cast(u32x4, vv[u][c]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) hit |= (x[j] & kE) + kLow;
+        }
+      if (__builtin_expect(hit & 0x80008000u, 0)) {
+        odd_values = 1;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < KC; ++c)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vv[u][c][j] = (vv[u][c][j] & kExp) == kExp ? (unsigned short)0 : vv[u][c][j];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+        *reinterpret_cast<u16x8*>(vl + (o_w ^ (c << 6)) + 16 * u * (D * 2)) = vv[u][c];
+    f32x4 sc[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < KC; ++c) sc[u] = mfma16<F16>(__builtin_bit_cast(bf16x8, kk[u][c]), qf[c], sc[u]);
+    }
+    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 16 u + 4 h + e is hidden iff 16 u + e >= lim
+    float mt = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sc[u][e] = 16 * u + e >= lim ? -INFINITY : sc[u][e] * sl2;
+        mt = fmaxf(mt, sc[u][e]);
+      }
+    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - base);
+    m = mn;
+    bf16x8 pf;
+    float ps = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = __builtin_amdgcn_exp2f(sc[u][e] - base);
+        ps += p;
+        pf[4 * u + e] = __builtin_bit_cast(__bf16, cvt16<F16>(p));
+      }
+    l = l * alpha + ps;
+    float ar[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ar[e] = __shfl(alpha, 4 * h + e, 64);   // O's row 4 h + e has its state in that lane
+#pragma unroll
+    for (int t2 = 0; t2 < DT; ++t2) {
+      const s16x4 lo = lds_tr(vl, o_r ^ (t2 << 5)), hi = lds_tr(vl + 16 * (D * 2), o_r ^ (t2 << 5));
+      const s16x8 v8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[t2][e] *= ar[e];
+      o[t2] = mfma16<F16>(pf, __builtin_bit_cast(bf16x8, v8), o[t2]);
+    }
+  };
+  // Two tiles a turn without an exit between them; past the last tile keys are hidden and loads read zeros
+  u16x8 ka[2][KC], va[2][KC], kb[2][KC], vb[2][KC];
+  if (w < ntiles) {
+    int pa[2], pb[2];
+    pages(w, pa);
+    pages(w + W, pb);
+    load(w, pa, ka, va);
+    for (int t = w; t < ntiles; t += 2 * W) {
+      pages(t + 2 * W, pa);
+      load(t + W, pb, kb, vb);
+      __builtin_amdgcn_sched_barrier(0);   // the loads stay ahead of the work
+      compute(t, ka, va);
+      pages(t + 3 * W, pb);
+      load(t + 2 * W, pa, ka, va);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(t + W, kb, vb);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  __syncthreads();   // every wave is done with its V image
+  float* const ow = reinterpret_cast<float*>(lds);   // [W][16][D]
+  if (h == 0) {
+    ml[w][c16][0] = m;
+    ml[w][c16][1] = l;
+  }
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) ow[(w * kFewRows + 4 * h + e) * D + 16 * t + c16] = o[t][e];
+  __syncthreads();
+  const int rows = ntok * a.G;
+  for (int i = tid; i < rows * (D / 4); i += 64 * W) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float M = -INFINITY, L = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int x = 0; x < W; ++x) M = fmaxf(M, ml[x][row][0]);
+    const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int x = 0; x < W; ++x) {
+      const float wt = __builtin_amdgcn_exp2f(ml[x][row][0] - base);
+      L += ml[x][row][1] * wt;
+      acc += *reinterpret_cast<const f32x4*>(ow + (x * kFewRows + row) * D + d) * wt;
+    }
+    const int tok = row / a.G, hq = hk * a.G + row % a.G;
+    if (__builtin_expect(odd_values, 0)) {   // the values that were taken out, where this row sees them
+      for (int j = k0 + max(pos0 - k0, 0) / kFewKeys * kFewKeys; j < k1 && j <= pos0 + tok; ++j) {
+        const int blk = block_of(a, j), page = tab[blk];
+        if ((unsigned)page >= (unsigned)a.num_blocks) continue;
+        const unsigned short* vr = a.v + (long)page * a.s_blk + (unsigned)((j - blk * a.block) * a.s_tok + hk * a.s_head) + d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if ((vr[e] & kExp) == kExp) acc[e] += F16 ? h2f(vr[e]) : bf2f(vr[e]);
+      }
+    }
+    const long trow = s.q0 + tok0 + tok;
+    if (whole) {
+      const float inv = L != 0.f ? 1.f / L : 0.f;
+      typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
+      u16x4 r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = cvt16<F16>(acc[e] * inv);
+      *reinterpret_cast<u16x4*>(a.out + trow * a.so_tok + (long)hq * a.so_head + d) = r;
+    } else {
+      const long pi = ((long)sp * a.T + trow) * a.Hq + hq;
+      *reinterpret_cast<f32x4*>(a.part_o + pi * D + d) = acc;
+      if (d == 0) {
+        a.part_ml[pi * 2] = M;
+        a.part_ml[pi * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+template <int D, bool F16>
+__global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * kFewKeys * D * 2];
+  int hk, sp;
+  bool few;
+  const Seq s = find_part<true>(a, threadIdx.x & 63, hk, sp, few);
+  if (s.tile >= 0) few_rows<D, F16, 4>(a, s, hk, sp, lds);
+}
+
+// A K or V tile on its way from the pages to LDS: a thread brings chunk tid % NCH of rows tid / NCH + ROWS * i.
 // UNI: the block size is a multiple of the RW rows that one wave's load covers, so a wave's rows of a load lie in one page.
 // Lane i works out load i's page, byte offset and extent, and the load is a buffer load from a scalar base whose extent
 // ends with the valid rows (past it, and for page numbers outside the pool, it reads zeros): K and V share all of that.
-// Otherwise every thread looks up its own rows' pages and points the missing ones at a block of zeros.
+// It goes to LDS without passing registers, whose order of chunks the lanes' addresses have to follow then.
+// Otherwise every thread looks up its own rows' pages, points the missing ones at a block of zeros, and stores what it
+// loaded.
 template <int D, bool UNI>
 struct Stage {
   static constexpr int NCH = D / 8, NLOAD = kBN * NCH / 256, ROWS = 256 / NCH, RW = 64 / NCH;
   const Args& a;
   const int* tab;
   int k1, first_row, o_st, voff;
-  int page[UNI ? 1 : NLOAD], rest[UNI ? 1 : NLOAD], extent;   // of the tile to come
-  u16x8 st[NLOAD];
+  int page[UNI ? 1 : NLOAD], rest[UNI ? 1 : NLOAD], rows;   // of the tile to come
+  unsigned lo[NLOAD], hi[NLOAD];                            // UNI: of the present one (scalar)
+  int bytes[NLOAD];
+  u16x8 st[UNI ? 1 : NLOAD];
   __device__ __forceinline__ Stage(const Args& a_, const Seq& s, int hk, int tid, int k1_) : a(a_) {
     tab = a.table + (long)s.b * a.max_blocks;
     k1 = k1_;
-    const int lrow = tid / NCH, lch = tid % NCH;
     // (the swizzle has the row's lowest 4 bits, which ROWS leaves alone)
-    o_st = lrow * (D * 2) + swz<D>(lrow, lch) * 16;
+    const int lrow = tid / NCH, lch = tid % NCH, sch = swz<D>(lrow, lch);
     if constexpr (UNI) {
+      o_st = __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
       first_row = (tid >> 6) * RW + ROWS * (tid & (NLOAD - 1));
-      voff = (lrow % RW) * a.s_tok * 2 + (hk * a.s_head + lch * 8) * 2;
+      voff = (lrow % RW) * a.s_tok * 2 + (hk * a.s_head + sch * 8) * 2;
     } else {
+      o_st = lrow * (D * 2) + sch * 16;
       first_row = lrow;
       voff = hk * a.s_head + lch * 8;
     }
@@ -230,29 +498,44 @@ struct Stage {
       const int key = n0 + first_row + ROWS * i, blk = block_of(a, min(key, k1 - 1));
       page[i] = tab[blk];
       rest[i] = (key - blk * a.block) * a.s_tok;
-      if constexpr (UNI) extent = min(max(k1 - key, 0), RW);
+      if constexpr (UNI) rows = min(max(k1 - key, 0), RW);
       else rest[i] = key < k1 ? rest[i] : -1;
     }
   }
   // where they lie, once they have arrived: K and V alike
-  unsigned lo, hi;
   __device__ __forceinline__ void locate(int hk) {
     if constexpr (UNI) {
       const unsigned long long off = ((unsigned long long)(unsigned)page[0] * (unsigned)a.s_blk + (unsigned)rest[0]) * 2;
-      lo = (unsigned)off, hi = (unsigned)(off >> 32);
+      const bool ok = (unsigned)page[0] < (unsigned)a.num_blocks && rows > 0;
       // (rows of other heads may lie between: the extent reaches to the end of the last row's head)
-      extent = (unsigned)page[0] < (unsigned)a.num_blocks && extent > 0 ? ((extent - 1) * a.s_tok + hk * a.s_head + D) * 2 : 0;
+      const int b = ok ? ((rows - 1) * a.s_tok + hk * a.s_head + D) * 2 : 0;
+#pragma unroll
+      for (int i = 0; i < NLOAD; ++i) {
+        lo[i] = __builtin_amdgcn_readlane((int)(unsigned)off, i);
+        hi[i] = __builtin_amdgcn_readlane((int)(unsigned)(off >> 32), i);
+        bytes[i] = __builtin_amdgcn_readlane(b, i);
+      }
     }
   }
-  __device__ __forceinline__ void load(const unsigned short* cache) {
+  __device__ __forceinline__ void load(const unsigned short* cache, char* dst) {
 #pragma unroll
-    for (int i = 0; i < NLOAD; ++i) {
+    for (int i = 0; i < NLOAD; ++i) load(i, cache, dst);
+  }
+  __device__ __forceinline__ void load(int i, const unsigned short* cache, char* dst) {
+    {
       if constexpr (UNI) {
-        const unsigned long long off = (unsigned)__builtin_amdgcn_readlane((int)lo, i) |
-                                       (unsigned long long)(unsigned)__builtin_amdgcn_readlane((int)hi, i) << 32;
-        const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
-            (void*)((unsigned long long)cache + off), (short)0, __builtin_amdgcn_readlane(extent, i), 0x00020000);
-        st[i] = __builtin_bit_cast(u16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, voff, 0, 0));
+        const unsigned long long at = (unsigned long long)cache + (lo[i] | (unsigned long long)hi[i] << 32);
+        const i32x4 rs = {(int)at, (int)(at >> 32) & 0xffff, bytes[i], 0x00020000};
+        const unsigned m0 = (unsigned)(size_t)(lds_char*)dst + o_st + i * ROWS * (D * 2);
+        // (five wait states between a lane read and a buffer's use of its result; the compiler counts none inside here.
+        // Its own waits for LDS reads would wait for every such load: nothing here tells it that they don't meet)
+        asm volatile(
+            "s_mov_b32 m0, %0\n\t"
+            "s_nop 4\n\t"
+            "buffer_load_dwordx4 %1, %2, 0 offen lds"
+            :
+            : "s"(m0), "v"(voff), "s"(rs)
+            : "memory", "m0");
       } else {
         const bool ok = rest[i] >= 0 && (unsigned)page[i] < (unsigned)a.num_blocks;
         const unsigned short* p = cache + (long)page[i] * a.s_blk + (unsigned)(rest[i] + voff);
@@ -261,8 +544,17 @@ struct Stage {
     }
   }
   __device__ __forceinline__ void store(char* dst) const {
+    if constexpr (!UNI) {
 #pragma unroll
-    for (int i = 0; i < NLOAD; ++i) *reinterpret_cast<u16x8*>(dst + o_st + i * ROWS * (D * 2)) = st[i];
+      for (int i = 0; i < NLOAD; ++i) *reinterpret_cast<u16x8*>(dst + o_st + i * ROWS * (D * 2)) = st[i];
+    }
+  }
+  __device__ __forceinline__ void take(const Stage& s) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; ++i) lo[i] = s.lo[i], hi[i] = s.hi[i], bytes[i] = s.bytes[i];
+  }
+  __device__ __forceinline__ void arrived() const {
+    if constexpr (UNI) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
 };
 
@@ -283,13 +575,18 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   const int tile_tokens = kBM / a.G;
 
   int hk, sp;
-  const Seq s = find_part<false>(a, tile_tokens, lane, hk, sp);
+  bool few;
+  const Seq s = find_part<false>(a, lane, hk, sp, few);
   if (s.tile < 0) return;
+  if (few) {
+    few_rows<D, F16, 4 * KG>(a, s, hk, sp, lds);
+    return;
+  }
   const int tok0 = s.tile * tile_tokens;                        // first token of the tile within the sequence
   const int ntok = min(tile_tokens, s.n - tok0);
   const int pos0 = s.len - s.n + tok0;                          // its position (negative: it sees nothing)
   const int keys = max(pos0 + ntok, 0);                         // keys the tile's last token sees
-  const int piece = piece_of(a, keys);
+  const int piece = piece_of(a, keys, kBN);
   const int k0 = sp * piece, k1 = min(keys, k0 + piece);
   const bool whole = piece >= keys;
   if (a.splits > 1 && sp == 0 && hk == 0)
@@ -312,23 +609,31 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   }
 
   St stage(a, s, hk, tid, k1);
-  // V rows in registers, of a tile that some row does not see in full: values that are not finite become 0 (rare)
-  auto finite_only = [&](int n0) {
+  // The thread's share of a V tile at n0 that some row does not see in full: values that are not finite become 0 (rare).
+  // UNI: it lies in LDS at dst, else still in registers
+  auto finite_only = [&](int n0, char* dst) {
     if (n0 + kBN - 1 <= pos0) return;
     constexpr unsigned kE = kExp | (unsigned)kExp << 16, kLow = F16 ? 0x04000400u : 0x00800080u;
     unsigned hit = 0;   // exponent + its lowest bit carries into bit 15 iff all exponent bits are set
+    auto share = [&](int i) -> u16x8& {
+      if constexpr (UNI) return *reinterpret_cast<u16x8*>(dst + tid * 16 + i * (St::ROWS * D * 2));
+      else return stage.st[i];
+    };
 #pragma unroll
     for (int i = 0; i < NLOAD; ++i) {
-      const auto w = __builtin_bit_cast(u32x4, stage.st[i]);
+      const auto w = __builtin_bit_cast(u32x4, share(i));
 #pragma unroll
       for (int j = 0; j < 4; ++j) hit |= (w[j] & kE) + kLow;
     }
     if (__builtin_expect(hit & 0x80008000u, 0)) {
       odd_values = 1;
 #pragma unroll
-      for (int i = 0; i < NLOAD; ++i)
+      for (int i = 0; i < NLOAD; ++i) {
+        u16x8 v = share(i);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) stage.st[i][j] = (stage.st[i][j] & kExp) == kExp ? (unsigned short)0 : stage.st[i][j];
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] & kExp) == kExp ? (unsigned short)0 : v[j];
+        share(i) = v;
+      }
     }
   };
 
@@ -349,17 +654,29 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   // tiles ahead and V one (K and V have two stages each: a stage is written in the round after its last read).
   if (ntiles > 0) {
     stage.pages(kg);
-    stage.locate(hk);
-    stage.load(a.k);
-    St first(stage);   // (K and V on their way together)
-    stage.load(a.v);
-    stage.pages(kg + kStep);
-    first.store(smem);
-    finite_only(kg);
-    stage.store(smem + 2 * TILE);
-    stage.locate(hk);
-    stage.load(a.k);
-    stage.store(smem + TILE);
+    if constexpr (UNI) {   // K and V of the first tile and K of the second, all on their way together
+      St next(stage);
+      next.pages(kg + kStep);
+      stage.locate(hk);
+      stage.load(a.k, smem);
+      stage.load(a.v, smem + 2 * TILE);
+      next.locate(hk);
+      next.load(a.k, smem + TILE);
+      stage.take(next);
+      stage.pages(kg + 2 * kStep);
+      stage.arrived();
+      finite_only(kg, smem + 2 * TILE);
+    } else {
+      stage.load(a.k, smem);
+      St first(stage);
+      stage.load(a.v, smem);
+      stage.pages(kg + kStep);
+      first.store(smem);
+      finite_only(kg, smem);
+      stage.store(smem + 2 * TILE);
+      stage.load(a.k, smem);
+      stage.store(smem + TILE);
+    }
   }
   lds_barrier();
 
@@ -418,6 +735,42 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
     const s16x8 vv = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(bf16x8, vv);
   };
+  // The staging of a turn: V of the next tile, K of the one after it, and the pages of a later one are looked up.
+  // Through registers V is loaded at the turn's start and stored at its middle, K loaded then and stored at its end; straight
+  // to LDS both are loaded at the start and there at the end.
+  auto stage_begin = [&](int n0) {
+    stage.load(a.v, smem + 2 * TILE + (buf ^ TILE));
+    if constexpr (UNI) {
+      stage.locate(hk);
+      stage.load(a.k, smem + buf);
+      stage.pages(n0 + 3 * kStep);
+    } else {
+      stage.pages(n0 + 2 * kStep);
+    }
+  };
+  auto stage_middle = [&](int n0, bool edge) {
+    if constexpr (!UNI) {
+      char* const dst = smem + 2 * TILE + (buf ^ TILE);
+      if (edge) finite_only(n0 + kStep, dst);
+      stage.store(dst);
+      stage.locate(hk);
+      stage.load(a.k, smem);
+    }
+  };
+  auto stage_end = [&](int n0, bool edge) {
+    stage.store(smem + buf);
+    stage.arrived();
+    if (UNI && edge) finite_only(n0 + kStep, smem + 2 * TILE + (buf ^ TILE));
+    lds_barrier();
+  };
+  // the same in 2 * KS steps
+  auto stage_step = [&](int i, int n0) {
+    constexpr int N = KS, EVERY = N / NLOAD;   // V over the first KS steps, then K
+    if (i < N && i % EVERY == 0) stage.load(i / EVERY, a.v, smem + 2 * TILE + (buf ^ TILE));
+    if (i == N) stage.locate(hk);
+    if (i >= N && i % EVERY == 0) stage.load((i - N) / EVERY, a.k, smem + buf);
+    if (i == 2 * N - 1) stage.pages(n0 + 3 * kStep);
+  };
   // One tile, whose scores are in cur, the next one's in nxt at the end.  EDGE: some row may not see all keys of the next
   // tile (two loops, one body each: with both in one loop O was copied between registers at their joint).
   // The order of the inner body is written down step by step: an LDS read for a later product, a product, and a share of
@@ -426,8 +779,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   auto tile_step = [&](auto EDGE_, int n0, f32x16 (&cur)[2], f32x16 (&nxt)[2]) {
     constexpr bool EDGE = decltype(EDGE_)::value;
     asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
-    stage.load(a.v);              // V of the next tile (stage still points at it), in flight under the exponentials
-    stage.pages(n0 + 2 * kStep);
+    if constexpr (!UNI) stage_begin(n0);
     const int next = o_k + (buf ? -TILE : TILE);
     const float base = m == -INFINITY ? 0.f : m;
     float ls[4] = {0.f, 0.f, 0.f, 0.f};
@@ -439,6 +791,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
     };
     if constexpr (EDGE) {
       scores(nxt, next);
+      if constexpr (UNI) stage_begin(n0);
 #pragma unroll
       for (int i = 0; i < 32; ++i) weight(i);
     } else {
@@ -455,16 +808,14 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
       for (int i = 0; i < N; ++i) {
         if (i + AHEAD < N) f[(i + AHEAD) % (AHEAD + 1)] = k_frag(i + AHEAD);
         nxt[i / KS] = mfma<F16>(f[i % (AHEAD + 1)], qf[i % KS], nxt[i / KS]);
+        if constexpr (UNI) stage_step(i, n0);
 #pragma unroll
         for (int j = 32 * i / N; j < 32 * (i + 1) / N; ++j) weight(j);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
-    if constexpr (EDGE) finite_only(n0 + kStep);
-    stage.store(smem + 2 * TILE + (buf ^ TILE));
-    stage.locate(hk);
-    stage.load(a.k);              // K of the tile after it, in flight under P.V
+    stage_middle(n0, EDGE);
     if constexpr (EDGE) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -495,18 +846,12 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
       }
       raise(fmaxf(mx[0], mx[1]));
     }
-    stage.store(smem + buf);
-    lds_barrier();
+    stage_end(n0, EDGE);
   };
   auto stage_only = [&](int n0) {   // a wave with nothing to see helps to stage
-    stage.load(a.v);
-    stage.pages(n0 + 2 * kStep);
-    finite_only(n0 + kStep);
-    stage.store(smem + 2 * TILE + (buf ^ TILE));
-    stage.locate(hk);
-    stage.load(a.k);
-    stage.store(smem + buf);
-    lds_barrier();
+    stage_begin(n0);
+    stage_middle(n0, true);
+    stage_end(n0, true);
   };
   auto turn = [&]() {
     const int d = buf ? -TILE : TILE;
@@ -621,231 +966,6 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
   }
 }
 
-// Few rows (decoding, drafted tokens): 16 rows of one (sequence, kv head) per workgroup, bound by the reads of K and V.
-// Each of the four waves takes every fourth 32-key tile of the piece on its own, with no barrier in the loop:
-//  * S^T = K . Q^T on 16x16x32 MFMA; a lane loads its K operands (16 bytes of a key's row) straight into registers, V goes
-//    through a wave's own LDS image for the transposed reads;
-//  * two register sets in turn: 32 loads of 16 bytes a lane are in flight (D = 128), page numbers one tile further ahead;
-//  * the waves' (m, l, O) are joined through LDS at the end.
-// The tiled kernel above needs 20 us for 8 x 4 drafted tokens over 350 - 700 keys, most of it the latency of its steps.
-template <bool F16>
-__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
-  if constexpr (F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-}
-
-constexpr int kFewRows = 16, kFewKeys = 32;
-
-template <int D, bool F16>
-__global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
-  constexpr int KC = D / 32, DT = D / 16;
-  constexpr unsigned short kExp = F16 ? 0x7c00 : 0x7f80;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kFewKeys * D * 2];   // the waves' V images, then their O
-  __shared__ float ml[4][kFewRows][2];
-  __shared__ int odd_values;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c16 = lane & 15, h = lane >> 4;
-  const int tile_tokens = kFewRows / a.G;
-  int hk, sp;
-  const Seq s = find_part<true>(a, tile_tokens, lane, hk, sp);
-  if (s.tile < 0) return;
-  const int tok0 = s.tile * tile_tokens, ntok = min(tile_tokens, s.n - tok0);
-  const int pos0 = s.len - s.n + tok0, keys = max(pos0 + ntok, 0);
-  const int piece = piece_of(a, keys), k0 = sp * piece, k1 = min(keys, k0 + piece);
-  const bool whole = piece >= keys;
-  if (a.splits > 1 && sp == 0 && hk == 0 && tid < ntok) a.pieces[s.q0 + tok0 + tid] = whole ? 1 : (keys + piece - 1) / piece;
-  if (sp > 0 && k0 >= keys) return;
-  if (tid == 0) odd_values = 0;
-  lds_barrier();
-
-  const int rt = c16 / a.G, rh = hk * a.G + c16 % a.G, pos = pos0 + rt;
-  const bool live = rt < ntok;
-  bf16x8 qf[KC];
-  {
-    const unsigned short* qp = a.q + (long)(s.q0 + tok0 + (live ? rt : 0)) * a.sq_tok + (long)(live ? rh : 0) * a.sq_head + 8 * h;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      qf[c] = *reinterpret_cast<const bf16x8*>(qp + 32 * c);
-      if (!live) qf[c] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    }
-  }
-  const int* tab = a.table + (long)s.b * a.max_blocks;
-  const unsigned head_off = hk * a.s_head + 8 * h;
-  const int ntiles = k1 > k0 ? (k1 - k0 + kFewKeys - 1) / kFewKeys : 0;
-  auto pages = [&](int t, int (&pg)[2]) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) pg[u] = tab[block_of(a, min(k0 + kFewKeys * t + 16 * u + c16, k1 - 1))];
-  };
-  auto load = [&](int t, const int (&pg)[2], u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int key = k0 + kFewKeys * t + 16 * u + c16, blk = block_of(a, key);
-      const bool ok = key < k1 && (unsigned)pg[u] < (unsigned)a.num_blocks;
-      const long off = (long)pg[u] * a.s_blk + (unsigned)((key - blk * a.block) * a.s_tok + head_off);
-      global_u16x8 *pk = row_or_zeros(ok, a.k + off), *pv = row_or_zeros(ok, a.v + off);
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        kk[u][c] = pk[4 * c];
-        vv[u][c] = pv[4 * c];
-      }
-    }
-  };
-  f32x4 o[DT];
-#pragma unroll
-  for (int t = 0; t < DT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
-  const float sl2 = a.scale_log2;
-  char* const vl = lds + w * (kFewKeys * D * 2);
-  const int qq = c16 >> 2, pp = c16 & 3;
-  auto compute = [&](int t, const u16x8 (&kk)[2][KC], u16x8 (&vv)[2][KC]) {
-    const int n0 = k0 + kFewKeys * t;
-    if (n0 + kFewKeys - 1 > pos0) {   // some row does not see all of it: values that are not finite are put in at the end
-      constexpr unsigned kE = kExp | (unsigned)kExp << 16, kLow = F16 ? 0x04000400u : 0x00800080u;
-      unsigned hit = 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const auto x = __builtin_bit_cast(u32x4, vv[u][c]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) hit |= (x[j] & kE) + kLow;
-        }
-      if (__builtin_expect(hit & 0x80008000u, 0)) {
-        odd_values = 1;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int c = 0; c < KC; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) vv[u][c][j] = (vv[u][c][j] & kExp) == kExp ? (unsigned short)0 : vv[u][c][j];
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-        *reinterpret_cast<u16x8*>(vl + (16 * u + c16) * (D * 2) + 16 * swz<D>(16 * u + c16, 4 * c + h)) = vv[u][c];
-    f32x4 sc[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      sc[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < KC; ++c) sc[u] = mfma16<F16>(__builtin_bit_cast(bf16x8, kk[u][c]), qf[c], sc[u]);
-    }
-    const int lim = min(k1, pos + 1) - n0 - 4 * h;   // key n0 + 16 u + 4 h + e is hidden iff 16 u + e >= lim
-    float mt = -INFINITY;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[u][e] = 16 * u + e >= lim ? -INFINITY : sc[u][e] * sl2;
-        mt = fmaxf(mt, sc[u][e]);
-      }
-    mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-    mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
-    m = mn;
-    bf16x8 pf;
-    float ps = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = __builtin_amdgcn_exp2f(sc[u][e] - base);
-        ps += p;
-        pf[4 * u + e] = __builtin_bit_cast(__bf16, cvt16<F16>(p));
-      }
-    l = l * alpha + ps;
-    float ar[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ar[e] = __shfl(alpha, 4 * h + e, 64);   // O's row 4 h + e has its state in that lane
-#pragma unroll
-    for (int t2 = 0; t2 < DT; ++t2) {
-      const s16x4 lo = lds_tr(vl, (4 * h + qq) * (D * 2) + 16 * swz<D>(4 * h + qq, 2 * t2 + (pp >> 1)) + 8 * (pp & 1));
-      const s16x4 hi = lds_tr(vl, (16 + 4 * h + qq) * (D * 2) + 16 * swz<D>(16 + 4 * h + qq, 2 * t2 + (pp >> 1)) + 8 * (pp & 1));
-      const s16x8 v8 = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[t2][e] *= ar[e];
-      o[t2] = mfma16<F16>(pf, __builtin_bit_cast(bf16x8, v8), o[t2]);
-    }
-  };
-  // Two tiles a turn without an exit between them; past the last tile keys are hidden and loads read zeros
-  u16x8 ka[2][KC], va[2][KC], kb[2][KC], vb[2][KC];
-  if (w < ntiles) {
-    int pa[2], pb[2];
-    pages(w, pa);
-    pages(w + 4, pb);
-    load(w, pa, ka, va);
-    for (int t = w; t < ntiles; t += 8) {
-      pages(t + 8, pa);
-      load(t + 4, pb, kb, vb);
-      __builtin_amdgcn_sched_barrier(0);   // the loads stay ahead of the work
-      compute(t, ka, va);
-      pages(t + 12, pb);
-      load(t + 8, pa, ka, va);
-      __builtin_amdgcn_sched_barrier(0);
-      compute(t + 4, kb, vb);
-    }
-  }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
-  __syncthreads();   // every wave is done with its V image
-  float* const ow = reinterpret_cast<float*>(lds);   // [4][16][D]
-  if (h == 0) {
-    ml[w][c16][0] = m;
-    ml[w][c16][1] = l;
-  }
-#pragma unroll
-  for (int t = 0; t < DT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) ow[(w * kFewRows + 4 * h + e) * D + 16 * t + c16] = o[t][e];
-  __syncthreads();
-  const int rows = ntok * a.G;
-  for (int i = tid; i < rows * (D / 4); i += 256) {
-    const int row = i / (D / 4), d = i % (D / 4) * 4;
-    float M = -INFINITY, L = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int x = 0; x < 4; ++x) M = fmaxf(M, ml[x][row][0]);
-    const float base = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const float wt = __builtin_amdgcn_exp2f(ml[x][row][0] - base);
-      L += ml[x][row][1] * wt;
-      acc += *reinterpret_cast<const f32x4*>(ow + (x * kFewRows + row) * D + d) * wt;
-    }
-    const int tok = row / a.G, hq = hk * a.G + row % a.G;
-    if (__builtin_expect(odd_values, 0)) {   // the values that were taken out, where this row sees them
-      for (int j = k0 + max(pos0 - k0, 0) / kFewKeys * kFewKeys; j < k1 && j <= pos0 + tok; ++j) {
-        const int blk = block_of(a, j), page = tab[blk];
-        if ((unsigned)page >= (unsigned)a.num_blocks) continue;
-        const unsigned short* vr = a.v + (long)page * a.s_blk + (unsigned)((j - blk * a.block) * a.s_tok + hk * a.s_head) + d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if ((vr[e] & kExp) == kExp) acc[e] += F16 ? h2f(vr[e]) : bf2f(vr[e]);
-      }
-    }
-    const long trow = s.q0 + tok0 + tok;
-    if (whole) {
-      const float inv = L != 0.f ? 1.f / L : 0.f;
-      typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
-      u16x4 r;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) r[e] = cvt16<F16>(acc[e] * inv);
-      *reinterpret_cast<u16x4*>(a.out + trow * a.so_tok + (long)hq * a.so_head + d) = r;
-    } else {
-      const long pi = ((long)sp * a.T + trow) * a.Hq + hq;
-      *reinterpret_cast<f32x4*>(a.part_o + pi * D + d) = acc;
-      if (d == 0) {
-        a.part_ml[pi * 2] = M;
-        a.part_ml[pi * 2 + 1] = L;
-      }
-    }
-  }
-}
-
 // joins the pieces of every row that was split: grid (tokens, groups of heads), D / 4 lanes per query head
 template <int D, bool F16>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
@@ -897,20 +1017,21 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 
 using namespace pd;
 
-// upper bound of the batch's row tiles: every sequence may end in a part of one
-extern "C" int pd_chunk_attn_tiles(int T, int B, int G, int few) {
-  const int tt = (few ? ca::kFewRows : ca::kBM) / G, some = B < T ? B : T;
-  return (int)((T + (long)some * (tt - 1)) / tt);
+// An upper bound of the batch's tiles of 16 or 128 rows: every sequence may end in a part of one
+extern "C" long pd_chunk_attn_tiles(int T, int B, int G, int rows) {
+  const int tt = rows / G, some = B < T ? B : T;
+  return (T + (long)some * (tt - 1)) / tt;
 }
 
+// rows: of a tile, 16, or 128 and 16 for the sequences that have no more (one tile either way)
 extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, const void* k, const void* v, long s_blk,
                              long s_tok, long s_head, const int* table, int max_blocks, int num_blocks, int block,
                              const int* cu, const int* lens, void* out, long so_tok, long so_head, int B, int T, int Hq,
-                             int Hk, int D, int splits, int min_keys, float scale, int few, int groups, float* part_o,
-                             float* part_ml, int* pieces, void* stream) {
+                             int Hk, int D, int rows, int groups, int splits, int min_keys, float scale,
+                             float* part_o, float* part_ml, int* pieces, void* stream) {
   if (T <= 0 || B <= 0) return 0;
   if (Hk <= 0 || Hq % Hk || Hq / Hk > ca::kBM || block <= 0 || max_blocks <= 0 || num_blocks <= 0 || splits < 1 ||
-      (few && Hq / Hk > ca::kFewRows))
+      (rows != 16 && rows != 128) || Hq / Hk > rows || groups < 1 || groups > 2)
     return -1;
   if (splits > 1 && (!part_o || !part_ml || !pieces)) return -1;
   // a page's span in 32 bits (its number times s_blk is taken in 64)
@@ -934,28 +1055,27 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   while ((1L << L) < block) ++L;
   a.block_shift = block == 1 ? 0 : 31 + L;
   a.block_mul = block == 1 ? 1u : (unsigned)(((1UL << (31 + L)) + block - 1) / block);
-  a.grain = few ? 4 * ca::kFewKeys : ca::kBN;
-  a.splits = splits, a.min_keys = min_keys < a.grain ? a.grain : min_keys;
+  a.splits = splits, a.min_keys = min_keys < 1 ? 1 : min_keys;
   a.scale_log2 = scale * ca::kLog2e;
   a.part_o = part_o, a.part_ml = part_ml, a.pieces = pieces;
-  const long wgs = (long)pd_chunk_attn_tiles(T, B, a.G, few) * Hk * splits;
+  const long wgs = pd_chunk_attn_tiles(T, B, a.G, rows) * Hk * splits;
   if (wgs > 0x7fffffffL) return -1;
   hipStream_t st = (hipStream_t)stream;
   // (a wave's load covers 512 / D rows: see Stage)
   const bool uni = block % (512 / D) == 0 && s_tok >= D && span + 8 * s_tok < 1L << 30;
-#define PD_CHUNK3(DV, F, U)                                                                 \
+#define PD_MANY(DV, F, U)                                                                   \
   do {                                                                                      \
     if (groups == 2) ca::chunk_kernel<DV, F, U, 2><<<(unsigned)wgs, 512, 0, st>>>(a);       \
     else ca::chunk_kernel<DV, F, U, 1><<<(unsigned)wgs, 256, 0, st>>>(a);                   \
   } while (0)
 #define PD_CHUNK(DV)                                                                        \
   do {                                                                                      \
-    if (few && f16) ca::few_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);             \
-    else if (few) ca::few_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);              \
-    else if (f16 && uni) PD_CHUNK3(DV, true, true);                                            \
-    else if (f16) PD_CHUNK3(DV, true, false);                                               \
-    else if (uni) PD_CHUNK3(DV, false, true);                                               \
-    else PD_CHUNK3(DV, false, false);                                                       \
+    if (rows == 16 && f16) ca::few_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);      \
+    else if (rows == 16) ca::few_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);       \
+    else if (f16 && uni) PD_MANY(DV, true, true);                                           \
+    else if (f16) PD_MANY(DV, true, false);                                                 \
+    else if (uni) PD_MANY(DV, false, true);                                                 \
+    else PD_MANY(DV, false, false);                                                         \
     if (splits > 1) {                                                                       \
       const dim3 jg(T, (Hq * DV / 4 + 255) / 256);                                          \
       if (f16) ca::join_kernel<DV, true><<<jg, 256, 0, st>>>(a);                            \
@@ -966,6 +1086,6 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   else if (D == 128) PD_CHUNK(128);
   else return -2;
 #undef PD_CHUNK
-#undef PD_CHUNK3
+#undef PD_MANY
   return (int)hipGetLastError();
 }

@@ -101,7 +101,7 @@ def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=Non
     if not (scale > 0.0 and math.isfinite(scale)):
         raise ValueError(f"chunk_attention: scale {scale}")
     if out is None:
-        out = torch.empty(qs, dtype=dt, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != qs or out.dtype is not dt or out.device != dev:
         raise ValueError(f"chunk_attention: out {tuple(out.shape)} {out.dtype} on {out.device}")
     if T and B:
@@ -136,29 +136,34 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     pq, pk, pv, po = q.data_ptr(), kc.data_ptr(), vc.data_ptr(), out.data_ptr()
     if sk[3] != 1 or so[2] != 1 or ((sk[0] | sk[1] | sk[2] | so[0] | so[1]) * 2 | pk | pv | po) & 15:
         raise ValueError("chunk_attention: the caches and out need contiguous, 16-byte aligned rows")
-    m = N.native()
-    few = G <= 16 and T * G <= _FEW_ROWS * B
-    # Pieces of a tile's keys.  Two workgroups fit a CU: as many pieces as fit the chip at once.  Few rows over many
-    # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
-    # are left whole, their pieces' O costs more than it evens out.
-    per = (16 if few else 128) // G   # tokens of a tile
-    tiles = max(min(B, T), -(-T // per)) * Hk
-    # No more tiles than CUs, parts of tiles at the sequences' ends counted: two groups of waves per tile, whose halves of
-    # the keys are joined through LDS (700 tokens, 32 heads: 21 us, with one 30; 1,000 over 3,000, 32 heads on 8: 77 and 81;
-    # 128 over 16,000, 16 on 4: 36 and 40; the other way 2 x 2,000 over 10,000, 8 on 1: 194 and 181).  With 512 tiles it is
-    # 67 and 60, with mostly single tokens 56 and 45, with 64 rows per sequence no difference.
-    most = (T + min(B, T) * (per - 1)) // per * Hk
-    groups = 2 if not few and most <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
-    slots = _CHUNK_WGS // groups
-    splits = slots // tiles if tiles < slots or not few else 4 * slots // tiles
-    splits = max(1, min(splits, max_blocks * bs // _CHUNK_MIN_KEYS, 64))
+    rows, groups, splits = _chunk_plan(T, B, G, Hk, max_blocks * bs)
     # scratch of a split: the pieces' O, their (maximum, sum), and into how many a token's keys were split
     ws = torch.empty(splits * T * Hq * (D + 2) + T, dtype=torch.float32, device=q.device) if splits > 1 else None
     w0 = 0 if ws is None else ws.data_ptr()
     w1 = w0 + 4 * splits * T * Hq * D
-    _launch(q.device, m.chunk_attn, int(q.dtype is torch.float16), pq, sq[0], sq[1], pk, pv, sk[0], sk[tok], sk[head],
-            table.data_ptr(), max_blocks, ks[0], bs, cu.data_ptr(), lens.data_ptr(), po, so[0], so[1], B, T, Hq, Hk, D,
-            splits, _CHUNK_MIN_KEYS, scale, int(few), groups, w0, w1, w1 + 8 * splits * T * Hq)
+    _launch(q.device, N.native().chunk_attn, int(q.dtype is torch.float16), pq, sq[0], sq[1], pk, pv, sk[0], sk[tok],
+            sk[head], table.data_ptr(), max_blocks, ks[0], bs, cu.data_ptr(), lens.data_ptr(), po, so[0], so[1], B, T, Hq,
+            Hk, D, rows, groups, splits, _CHUNK_MIN_KEYS, scale, w0, w1, w1 + 8 * splits * T * Hq)
+
+
+def _chunk_plan(T, B, G, Hk, capacity):
+    """Rows of a tile (16, or 128 and 16 for the sequences that have no more), groups of waves that share one of 128, and
+    into how many pieces a tile's keys are split at most."""
+    # Pieces of a tile's keys.  Two workgroups fit a CU: as many pieces as fit the chip at once.  Few rows over many
+    # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
+    # are left whole, their pieces' O costs more than it evens out.
+    longest = min(capacity // _CHUNK_MIN_KEYS, 64)
+    if G <= 16 and T * G <= _FEW_ROWS * B:
+        tiles = max(min(B, T), -(-T // (16 // G))) * Hk
+        return 16, 1, max(1, min((_CHUNK_WGS if tiles < _CHUNK_WGS else 4 * _CHUNK_WGS) // tiles, longest))
+    per = 128 // G   # tokens of a tile
+    tiles = max(min(B, T), -(-T // per)) * Hk
+    # No more tiles than CUs, parts of tiles at the sequences' ends counted: two groups of waves per tile, whose halves of
+    # the keys are joined through LDS (700 tokens, 32 heads: 20 us, with one 28; 1,000 over 3,000, 32 heads on 8: 70 and 74;
+    # 128 over 16,000, 16 on 4: 35 and 39).  With 512 tiles it is 62 and 55, with 64 rows per sequence no difference.
+    most = (T + min(B, T) * (per - 1)) // per * Hk
+    groups = 2 if most <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
+    return 128, groups, max(1, min(_CHUNK_WGS // (groups * tiles), longest))
 
 
 def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):

@@ -341,17 +341,17 @@ def test_chunk_attention_refusals_cpu():
     _refused("cpu", torch.float32)
     m = N.native()
     with pytest.raises(ValueError):
-        m.chunk_attn_tiles(4, 1, 129, 0)
+        m.chunk_attn_tiles(4, 1, 129, 128)
     with pytest.raises(ValueError):
-        m.chunk_attn_tiles(4, 1, 17, 1)
+        m.chunk_attn_tiles(4, 1, 17, 16)
     # enough tiles for every split of T rows over B sequences
     for T in (1, 5, 2048):
         for B in (1, 3, 64):
-            for rows, few, Gs in ((128, 0, (1, 3, 128)), (16, 1, (1, 3, 16))):
+            for rows, Gs in ((128, (1, 3, 128)), (16, (1, 3, 16))):
                 for G in Gs:
                     per, some = rows // G, min(B, T)
                     most = some + (T - some) // per        # `some` sequences of one row, the rest in full tiles
-                    assert most <= m.chunk_attn_tiles(T, B, G, few) <= most + some
+                    assert most <= m.chunk_attn_tiles(T, B, G, rows) <= most + some
 
 
 @pytest.mark.gpu
