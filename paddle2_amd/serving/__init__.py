@@ -152,7 +152,8 @@ class PagedKVCache:
     """Per-layer K/V block pools [num_blocks, block_size, Hk, D] with a free list and block tables.
 
     Pages may be shared: ``fork`` gives another sequence the full pages of one, and a page goes back to the free list
-    when its last holder lets go.  Full pages are only read; the page a sequence still writes is always its own."""
+    when its last holder lets go.  Full pages are only read; the page a sequence still writes is always its own, and to
+    write earlier tokens again it has to be truncated (check_writable)."""
 
     def __init__(self, num_layers, num_blocks, block_size, num_kv_heads, head_dim, max_batch, max_seq_len,
                  dtype=torch.bfloat16, device=None):
@@ -203,9 +204,16 @@ class PagedKVCache:
         return len(self._free)
 
     # ------------------------------------------------------------------ shared pages
+    def check_writable(self, slot, start=0):
+        """ValueError if sequence ``slot`` shares a page that holds tokens from ``start`` on: writing them would change the
+        sequences it shares with.  truncate(slot, start) makes room, free(slot) lets go of all."""
+        if any(self._holders[b] > 1 for b in self._owned.get(slot, [])[start // self.block_size:]):
+            raise ValueError(f"PagedKVCache: slot {slot} shares pages behind token {start}: truncate or free it first")
+
     def copy_blocks(self, src, dst):
         """Page src[i] -> page dst[i] in the K and V pools of every layer, one launch (KVBlockCopier.copy)."""
-        if self._copier is None or any(a is not b for a, b in zip(self._copier.pools, self.k + self.v)):
+        pools = self._copier.pools if self._copier is not None else []
+        if len(pools) != len(self.k) + len(self.v) or any(a is not b for a, b in zip(pools, self.k + self.v)):
             self._copier = KVBlockCopier(self.k, self.v)
         self._copier.copy(src, dst)
 

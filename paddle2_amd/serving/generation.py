@@ -212,6 +212,7 @@ class LlamaGenerator:
     def prefill(self, slot, ids):
         """Run prompt ``ids`` (1-D LongTensor) for sequence ``slot``; returns last-token logits [V]."""
         n = ids.numel()
+        self.cache.check_writable(slot)
         self.cache.allocate(slot, n + 1)
         nh, nkv, d = self.nh, self.nkv, self.d
         x = self.model.llama.embed_tokens.weight._t[ids.to(self.dev)][None]  # [1, n, h]
@@ -239,6 +240,8 @@ class LlamaGenerator:
         lens = [len(p) for p in prompts]
         total = sum(lens)
         nh, nkv, d = self.nh, self.nkv, self.d
+        for s in slots:
+            self.cache.check_writable(s)
         for s, n in zip(slots, lens):
             self.cache.allocate(s, n + 1)
         ids = torch.as_tensor([int(t) for p in prompts for t in p], dtype=torch.long).to(self.dev)
@@ -279,6 +282,8 @@ class LlamaGenerator:
         held = self.cache.seq_lens[slot_t].tolist() if held is None else [int(h) for h in held]
         if len(held) != len(lens) or min(held, default=0) < 0:
             raise ValueError(f"extend: held {held} for {len(lens)} slots")
+        for s, h in zip(slots, held):
+            self.cache.check_writable(s, h)
         for s, n, h in zip(slots, lens, held):
             self.cache.allocate(s, h + n + 1)
         ids = torch.as_tensor([int(t) for c in chunks for t in c], dtype=torch.long).to(self.dev)
@@ -388,6 +393,8 @@ class LlamaGenerator:
         if sampler not in ("fused", "multinomial") or (sampler == "multinomial" and fused_only):
             raise ValueError(f"generate: sampler {sampler!r} with temperature={temperature}, top_k={top_k}, top_p={top_p}, "
                              f"min_p={min_p}")
+        for s in range(self.max_batch):   # (idle slots are written too)
+            self.cache.check_writable(s)
         gen = torch.Generator(device=self.dev).manual_seed(seed) if self.dev.type == "cuda" else \
             torch.Generator().manual_seed(seed)
         B = self.max_batch

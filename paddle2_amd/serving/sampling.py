@@ -1,7 +1,6 @@
 """The next token of every row of logits, from given random numbers (csrc/kernels/sampling.hip)."""
 from __future__ import annotations
 
-import math
 import numbers
 
 import torch
@@ -60,7 +59,7 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     if u.shape != (B,) or u.dtype is not torch.float32 or u.device != dev:
         raise ValueError(f"sample_tokens: uniform {tuple(u.shape)} {u.dtype} on {u.device}, expected ({B},) float32 on {dev}")
     t = _setting(temperature, "temperature", B, dev, torch.float32, 0.0, 1e30)
-    k = _setting(top_k, "top_k", B, dev, torch.int32, -1, math.inf)
+    k = _setting(top_k, "top_k", B, dev, torch.int32, -1, 2 ** 63 - 1)
     p = _setting(top_p, "top_p", B, dev, torch.float32, 0.0, 1.0)
     m = _setting(min_p, "min_p", B, dev, torch.float32, 0.0, 1.0)
     if out is None:

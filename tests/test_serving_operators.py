@@ -363,6 +363,8 @@ def test_chunk_attention_refusals_gpu():
                                               vc[..., :32].contiguous(), cu, lens, table),
               lambda: serving.chunk_attention(q, kc, vc, cu.cpu(), lens, table),
               lambda: serving.chunk_attention(q, kc, vc.cpu(), cu, lens, table),
+              lambda: serving.chunk_attention(q, kc[:1].repeat(1, 4096, 1, 1), vc[:1].repeat(1, 4096, 1, 1), cu, lens,
+                                              torch.zeros(1, 2 ** 15, dtype=torch.int32, device="cuda")),
               lambda: serving.chunk_attention(q, kc, vc.transpose(1, 2).contiguous().transpose(1, 2), cu, lens, table)):
         with pytest.raises(ValueError):
             f()
@@ -631,7 +633,7 @@ def test_sample_tokens_refusals():
     x, u = torch.zeros(3, 5), torch.zeros(3)
     f = serving.sample_tokens
     for kw in (dict(temperature=-1.0), dict(temperature=float("nan")), dict(temperature=float("inf")), dict(top_p=1.5),
-               dict(top_p=-0.1), dict(min_p=2.0), dict(min_p=-1.0), dict(top_k=2.5), dict(top_k=-7), dict(top_k="3"),
+               dict(top_p=-0.1), dict(min_p=2.0), dict(min_p=-1.0), dict(top_k=2.5), dict(top_k=-7), dict(top_k="3"), dict(top_k=float("inf")),
                dict(temperature=torch.zeros(2)), dict(top_k=torch.zeros(3, 1, dtype=torch.int32)),
                dict(out=torch.zeros(3)), dict(out=torch.zeros(4, dtype=torch.int64))):
         with pytest.raises(ValueError):
@@ -786,6 +788,34 @@ def test_generate_with_shared_prompts_and_fused_sampling(dev):
     for bad in (dict(sampler="multinomial", min_p=0.1), dict(sampler="beam"), dict(temperature=[1.0])):
         with pytest.raises(ValueError):
             gen.generate(prompts, 3, **bad)
+
+
+def test_shared_pages_are_not_written():
+    """A prompt, a chunk or a whole generation over a slot that shares the pages it would write is refused, with nothing
+    changed; pools that were added to a cache are copied too."""
+    from paddle2_amd.serving import LlamaGenerator
+
+    gen = LlamaGenerator(_llama("cpu"), max_batch=3, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill_chunks([0], [list(range(1, 22))], 8)
+    gen.cache.fork(0, [1])
+    pools = [t.clone() for t in gen.cache.k + gen.cache.v]
+    for f in (lambda: gen.extend([1], [[5]], held=[15]), lambda: gen.prefill(1, torch.tensor([3, 4])),
+              lambda: gen.prefill_batch([2, 0], [[1], [2]]), lambda: gen.generate([[1, 2]], 2)):
+        with pytest.raises(ValueError, match="shares pages"):
+            f()
+    assert all(torch.equal(a, b) for a, b in zip(pools, gen.cache.k + gen.cache.v))
+    gen.cache.truncate(1, 15)
+    gen.extend([1], [[5]], held=[15])
+    gen.extend([0], [[5]], held=[16])    # behind the shared pages
+    gen.cache.free(1), gen.cache.free(0)
+    assert len(gen.generate([[1, 2]], 2)[0]) == 2
+
+    c = _cache("cpu")
+    c.copy_blocks([0], [1])
+    c.k.append(torch.arange(12.0).repeat_interleave(c.k[0][0].numel()).view_as(c.k[0]).to(c.k[0].dtype))
+    c.v.append(c.k[-1].clone())
+    c.copy_blocks([3], [5])
+    assert (c.k[-1][5] == 3).all() and (c.v[-1][5] == 3).all()
 
 
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
