@@ -231,8 +231,8 @@ __device__ __forceinline__ int block_of(const Args& a, int key) {
 //  * the waves' (m, l, O) are joined through LDS at the end.
 // A step that mixes single tokens with pieces of prompts has both kinds of tiles in one launch: 45 sequences over 1,250 -
 // 2,500 keys, 33 of them single tokens, take 44 us, with 128-row tiles for all of them 48 (D = 64, 16 heads on 4).  Where
-// few rows are all there is, a kernel of their own with a quarter of the LDS and smaller pieces: 64 single tokens over 4,000
-// - 8,000 keys take 311 us in it, 338 in the other; 8 x 4 drafted tokens over 350 - 700 take 22 in both.
+// few rows are all there is, a kernel of their own with less LDS and smaller pieces: 64 single tokens over 4,000 - 8,000
+// keys take 311 us in it, 338 in the other; 8 x 4 drafted tokens over 350 - 700, 32 heads, 19 us (13.5 at a copy's rate).
 
 template <bool F16>
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
@@ -450,13 +450,13 @@ __device__ __forceinline__ void few_rows(const Args& a, const Seq& s, int hk, in
   }
 }
 
-template <int D, bool F16>
-__global__ __launch_bounds__(256, 2) void few_kernel(Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * kFewKeys * D * 2];
+template <int D, bool F16, int W>
+__global__ __launch_bounds__(64 * W, W == 8 ? 1 : 2) void few_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[W * kFewKeys * D * 2];
   int hk, sp;
   bool few;
   const Seq s = find_part<true>(a, threadIdx.x & 63, hk, sp, few);
-  if (s.tile >= 0) few_rows<D, F16, 4>(a, s, hk, sp, lds);
+  if (s.tile >= 0) few_rows<D, F16, W>(a, s, hk, sp, lds);
 }
 
 // A K or V tile on its way from the pages to LDS: a thread brings chunk tid % NCH of rows tid / NCH + ROWS * i.
@@ -1068,10 +1068,15 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
     if (groups == 2) ca::chunk_kernel<DV, F, U, 2><<<(unsigned)wgs, 512, 0, st>>>(a);       \
     else ca::chunk_kernel<DV, F, U, 1><<<(unsigned)wgs, 256, 0, st>>>(a);                   \
   } while (0)
+#define PD_FEW(DV, F)                                                                       \
+  do {                                                                                      \
+    if (groups == 2) ca::few_kernel<DV, F, 8><<<(unsigned)wgs, 512, 0, st>>>(a);            \
+    else ca::few_kernel<DV, F, 4><<<(unsigned)wgs, 256, 0, st>>>(a);                        \
+  } while (0)
 #define PD_CHUNK(DV)                                                                        \
   do {                                                                                      \
-    if (rows == 16 && f16) ca::few_kernel<DV, true><<<(unsigned)wgs, 256, 0, st>>>(a);      \
-    else if (rows == 16) ca::few_kernel<DV, false><<<(unsigned)wgs, 256, 0, st>>>(a);       \
+    if (rows == 16 && f16) PD_FEW(DV, true);                                                \
+    else if (rows == 16) PD_FEW(DV, false);                                                 \
     else if (f16 && uni) PD_MANY(DV, true, true);                                           \
     else if (f16) PD_MANY(DV, true, false);                                                 \
     else if (uni) PD_MANY(DV, false, true);                                                 \
@@ -1086,6 +1091,7 @@ extern "C" int pd_chunk_attn(int f16, const void* q, long sq_tok, long sq_head, 
   else if (D == 128) PD_CHUNK(128);
   else return -2;
 #undef PD_CHUNK
+#undef PD_FEW
 #undef PD_MANY
   return (int)hipGetLastError();
 }

@@ -16,8 +16,8 @@ _HEAD_DIMS = (64, 128)
 _CHUNK_WGS = 512        # workgroups that fit the chip at once
 _CHUNK_MIN_KEYS = 256   # keys of a piece at least (128: the join costs more than the shorter pieces give)
 _FEW_ROWS = 16          # rows (query heads of a kv head times new tokens) per sequence up to which they are few, on average
-_PAIR_TILES = 256       # tiles (of 128 rows) up to which two groups of waves share one,
-_PAIR_ROWS = 64         # if the sequences have that many rows, on average
+_PAIR_TILES = 256       # tiles up to which two groups of waves share one (the CUs),
+_PAIR_ROWS = 64         # if of 128 rows: where the sequences have that many, on average
 _MAX_KEYS = 2**31 - 2**14   # positions are 32-bit, and a tile's loads reach past its last key
 
 
@@ -147,14 +147,20 @@ def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
 
 
 def _chunk_plan(T, B, G, Hk, capacity):
-    """Rows of a tile (16, or 128 and 16 for the sequences that have no more), groups of waves that share one of 128, and
-    into how many pieces a tile's keys are split at most."""
-    # Pieces of a tile's keys.  Two workgroups fit a CU: as many pieces as fit the chip at once.  Few rows over many
-    # sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us); many rows
-    # are left whole, their pieces' O costs more than it evens out.
+    """Rows of a tile (16, or 128 and 16 for the sequences that have no more), groups of four waves that share one, and into
+    how many pieces a tile's keys are split at most."""
+    # Pieces of a tile's keys.  Two workgroups of four waves fit a CU: as many pieces as fit the chip at once.  Few rows
+    # over many sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us);
+    # many rows are left whole, their pieces' O costs more than it evens out.
     longest = min(capacity // _CHUNK_MIN_KEYS, 64)
     if G <= 16 and T * G <= _FEW_ROWS * B:
         tiles = max(min(B, T), -(-T // (16 // G))) * Hk
+        # No more tiles than CUs, but work for all: one workgroup of eight waves a CU, half as many pieces to join (8 x 4
+        # tokens over 350 - 700, 32 heads: 18.9 us, with four waves 21.6; 1 over 16,000, 32 heads on 8: 24.8 and 31.6; the
+        # other way 16 over 600 - 1,200, 32 on 8: 22.6 and 21.5).  With less work four waves: 1 over 1,400, 16 heads on 4,
+        # takes 14.4 us, with eight 16.0.
+        if tiles <= _PAIR_TILES < tiles * longest:
+            return 16, 2, max(1, min(_CHUNK_WGS // 2 // tiles, longest))
         return 16, 1, max(1, min((_CHUNK_WGS if tiles < _CHUNK_WGS else 4 * _CHUNK_WGS) // tiles, longest))
     per = 128 // G   # tokens of a tile
     tiles = max(min(B, T), -(-T // per)) * Hk

@@ -118,14 +118,17 @@ def test_chunk_attention_long_gpu(new, held, Hq, Hk, D):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows,pairs", [(0, 0), (0, 10 ** 6), (10 ** 6, 0)])
+@pytest.mark.parametrize("rows,pairs", [(0, 0), (0, 10 ** 6), (10 ** 6, 0), (10 ** 6, 1000)])
 @pytest.mark.parametrize("splits", [1, 10 ** 6])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_chunk_attention_every_kernel_gpu(rows, pairs, splits, dtype, monkeypatch):
-    """The kernels for few rows and for many (one group of waves or two per tile), with the keys in one piece and in as many
+    """The kernels for few rows and for many, one group of waves or two per tile, with the keys in one piece and in as many
     as possible, on the same batches."""
     from paddle2_amd.serving import paged
 
+    plan = paged._chunk_plan
+    if pairs == 1000:       # two groups whatever the work
+        monkeypatch.setattr(paged, "_chunk_plan", lambda *a: (16, 2, 1 if splits == 1 else plan(*a)[2]))
     monkeypatch.setattr(paged, "_FEW_ROWS", rows)
     monkeypatch.setattr(paged, "_PAIR_TILES", pairs)
     monkeypatch.setattr(paged, "_PAIR_ROWS", 0)
