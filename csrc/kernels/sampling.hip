@@ -18,6 +18,12 @@
 //                  below, so some k groups are read, and the few logits above the bound are ranked all against all.
 // Rows that fit none of this (a larger k, an infinite logit, a border in the tail or with more than 8,192 logits in its
 // bin, a number below 2^-40) are taken from the start in choose_kernel: radix selection on the ordered bits of the logits.
+//
+// Measured: 256 rows of 131,072 bf16 logits with settings of their own 102 us (peaks 15, 4.6 TB/s; bins 38 and sweep 39, bound
+// by some 25 double-precision operations a logit, bins by an LDS atomic each too; choose 26, bound by latency); 32 of
+// 50,257 fp32 with top-k and top-p 13 (two launches); 64 of 32,000 fp16 with min-p 15 (three); one of 32,000 with top-p 25
+// (four, 3 - 9 each).  choose_kernel with its arguments in registers alone, one inlined call of the rare path, is 4 - 9 us
+// shorter than with that path as a function.
 #include "common.h"
 
 namespace pd {
@@ -497,7 +503,7 @@ struct Shared {   // of choose_kernel
 
 // ---- a row from the start, by radix selection
 template <int kWaves, typename T>
-__device__ void choose_from_start(const Args<T>& a, const Of& of, int b, Shared& sh) {
+__device__ __forceinline__ void choose_from_start(const Args<T>& a, const Of& of, int b, Shared& sh) {
   const int V = a.V;
   u64 *const red = sh.red, *const hist = sh.hist, *const part = sh.part, *const found = sh.found;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -791,48 +797,31 @@ __device__ __forceinline__ u64 resolve(Shared& sh, int n, u64 left, const Weighe
   return sh.found[3];
 }
 
-// grid B, one row each
-template <typename T, int kWaves>
-__global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
+// v[0 .. kShort) becomes its inclusive prefix sums (the caller's barrier before it, its own after it)
+template <int WAVES>
+__device__ __forceinline__ void group_scan(u64* v, u64* red) {
+  constexpr int PER = kShort / (WAVES * 64);
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  u64 x[PER], sum = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) sum += x[j] = v[threadIdx.x * PER + j];
+  u64 run = wave_scan64(sum);
+  if (lane == 63) red[wv] = run;
+  __syncthreads();
+  run -= sum;
+  for (int i = 0; i < wv; ++i) run += red[i];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) v[threadIdx.x * PER + j] = run += x[j];
+  __syncthreads();
+}
+
+// a row whose sums or peaks the other kernels have prepared; false: it has to be taken from the start
+template <int kWaves, typename T>
+__device__ __forceinline__ bool choose_by_mass(const Args<T>& a, const Of& of, int b, Shared& sh, float top, Kind kind) {
   constexpr int kThreads = kWaves * 64;
-  __shared__ Shared sh;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, V = a.V, chunks = a.chunks;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, V = a.V, chunks = a.chunks;
   const T* row = a.logits + (long)b * a.stride;
   const float* peaks = a.peaks + (long)b * a.groups;
-  const Of of = row_of(a, b);
-  if (tid == 0) sh.listed = 0;
-  const float top = row_peak<kWaves>(peaks, a.groups, reinterpret_cast<float*>(sh.red));
-  const Kind kind = kind_of(a, of, top);
-  if (kind == kGreedy) {   // the lowest index of the largest logit; 0 where no token is allowed
-    int g = a.groups;
-    for (int i = tid; i < a.groups; i += kThreads)
-      if (peaks[i] == top) {
-        g = i;
-        break;
-      }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) g = min(g, __shfl_xor(g, o, 64));
-    if (lane == 0) sh.part[wv] = g;
-    __syncthreads();
-    if (wv == 0) {
-      g = lane < kWaves ? (int)sh.part[lane] : a.groups;
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) g = min(g, __shfl_xor(g, o, 64));
-      float x[8];
-      const int i = g * a.group_lanes * 8 + (lane & (a.group_lanes - 1)) * 8;
-      load8(row, i, V, x);
-      int first = 8;
-#pragma unroll
-      for (int j = 7; j >= 0; --j) first = x[j] == top ? j : first;
-      const u64 hit = __ballot(first < 8 && lane < a.group_lanes);
-      if (lane == (hit ? __ffsll((long long)hit) - 1 : 0)) a.out[b] = hit && top > -INFINITY ? i + first : 0;
-    }
-    return;
-  }
-  if (kind == kFromStart) {
-    choose_from_start<kWaves>(a, of, b, sh);
-    return;
-  }
   const Weigher weigh = weigher(top, of.t, a.shift);
   const u64 least = least_weight(of.m, a.shift);
   auto target = [&](u64 total) {
@@ -876,62 +865,57 @@ __global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
     const int n = sh.listed;
     if (!ok || n > kShort) {
       __syncthreads();
-      choose_from_start<kWaves>(a, of, b, sh);
-      return;
+      return false;
     }
-    // All against all, `parts` threads to an entry where there are fewer entries than threads: rank and mass before it,
-    // then the kept mass at smaller indexes
-    constexpr u64 kFlip = 0xffffffffull;
-    u64 *const before = sh.part, *const weight = sh.weight;
-    int* const rank = reinterpret_cast<int*>(sh.hist);
+    // Ranks by counting, all against all, `parts` threads to an entry where there are fewer entries than threads; masses by
+    // prefix sums of the weights in that order: by logit for what top-k and top-p keep, then by index for the token
+    constexpr u64 kFlip = 0xffffffffull;   // (the lower index first, as the larger logit)
+    u64 *const upto = sh.part, *const weight = sh.weight;
+    int *const rank = reinterpret_cast<int*>(sh.hist), *const place = rank + kShort;
     int step = 64;
     while (step < n && step < kThreads) step *= 2;
     const int part = tid / step, parts = kThreads / step, first = tid & (step - 1);
+    const int per = (n + parts - 1) / parts, i0 = part * per, i1 = min(n, i0 + per);
     __syncthreads();
     for (int at = tid; at < kShort; at += kThreads) {
       if (at < n) {
         sh.list[at] ^= kFlip;
         weight[at] = weigh(value_of((unsigned)(sh.list[at] >> 32)));
       }
-      before[at] = 0, rank[at] = 0;
+      upto[at] = 0, rank[at] = 0, place[at] = 0;
     }
     __syncthreads();
     for (int at = first; at < n; at += step) {
       const u64 mine = sh.list[at];
-      u64 sum = 0;
-      int ahead = 0;
-#pragma unroll 4
-      for (int i = part; i < n; i += parts) {
-        const bool is = sh.list[i] > mine;
-        ahead += is;
-        sum += is ? weight[i] : 0;
+      int ahead = 0, left = 0;
+#pragma unroll 8
+      for (int i = i0; i < i1; ++i) {
+        const u64 other = sh.list[i];
+        ahead += other > mine;
+        left += (unsigned)other > (unsigned)mine;
       }
-      if (parts == 1) before[at] = sum, rank[at] = ahead;
-      else if (ahead) atomicAdd(&before[at], sum), atomicAdd(&rank[at], ahead);
+      if (parts == 1) rank[at] = ahead, place[at] = left;
+      else atomicAdd(&rank[at], ahead), atomicAdd(&place[at], left);
     }
     __syncthreads();
-    u64 in_k = 0, in_all = 0;
-    for (int at = tid; at < n; at += kThreads) in_k += rank[at] < of.k ? weight[at] : 0;
-    const u64 share = of.p < 1.f ? share_of(of.p, group_sum<kWaves>(in_k, sh.red)) : ~0ull;
+    for (int at = tid; at < n; at += kThreads) upto[rank[at]] = weight[at];
+    __syncthreads();
+    group_scan<kWaves>(upto, sh.red);
+    const u64 share = of.p < 1.f ? share_of(of.p, upto[min(of.k, n) - 1]) : ~0ull;
     for (int at = tid; at < n; at += kThreads) {
-      const bool kept = rank[at] < of.k && before[at] < share && weight[at] >= least;
+      const bool kept = rank[at] < of.k && upto[rank[at]] - weight[at] < share && weight[at] >= least;
       if (!kept) weight[at] = 0;
-      in_all += weight[at];
-      before[at] = 0;
-    }
-    const u64 want = target(group_sum<kWaves>(in_all, sh.red));   // (its barriers publish the kept weights)
-    for (int at = first; at < n; at += step) {
-      const unsigned mine = (unsigned)sh.list[at];   // the index, flipped
-      u64 sum = 0;
-#pragma unroll 4
-      for (int i = part; i < n; i += parts) sum += (unsigned)sh.list[i] > mine ? weight[i] : 0;
-      if (parts == 1) before[at] = sum;
-      else if (sum) atomicAdd(&before[at], sum);
     }
     __syncthreads();
-    for (int at = tid; at < n; at += kThreads)
-      if (weight[at] && before[at] <= want && want < before[at] + weight[at]) a.out[b] = (int64_t)(unsigned)~(unsigned)sh.list[at];
-    return;
+    for (int at = tid; at < n; at += kThreads) upto[place[at]] = weight[at];
+    __syncthreads();
+    group_scan<kWaves>(upto, sh.red);
+    const u64 want = target(upto[n - 1]);
+    for (int at = tid; at < n; at += kThreads) {
+      const u64 end = upto[place[at]];
+      if (weight[at] && end - weight[at] <= want && want < end) a.out[b] = (int64_t)(unsigned)~(unsigned)sh.list[at];
+    }
+    return true;
   }
   // a logit is kept when its key is above kmin, or equals it at an index up to last, and its weight is `least` or more
   unsigned kmin = 0;
@@ -942,8 +926,7 @@ __global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
     u64 left = 0;
     const int n = a.listed[b];
     if (!border_bin<kWaves>(a.hist + (long)b * kBins, of.p, sh.red, sh.found, bin, left) || n > kList) {
-      choose_from_start<kWaves>(a, of, b, sh);
-      return;
+      return false;
     }
     for (int i = tid; i < n; i += kThreads) sh.list[i] = a.list[(long)b * kList + i];
     __syncthreads();
@@ -985,6 +968,49 @@ __global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
       a.out[b] = token;
     }
   }
+  return true;
+}
+
+// grid B, one row each
+template <typename T, int kWaves>
+__global__ __launch_bounds__(kWaves * 64) void choose_kernel(Args<T> a) {
+  constexpr int kThreads = kWaves * 64;
+  __shared__ Shared sh;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, V = a.V;
+  const T* row = a.logits + (long)b * a.stride;
+  const float* peaks = a.peaks + (long)b * a.groups;
+  const Of of = row_of(a, b);
+  if (tid == 0) sh.listed = 0;
+  const float top = row_peak<kWaves>(peaks, a.groups, reinterpret_cast<float*>(sh.red));
+  const Kind kind = kind_of(a, of, top);
+  if (kind == kGreedy) {   // the lowest index of the largest logit; 0 where no token is allowed
+    int g = a.groups;
+    for (int i = tid; i < a.groups; i += kThreads)
+      if (peaks[i] == top) {
+        g = i;
+        break;
+      }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) g = min(g, __shfl_xor(g, o, 64));
+    if (lane == 0) sh.part[wv] = g;
+    __syncthreads();
+    if (wv == 0) {
+      g = lane < kWaves ? (int)sh.part[lane] : a.groups;
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) g = min(g, __shfl_xor(g, o, 64));
+      float x[8];
+      const int i = g * a.group_lanes * 8 + (lane & (a.group_lanes - 1)) * 8;
+      load8(row, i, V, x);
+      int first = 8;
+#pragma unroll
+      for (int j = 7; j >= 0; --j) first = x[j] == top ? j : first;
+      const u64 hit = __ballot(first < 8 && lane < a.group_lanes);
+      if (lane == (hit ? __ffsll((long long)hit) - 1 : 0)) a.out[b] = hit && top > -INFINITY ? i + first : 0;
+    }
+    return;
+  }
+  // (one call of choose_from_start, which is inlined then: as a function it had the arguments in scratch memory)
+  if (kind == kFromStart || !choose_by_mass<kWaves>(a, of, b, sh, top, kind)) choose_from_start<kWaves>(a, of, b, sh);
 }
 
 }  // namespace smp
