@@ -21,7 +21,7 @@
 //  * Few tiles over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
 //    second kernel.  How often is decided per tile, from its own length.
 //
-// Measured (bf16, D = 128, 32 heads on 8, pages of 64): 2,048 tokens over 30,720 take 1,000 - 1,060 us, 1.0 PFLOP/s, bound by
+// Measured (bf16, D = 128, 32 heads on 8, pages of 64): 2,048 tokens over 30,720 take 975 - 1,030 us by the card, 1.03 - 1.09 PFLOP/s, bound by
 // the exponentials and maxima beside the products (two waves per SIMD: the matrix unit is busy half the time); 64 single
 // tokens over 4,000 - 8,000 take 310 us, 5.1 TB/s, the rate of a large copy.
 #include "common.h"
@@ -803,6 +803,9 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
 #pragma unroll
       for (int i = 0; i < AHEAD; ++i) f[i] = k_frag(i);
       nxt[0] = f32x16{}, nxt[1] = f32x16{};
+      // a wave in its exponentials goes first, the SIMD's other one has products between them (2,048 tokens over 30,720:
+      // 975 us, without 1,029)
+      __builtin_amdgcn_s_setprio(1);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -814,6 +817,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    if constexpr (!EDGE) __builtin_amdgcn_s_setprio(0);
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
     stage_middle(n0, EDGE);
     if constexpr (EDGE) {
