@@ -162,13 +162,12 @@ def _chunk_plan(T, B, G, Hk, capacity):
         if tiles <= _PAIR_TILES < tiles * longest:
             return 16, 2, max(1, min(_CHUNK_WGS // 2 // tiles, longest))
         return 16, 1, max(1, min((_CHUNK_WGS if tiles < _CHUNK_WGS else 4 * _CHUNK_WGS) // tiles, longest))
-    per = 128 // G   # tokens of a tile
-    tiles = max(min(B, T), -(-T // per)) * Hk
+    tiles = max(min(B, T), -(-T // (128 // G))) * Hk
     # No more tiles than CUs, parts of tiles at the sequences' ends counted: two groups of waves per tile, whose halves of
     # the keys are joined through LDS (700 tokens, 32 heads: 20 us, with one 29; 1,000 over 3,000, 32 heads on 8: 74 and 78;
     # 128 over 16,000, 16 on 4: 36 and 40; the other way 2 x 2,000 over 10,000, 8 on 1: 183 and 176).  With 512 tiles it is
     # 65 and 57, with 64 rows per sequence no difference.
-    most = (T + min(B, T) * (per - 1)) // per * Hk
+    most = N.native().chunk_attn_tiles(T, B, G, 128) * Hk
     groups = 2 if most <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
     return 128, groups, max(1, min(_CHUNK_WGS // (groups * tiles), longest))
 

@@ -156,6 +156,11 @@ def test_chunk_attention_many_sequences_gpu():
     new = [(i * 7) % 5 for i in range(150)]
     held = [(i * 13) % 90 for i in range(150)]
     _check_attn("cuda", torch.bfloat16, new, held, 4, 2, 64, 16)
+    for i in range(3, 150, 11):      # pieces of prompts among them: both kinds of tiles in one launch
+        new[i] = 40 + i % 60
+    for D in (64, 128):
+        _check_attn("cuda", torch.float16, new, held, 4, 2, D, 16, seed=D)
+    _check_attn("cuda", torch.bfloat16, new, held, 34, 1, 64, 16)      # more heads than a tile of few rows has rows
 
 
 @pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
