@@ -637,6 +637,23 @@ def test_sample_tokens_views_streams_and_graphs_gpu():
     assert torch.equal(other, eager)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("V,shift", [(1000, 0.0), (33000, 500.0), (70001, -3e4)])
+def test_sample_tokens_min_p_at_every_temperature_gpu(V, shift):
+    """min-p alone, temperatures and floors from the smallest to the largest, logits far from zero: as in 64 bits on the CPU."""
+    t, m = torch.meshgrid(torch.tensor([1e-30, 1e-3, 0.7, 50.0, 1e30, float("inf")]),
+                          torch.tensor([1e-38, 1e-6, 0.05, 0.5, 1.0, 2.0, float("nan")]), indexing="ij")
+    t, m = t.flatten(), m.flatten()
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(len(t), V, generator=g) * 4 + shift
+    x[:, 7] = x.amax(1)
+    x[::5, ::3] = float("-inf")
+    u = torch.rand(len(t), generator=g)
+    want = serving.sample_tokens(x, u, temperature=t, min_p=m)
+    got = serving.sample_tokens(x.cuda(), u.cuda(), temperature=t.cuda(), min_p=m.cuda())
+    assert torch.equal(got.cpu(), want)
+
+
 def test_sample_tokens_refusals():
     x, u = torch.zeros(3, 5), torch.zeros(3)
     f = serving.sample_tokens
