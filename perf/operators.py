@@ -5,8 +5,8 @@ the choice of the next token.
 
 * ``chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table)`` - the packed new tokens of a ragged
   batch attend to everything their sequence holds in the cache up to and including themselves;
-* ``KVBlockCopier(k_caches, v_caches).copy(src, dst)`` - page ``src[i]`` of every layer's K and V pool is copied to page
-  ``dst[i]`` (forked sequences, reordered beams, compaction); a server makes the copier once, with its pools;
+* ``copy_kv_blocks(k_caches, v_caches, src, dst)`` - page ``src[i]`` of every layer's K and V pool is copied to page
+  ``dst[i]`` (forked sequences, reordered beams, compaction);
 * ``sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)`` - one token per row from a given random number.
 """
 import math
@@ -179,13 +179,8 @@ def prepare(case, seed):
         return dict(op="sample", logits=x.to(dt), uniform=u, temperature=t, top_k=k, top_p=p, min_p=m)
     src, dst = _pairs(case)
     shape = (case["pool"], case["block"], case["kv_heads"], case["dim"])
-    s = dict(op="pages", k=[normal(*shape) for _ in range(case["layers"])],
-             v=[normal(*shape) for _ in range(case["layers"])], src=src, dst=dst)
-    if own:
-        from paddle2_amd import serving
-
-        s["copier"] = serving.KVBlockCopier(s["k"], s["v"])
-    return s
+    return dict(op="pages", k=[normal(*shape) for _ in range(case["layers"])],
+                v=[normal(*shape) for _ in range(case["layers"])], src=src, dst=dst)
 
 
 def _attention(s):
@@ -254,7 +249,7 @@ def run(state):
     if state["op"] == "sample":
         return serving.sample_tokens(state["logits"], state["uniform"], state["temperature"], state["top_k"],
                                      state["top_p"], state["min_p"])
-    state["copier"].copy(state["src"], state["dst"])
+    serving.copy_kv_blocks(state["k"], state["v"], state["src"], state["dst"])
     return state["k"] + state["v"]
 
 
