@@ -312,13 +312,14 @@ class LlamaGenerator:
     @torch.no_grad()
     def prefill_chunks(self, slots, prompts, chunk_size):
         """Prompts in pieces of at most ``chunk_size`` tokens, all sequences' pieces of a round in one ``extend``: the
-        activations of a long prompt are chunk_size rows instead of the whole length.  Last-token logits [n, V]."""
+        activations of a long prompt are chunk_size rows instead of the whole length.  A prompt starts at position 0 and
+        replaces what its slot held, as in ``prefill``.  Last-token logits [n, V]."""
         if chunk_size < 1 or min((len(p) for p in prompts), default=1) < 1:
             raise ValueError(f"prefill_chunks: chunk_size {chunk_size}, prompts of {[len(p) for p in prompts]} tokens")
         out = [None] * len(slots)
         for at in range(0, max((len(p) for p in prompts), default=0), chunk_size):
             some = [i for i, p in enumerate(prompts) if len(p) > at]
-            logits = self.extend([slots[i] for i in some], [prompts[i][at:at + chunk_size] for i in some])
+            logits = self.extend([slots[i] for i in some], [prompts[i][at:at + chunk_size] for i in some], [at] * len(some))
             for row, i in zip(logits, some):
                 if len(prompts[i]) <= at + chunk_size:
                     out[i] = row
