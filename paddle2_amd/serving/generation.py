@@ -416,46 +416,48 @@ class LlamaGenerator:
             rows = {k: v[:logits.shape[0]] if torch.is_tensor(v) else v for k, v in settings.items()}
             return sample_tokens(logits, u, **rows)
 
-        heads = list(range(0, n_seq, n_ret))   # the slot that runs each prompt
-        if not prompts:
-            first = None
-        elif chunk_size is not None:
-            first = self.prefill_chunks(heads, prompts, int(chunk_size))
-        elif len(prompts) > 1:   # one packed prefill for all prompts (per-prompt when a single one is given)
-            first = self.prefill_batch(heads, prompts)
-        else:
-            first = self.prefill(0, torch.as_tensor(prompts[0], dtype=torch.long))[None]
-        if n_ret > 1 and prompts:
-            for s, p in zip(heads, prompts):
-                self.cache.fork(s, range(s + 1, s + n_ret), len(p))
-            first = first.repeat_interleave(n_ret, 0)
-        if sampler == "fused" and prompts:
-            first_toks = draw(first)
-        for i in range(n_seq):
-            t = first_toks[i] if sampler == "fused" else draw(first[i:i + 1])[0]
-            n = len(prompts[i // n_ret])
-            toks[i] = t
-            pos[i] = n
-            outs[i].append(int(t))
-            self.cache.allocate(i, n + max_new_tokens + 1)
-        for i in range(n_seq, B):  # idle slots decode a dummy token at position 0
-            self.cache.allocate(i, max_new_tokens + 2)
-        for _ in range(max_new_tokens - 1):
-            logits = self.decode_step(toks, pos)
-            nxt = draw(logits)
-            pos = pos + 1
+        try:
+            heads = list(range(0, n_seq, n_ret))   # the slot that runs each prompt
+            if not prompts:
+                first = None
+            elif chunk_size is not None:
+                first = self.prefill_chunks(heads, prompts, int(chunk_size))
+            elif len(prompts) > 1:   # one packed prefill for all prompts (per-prompt when a single one is given)
+                first = self.prefill_batch(heads, prompts)
+            else:
+                first = self.prefill(0, torch.as_tensor(prompts[0], dtype=torch.long))[None]
+            if n_ret > 1 and prompts:
+                for s, p in zip(heads, prompts):
+                    self.cache.fork(s, range(s + 1, s + n_ret), len(p))
+                first = first.repeat_interleave(n_ret, 0)
+            if sampler == "fused" and prompts:
+                first_toks = draw(first)
             for i in range(n_seq):
-                if done[i]:
-                    continue
-                ti = int(nxt[i])
-                outs[i].append(ti)
-                if eos_token_id is not None and ti == eos_token_id:
-                    done[i] = True
-            toks = nxt
-            if all(done):
-                break
-        for i in range(B):
-            self.cache.free(i)
+                t = first_toks[i] if sampler == "fused" else draw(first[i:i + 1])[0]
+                n = len(prompts[i // n_ret])
+                toks[i] = t
+                pos[i] = n
+                outs[i].append(int(t))
+                self.cache.allocate(i, n + max_new_tokens + 1)
+            for i in range(n_seq, B):  # idle slots decode a dummy token at position 0
+                self.cache.allocate(i, max_new_tokens + 2)
+            for _ in range(max_new_tokens - 1):
+                logits = self.decode_step(toks, pos)
+                nxt = draw(logits)
+                pos = pos + 1
+                for i in range(n_seq):
+                    if done[i]:
+                        continue
+                    ti = int(nxt[i])
+                    outs[i].append(ti)
+                    if eos_token_id is not None and ti == eos_token_id:
+                        done[i] = True
+                toks = nxt
+                if all(done):
+                    break
+        finally:   # (a call that fails half way would leave slots that share pages)
+            for i in range(B):
+                self.cache.free(i)
         return outs
 
 

@@ -54,3 +54,18 @@ def test_chunked_generation_after_an_earlier_prompt_and_a_failed_call():
     with pytest.raises(IndexError):
         gen.generate([[3] * 20], 60, chunk_size=4)
     assert gen.generate(prompts, 6, chunk_size=4) == plain
+
+
+# ============================================================================ calls that fail half way
+def test_generate_that_fails_leaves_its_slots_free():
+    """Out of room after the pages were forked, in the prompt, or at the draw: the slots are free and the next call works."""
+    m = _llama("cpu")
+    gen = LlamaGenerator(m, max_batch=2, max_seq_len=64, block_size=8, use_graph=False)
+    plain = gen.generate([[1, 2, 3]], 6)
+    for err, f in ((IndexError, lambda: gen.generate([list(range(1, 18))], 60, num_return_sequences=2)),
+                   (IndexError, lambda: gen.generate([[4] * 70, [1]], 2)),
+                   (ValueError, lambda: gen.generate([[1, 2]], 3, temperature=-1.0, sampler="fused"))):
+        with pytest.raises(err):
+            f()
+        assert gen.cache.num_free_blocks == len(gen.cache._holders) and gen.cache.seq_lens.tolist() == [0, 0]
+        assert gen.generate([[1, 2, 3]], 6) == plain
