@@ -394,8 +394,12 @@ class LlamaGenerator:
         if sampler not in ("fused", "multinomial") or (sampler == "multinomial" and fused_only):
             raise ValueError(f"generate: sampler {sampler!r} with temperature={temperature}, top_k={top_k}, top_p={top_p}, "
                              f"min_p={min_p}")
+        if chunk_size is not None and (int(chunk_size) < 1 or min((len(p) for p in prompts), default=1) < 1):
+            raise ValueError(f"generate: chunk_size {chunk_size}, prompts of {[len(p) for p in prompts]} tokens")
         for s in range(self.max_batch):   # (idle slots are written too)
             self.cache.check_writable(s)
+            if s < n_seq and s % n_ret and self.cache._owned.get(s):
+                raise ValueError(f"generate: slot {s} is to hold another continuation, but it is in use: free it first")
         gen = torch.Generator(device=self.dev).manual_seed(seed) if self.dev.type == "cuda" else \
             torch.Generator().manual_seed(seed)
         B = self.max_batch

@@ -69,3 +69,18 @@ def test_generate_that_fails_leaves_its_slots_free():
             f()
         assert gen.cache.num_free_blocks == len(gen.cache._holders) and gen.cache.seq_lens.tolist() == [0, 0]
         assert gen.generate([[1, 2, 3]], 6) == plain
+
+
+def test_generate_that_is_refused_changes_nothing():
+    """Bad arguments, and continuations whose slots hold something, are refused before anything is computed."""
+    gen = LlamaGenerator(_llama("cpu"), max_batch=3, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill(1, torch.arange(5, 16))
+    pools = [t.clone() for t in gen.cache.k + gen.cache.v]
+    calls = []
+    gen._layer_qkv = lambda *a: calls.append(a)
+    for f in (lambda: gen.generate([[1, 2]], 2, num_return_sequences=2), lambda: gen.generate([[1, 2]], 2, chunk_size=0),
+              lambda: gen.generate([[1, 2], []], 2, chunk_size=4), lambda: gen.generate([[1, 2]], 2, top_k=[1, 2])):
+        with pytest.raises(ValueError):
+            f()
+    assert not calls and gen.cache.seq_lens.tolist() == [0, 11, 0] and len(gen.cache._owned[1]) == 2
+    assert all(torch.equal(a, b) for a, b in zip(pools, gen.cache.k + gen.cache.v))
