@@ -56,7 +56,7 @@ __global__ __launch_bounds__(256) void decode_kernel(const bf16* __restrict__ q,
     long blk = b;
     int off = t;
     if (block_table) {
-      blk = block_table[(long)b * max_blocks + t / block_size];
+      blk = max(block_table[(long)b * max_blocks + t / block_size], 0);   // (negative: no page, an idle sequence's)
       off = t % block_size;
     }
     const long base = blk * s_blk + (long)off * s_tok + (long)hk * s_head + ln * 8;
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(256, 2) void decode_mfma_kernel(const bf16* __restr
   const int ntile = k_end > k_begin ? (k_end - k_begin + 31) / 32 : 0;
 
   // block of this lane's keys (u = 0, 1) in tile t; keys past the sequence are clamped so their (masked)
-  // loads stay inside valid blocks
+  // loads stay inside valid blocks (a negative entry, no page of an idle sequence, is read as page 0)
   auto blocks = [&](int t, int (&bk)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
@@ -187,7 +187,7 @@ __global__ __launch_bounds__(256, 2) void decode_mfma_kernel(const bf16* __restr
     for (int u = 0; u < 2; ++u) {
       const int key = min(k_begin + 32 * t + 16 * u + c16, len - 1);
       const int off = PAGED ? (key & ((1 << bs_shift) - 1)) : key;
-      const long a = (long)bk[u] * s_blk + (long)off * s_tok + (long)hk * s_head + 8 * h;
+      const long a = (long)(PAGED ? max(bk[u], 0) : bk[u]) * s_blk + (long)off * s_tok + (long)hk * s_head + 8 * h;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         kk[u][c] = *reinterpret_cast<const bf16x8*>(kc + a + 32 * c);
@@ -356,7 +356,9 @@ __global__ __launch_bounds__(256) void cache_write_kernel(const bf16* __restrict
     long blk = b;
     int off = t;
     if (block_table) {
+      if (t < 0 || t / block_size >= max_blocks) continue;
       blk = block_table[(long)b * max_blocks + t / block_size];
+      if (blk < 0) continue;   // no page: the token is not stored
       off = t % block_size;
     }
     const long dst = blk * s_blk + (long)off * s_tok + (long)h * s_head + c * 8;

@@ -54,6 +54,7 @@ def decode_attention(q, k_cache, v_cache, seq_lens, block_table=None, block_size
     q: [B, Hq, D] (any strides with unit inner stride); seq_lens: [B] int32 (#valid keys incl. the
     new token).  layout "paged": caches [num_blocks, block_size, Hk, D] + block_table [B, max_blocks];
     layout "bhsd": caches [B, Hk, max_s, D] (MMHA); layout "paddle_block": [num_blocks, Hk, block_size, D].
+    A negative entry of the block table is read as page 0 (the row of an idle sequence: its output means nothing).
     Returns out [B, Hq, D]."""
     B, Hq, D = q.shape
     if layout == "paged":
@@ -99,7 +100,7 @@ def decode_attention(q, k_cache, v_cache, seq_lens, block_table=None, block_size
             vs = v_cache[b, :, :L].float()
         else:
             idx = torch.arange(L, device=q.device)
-            blocks = block_table[b, idx // bs].long()
+            blocks = block_table[b, idx // bs].long().clamp(min=0)
             if layout == "paged":
                 ks = k_cache[blocks, idx % bs].permute(1, 0, 2).float()
                 vs = v_cache[blocks, idx % bs].permute(1, 0, 2).float()
@@ -114,7 +115,8 @@ def decode_attention(q, k_cache, v_cache, seq_lens, block_table=None, block_size
 
 
 def write_kv(k, v, k_cache, v_cache, tok_batch, tok_pos, block_table=None, layout="paged"):
-    """Store rows k/v [n_tok, Hk, D] at (sequence tok_batch[i], position tok_pos[i]) of the cache."""
+    """Store rows k/v [n_tok, Hk, D] at (sequence tok_batch[i], position tok_pos[i]) of the cache.  A token whose entry in the
+    block table is negative has no page and is not stored."""
     n, Hk, D = k.shape
     if layout == "paged":
         bs = k_cache.shape[1]
@@ -135,8 +137,17 @@ def write_kv(k, v, k_cache, v_cache, tok_batch, tok_pos, block_table=None, layou
         return
     tb, tp = tok_batch.long(), tok_pos.long()
     if block_table is not None:
+        if n == 0:
+            return
         blk = block_table.long()[tb, tp // bs]
         off = tp % bs
+        # tokens without a page repeat the store of the first that has one, or store what is there already where none has:
+        # nothing here waits for the device
+        kept = blk >= 0
+        at = torch.where(kept, torch.arange(n, device=blk.device), kept.int().argmax())
+        blk, off = blk[at].clamp(min=0), off[at]
+        old = (k_cache[blk, off], v_cache[blk, off]) if layout == "paged" else (k_cache[blk, :, off], v_cache[blk, :, off])
+        k, v = (torch.where(kept.any(), x[at].to(o.dtype), o) for x, o in zip((k, v), old))
     else:
         blk, off = tb, tp
     if layout == "paged":
@@ -149,7 +160,8 @@ def write_kv(k, v, k_cache, v_cache, tok_batch, tok_pos, block_table=None, layou
 
 # ============================================================================ paged KV cache
 class PagedKVCache:
-    """Per-layer K/V block pools [num_blocks, block_size, Hk, D] with a free list and block tables.
+    """Per-layer K/V block pools [num_blocks, block_size, Hk, D] with a free list and block tables.  Entries of the table that
+    are no page of the sequence are -1: write_kv stores nothing there.
 
     Pages may be shared: ``fork`` gives another sequence the full pages of one, and a page goes back to the free list
     when its last holder lets go.  Full pages are only read; the page a sequence still writes is always its own, and to
@@ -164,7 +176,7 @@ class PagedKVCache:
                   for _ in range(num_layers)]
         self.v = [torch.zeros_like(t) for t in self.k]
         self.max_blocks_per_seq = (max_seq_len + block_size - 1) // block_size
-        self.block_table = torch.zeros(max_batch, self.max_blocks_per_seq, dtype=torch.int32, device=dev)
+        self.block_table = torch.full((max_batch, self.max_blocks_per_seq), -1, dtype=torch.int32, device=dev)
         self.seq_lens = torch.zeros(max_batch, dtype=torch.int32, device=dev)
         self._free = list(range(num_blocks - 1, -1, -1))
         self._owned = {}
@@ -197,6 +209,7 @@ class PagedKVCache:
     def free(self, slot):
         for b in self._owned.pop(slot, []):
             self._drop(b)
+        self.block_table[slot] = -1
         self.seq_lens[slot] = 0
 
     @property
@@ -219,7 +232,7 @@ class PagedKVCache:
 
     def _write_rows(self, slots):
         """The block-table rows of ``slots`` from the host's lists, in one copy."""
-        rows = torch.zeros(len(slots), self.max_blocks_per_seq, dtype=torch.int32)
+        rows = torch.full((len(slots), self.max_blocks_per_seq), -1, dtype=torch.int32)
         for i, s in enumerate(slots):
             rows[i, :len(self._owned[s])] = torch.tensor(self._owned[s], dtype=torch.int32)
         dev = self.block_table.device
@@ -271,6 +284,8 @@ class PagedKVCache:
         shared = last is not None and self._holders[last] > 1
         if shared and not self._free and all(self._holders[b] > 1 for b in have[keep:]):
             raise RuntimeError("PagedKVCache out of blocks")
+        if len(have) > keep:
+            self.block_table[slot, keep:] = -1
         while len(have) > keep:
             self._drop(have.pop())
         if shared:

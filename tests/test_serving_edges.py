@@ -84,3 +84,82 @@ def test_generate_that_is_refused_changes_nothing():
             f()
     assert not calls and gen.cache.seq_lens.tolist() == [0, 11, 0] and len(gen.cache._owned[1]) == 2
     assert all(torch.equal(a, b) for a, b in zip(pools, gen.cache.k + gen.cache.v))
+
+
+# ============================================================================ pages that a sequence does not hold
+def _decode(gen, tokens, positions):
+    """One decode_step of all slots; returns the logits."""
+    return gen.decode_step(torch.tensor(tokens, device=gen.dev), torch.tensor(positions, dtype=torch.int32, device=gen.dev))
+
+
+def _alone(m, prompt, *tokens):
+    """The logits after ``tokens`` (one each) of a sequence that has a generator for itself."""
+    gen = LlamaGenerator(m, max_batch=1, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill(0, torch.tensor(prompt))
+    gen.cache.allocate(0, len(prompt) + len(tokens))
+    out = [_decode(gen, [t], [len(prompt) + i])[0].clone() for i, t in enumerate(tokens)]
+    return out[-1]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("dev,dtype", [("cpu", "float32"), pytest.param("cuda", "bfloat16", marks=pytest.mark.gpu),
+                                       pytest.param("cuda", "float16", marks=pytest.mark.gpu)])
+def test_idle_slots_write_nowhere(dev, dtype, graph):
+    """decode_step runs every slot: those without pages, and freed ones, leave the others' pages alone."""
+    if graph and dtype != "bfloat16":
+        pytest.skip("captured with the bfloat16 kernels alone")
+    m = _llama(dev, dtype=dtype)
+    a, b = [1, 5, 9, 3], [7, 2, 8, 6, 4]
+    gen = LlamaGenerator(m, max_batch=4, max_seq_len=64, block_size=8, use_graph=graph)
+    gen.prefill(0, torch.tensor(a))
+    got = _decode(gen, [11, 3, 3, 3], [4, 0, 9, 0])
+    torch.testing.assert_close(got[0].float(), _alone(m, a, 11).float(), **_near(dev))
+    gen.prefill(1, torch.tensor([9] * 20))
+    gen.cache.free(1)
+    gen.prefill(2, torch.tensor(b))          # takes a page that slot 1 gave back
+    got = _decode(gen, [12, 3, 13, 3], [5, 1, 5, 17])
+    torch.testing.assert_close(got[2].float(), _alone(m, b, 13).float(), **_near(dev))
+    torch.testing.assert_close(got[0].float(), _alone(m, a, 11, 12).float(), **_near(dev))
+
+
+@pytest.mark.parametrize("layout", ["paged", "paddle_block"])
+@pytest.mark.parametrize("dev,dtype", [("cpu", torch.float32), pytest.param("cuda", torch.bfloat16, marks=pytest.mark.gpu),
+                                       pytest.param("cuda", torch.float16, marks=pytest.mark.gpu)])
+def test_write_kv_drops_tokens_without_a_page(dev, dtype, layout):
+    g = torch.Generator().manual_seed(1)
+    shape = (5, 4, 2, 8) if layout == "paged" else (5, 2, 4, 8)
+    kc, vc = (torch.randn(shape, generator=g).to(dev, dtype) for _ in range(2))
+    k, v = (torch.randn(4, 2, 8, generator=g).to(dev, dtype) for _ in range(2))
+    table = torch.tensor([[3, -1], [-1, -1], [1, 0]], dtype=torch.int32, device=dev)
+    pos = torch.tensor([2, 5, 1, 7], dtype=torch.int32, device=dev)
+    for seqs, stored in (([0, 0, 1, 2], {0: (3, 2), 3: (0, 3)}), ([1, 0, 1, 1], {})):
+        want_k, want_v = kc.clone(), vc.clone()
+        for i, (page, row) in stored.items():
+            at = (page, row) if layout == "paged" else (page, slice(None), row)
+            want_k[at], want_v[at] = k[i], v[i]
+        serving.write_kv(k, v, kc, vc, torch.tensor(seqs, dtype=torch.int32, device=dev), pos, table, layout=layout)
+        assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
+        k, v = k + 1, v - 1
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_tables_hold_no_page_that_is_not_held(dev):
+    """Entries behind a sequence's own pages are -1, after every change of the cache."""
+    c = serving.PagedKVCache(1, 12, 4, 1, 8, 4, 16, dtype=torch.float32, device=torch.device(dev))
+
+    def check():
+        for s, row in enumerate(c.block_table.tolist()):
+            own = c._owned.get(s, [])
+            assert row == own + [-1] * (len(row) - len(own))
+
+    check()
+    c.allocate(0, 15), c.allocate(1, 6)
+    check()
+    c.fork(0, [2, 3], 8)
+    check()
+    c.truncate(0, 5), c.truncate(2, 3)
+    check()
+    c.free(1), c.compact()
+    check()
+    c.free(0), c.free(2), c.free(3)
+    check()
