@@ -245,8 +245,9 @@ class PagedKVCache:
 
     def fork(self, slot, new_slots, num_tokens=None):
         """Sequences ``new_slots`` (free ones) become copies of the first ``num_tokens`` tokens of ``slot`` (default: its
-        seq_lens).  Full pages are shared, the last, partly filled one is copied for each, so all of them may grow on
-        their own.  RuntimeError, with nothing changed, when there are too few free pages."""
+        seq_lens).  Full pages are shared; the page of position ``num_tokens``, where the next token goes, is each one's own
+        (a copy where tokens stand in it, and none where the table ends or ``slot`` holds no page), so all of them may grow
+        on their own.  RuntimeError, with nothing changed, when there are too few free pages."""
         new_slots = [self._slot(int(s)) for s in new_slots]
         have = self._owned.get(self._slot(slot), [])
         n = int(self.seq_lens[slot]) if num_tokens is None else int(num_tokens)
@@ -255,7 +256,8 @@ class PagedKVCache:
         if len(set(new_slots)) < len(new_slots) or any(self._owned.get(s) for s in new_slots):
             raise ValueError(f"PagedKVCache.fork: slots {new_slots} must be different and free")
         full, rest = n // self.block_size, n % self.block_size
-        if rest and len(self._free) < len(new_slots):
+        grow = bool(have) and full < self.max_blocks_per_seq
+        if grow and len(self._free) < len(new_slots):
             raise RuntimeError("PagedKVCache out of blocks")
         if not new_slots:
             return
@@ -264,10 +266,10 @@ class PagedKVCache:
             for b in have[:full]:
                 self._holders[b] += 1
             self._owned[s] = have[:full]
-            if rest:
+            if grow:
                 own.append(self._take())
                 self._owned[s].append(own[-1])
-        if own:
+        if rest:
             self.copy_blocks([have[full]] * len(own), own)
         self._write_rows(new_slots)
         self.seq_lens[torch.tensor(new_slots, device=self.seq_lens.device)] = n

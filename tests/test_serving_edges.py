@@ -163,3 +163,35 @@ def test_tables_hold_no_page_that_is_not_held(dev):
     check()
     c.free(0), c.free(2), c.free(3)
     check()
+
+
+# ============================================================================ sequences that end at a page's border
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("n", [13, 15, 16, 17, 24])
+def test_decoding_after_a_fork(dev, n):
+    """Every continuation has a page of its own for its next token, also where the prompt fills its pages."""
+    m = _llama(dev)
+    prompt = [(7 * i + 3) % 500 for i in range(n)]
+    gen = LlamaGenerator(m, max_batch=4, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill(1, torch.tensor(prompt))
+    gen.cache.fork(1, [0, 3])
+    got = _decode(gen, [11, 12, 9, 13], [n, n, 0, n])
+    for s, t in ((0, 11), (1, 12), (3, 13)):
+        torch.testing.assert_close(got[s].float(), _alone(m, prompt, t).float(), **_near(dev))
+    for s in range(4):
+        gen.cache.free(s)
+    assert gen.cache.num_free_blocks == len(gen.cache._holders)
+
+
+def test_fork_takes_the_next_page_where_there_is_one():
+    c = serving.PagedKVCache(1, 8, 4, 1, 8, 4, 16, dtype=torch.float32, device=torch.device("cpu"))
+    c.allocate(0, 16)
+    c.fork(0, [1], 16)             # the table ends there
+    assert c._owned[1] == c._owned[0] and c.num_free_blocks == 4
+    c.fork(0, [2], 8)
+    assert c._owned[2][:2] == c._owned[0][:2] and len(c._owned[2]) == 3 and c._holders[c._owned[2][2]] == 1
+    c.free(1), c.allocate(1, 12)
+    state = (list(c._free), {k: list(v) for k, v in c._owned.items()}, list(c._holders), c.block_table.clone())
+    with pytest.raises(RuntimeError):
+        c.fork(0, [3], 4)          # no page for its next token
+    assert state[:3] == (c._free, c._owned, c._holders) and torch.equal(state[3], c.block_table)
