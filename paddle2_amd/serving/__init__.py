@@ -275,14 +275,16 @@ class PagedKVCache:
         self.seq_lens[torch.tensor(new_slots, device=self.seq_lens.device)] = n
 
     def truncate(self, slot, num_tokens):
-        """Sequence ``slot`` goes back to its first ``num_tokens`` tokens: the pages behind them are given up, and a last
-        page that it will write again but shares is replaced by a copy."""
+        """Sequence ``slot`` goes back to its first ``num_tokens`` tokens.  The page of position ``num_tokens``, where the next
+        token goes, is kept (one that is shared is replaced, by a copy where tokens stand in it); those behind it are given
+        up.  RuntimeError, with nothing changed, when no page is free to replace it."""
         have = self._owned.get(self._slot(slot), [])
         n = int(num_tokens)
         if not 0 <= n <= len(have) * self.block_size:
             raise ValueError(f"PagedKVCache.truncate: {n} tokens, slot {slot} holds {len(have)} blocks of {self.block_size}")
-        keep = -(-n // self.block_size)
-        last = have[keep - 1] if n % self.block_size else None
+        full, rest = n // self.block_size, n % self.block_size
+        keep = min(full + 1, len(have))
+        last = have[full] if full < len(have) else None
         shared = last is not None and self._holders[last] > 1
         if shared and not self._free and all(self._holders[b] > 1 for b in have[keep:]):
             raise RuntimeError("PagedKVCache out of blocks")
@@ -292,7 +294,8 @@ class PagedKVCache:
             self._drop(have.pop())
         if shared:
             have[-1] = self._take()
-            self.copy_blocks([last], [have[-1]])
+            if rest:
+                self.copy_blocks([last], [have[-1]])
             self._drop(last)
             self._write_rows([slot])
         self.seq_lens[slot] = n

@@ -195,3 +195,54 @@ def test_fork_takes_the_next_page_where_there_is_one():
     with pytest.raises(RuntimeError):
         c.fork(0, [3], 4)          # no page for its next token
     assert state[:3] == (c._free, c._owned, c._holders) and torch.equal(state[3], c.block_table)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("keep", [15, 16, 17, 18])
+def test_decoding_after_a_truncation(dev, keep):
+    """Rejected tokens are given up, another sequence takes pages, and both go on."""
+    m = _llama(dev)
+    prompt, other = [(7 * i + 3) % 500 for i in range(15)], [(5 * i + 1) % 400 for i in range(18)]
+    gen = LlamaGenerator(m, max_batch=2, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill(0, torch.tensor(prompt))
+    gen.extend([0], [[21, 22, 23]])
+    gen.cache.truncate(0, keep)
+    gen.prefill(1, torch.tensor(other))
+    got = _decode(gen, [11, 12], [keep, 18])
+    torch.testing.assert_close(got[0].float(), _alone(m, (prompt + [21, 22, 23])[:keep], 11).float(), **_near(dev))
+    torch.testing.assert_close(got[1].float(), _alone(m, other, 12).float(), **_near(dev))
+
+
+def test_truncate_keeps_the_next_page():
+    """The page of the next token stays, and is replaced where it is shared; nothing changes when none is left for that."""
+    c = serving.PagedKVCache(1, 6, 4, 1, 8, 3, 24, dtype=torch.float32, device=torch.device("cpu"))
+    c.allocate(0, 14)
+    first = list(c._owned[0])
+    c.truncate(0, 8)
+    assert c._owned[0] == first[:3] and c.num_free_blocks == 3
+    c.truncate(0, 7)
+    assert c._owned[0] == first[:2]
+    c.truncate(0, 8)                       # no page was there for it: nothing is taken
+    assert c._owned[0] == first[:2]
+    c.fork(0, [1])
+    shared, own = c._owned[0], c._owned[1][2]
+    c.truncate(1, 4)
+    assert c._owned[1][0] == shared[0] and c._owned[1][1] not in shared and c._holders[c._owned[1][1]] == 1
+    assert c._owned[1][1] == own or c._holders[own] == 0
+    c.truncate(1, 0)
+    assert len(c._owned[1]) == 1 and c._holders[c._owned[1][0]] == 1 and c._holders[shared[0]] == 1
+    c.free(1), c.truncate(0, 0)
+    assert c._owned[0] == first[:1] and c.num_free_blocks == 5
+
+    c = serving.PagedKVCache(1, 4, 4, 1, 8, 3, 12, dtype=torch.float32, device=torch.device("cpu"))
+    c.allocate(0, 12)
+    c.fork(0, [1], 12)                     # all pages shared, the table ends there
+    c.allocate(2, 4)
+    state = ({k: list(v) for k, v in c._owned.items()}, list(c._holders), c.block_table.clone(), c.seq_lens.clone())
+    for n in (0, 4, 5):
+        with pytest.raises(RuntimeError):
+            c.truncate(1, n)
+        assert state[:2] == (c._owned, c._holders)
+        assert torch.equal(state[2], c.block_table) and torch.equal(state[3], c.seq_lens)
+    c.truncate(1, 12)
+    assert state[:2] == (c._owned, c._holders)
