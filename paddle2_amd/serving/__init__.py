@@ -181,6 +181,7 @@ class PagedKVCache:
         self._free = list(range(num_blocks - 1, -1, -1))
         self._owned = {}
         self._holders = [0] * num_blocks
+        self._shared = 0   # pages with more than one holder
         self._copier = None
 
     def _take(self):
@@ -192,6 +193,7 @@ class PagedKVCache:
 
     def _drop(self, b):
         self._holders[b] -= 1
+        self._shared -= self._holders[b] == 1
         if self._holders[b] == 0:
             self._free.append(b)
 
@@ -222,6 +224,15 @@ class PagedKVCache:
         sequences it shares with.  truncate(slot, start) makes room, free(slot) lets go of all."""
         if any(self._holders[b] > 1 for b in self._owned.get(slot, [])[start // self.block_size:]):
             raise ValueError(f"PagedKVCache: slot {slot} shares pages behind token {start}: truncate or free it first")
+
+    def check_step(self, positions):
+        """ValueError if a slot shares the page of its position in ``positions`` (one per slot): decode_step would write it.
+        Reads the positions on the host, but only while any page is shared."""
+        if self._shared:
+            for s, p in enumerate(positions.tolist()):
+                have = self._owned.get(s, [])
+                if 0 <= p // self.block_size < len(have) and self._holders[have[p // self.block_size]] > 1:
+                    raise ValueError(f"PagedKVCache: slot {s} shares the page of token {p}: truncate or free it first")
 
     def copy_blocks(self, src, dst):
         """Page src[i] -> page dst[i] in the K and V pools of every layer, one launch (KVBlockCopier.copy)."""
@@ -265,6 +276,7 @@ class PagedKVCache:
         for s in new_slots:
             for b in have[:full]:
                 self._holders[b] += 1
+                self._shared += self._holders[b] == 2
             self._owned[s] = have[:full]
             if grow:
                 own.append(self._take())

@@ -347,7 +347,11 @@ class LlamaGenerator:
 
     @torch.no_grad()
     def decode_step(self, tokens, positions):
-        """tokens/positions: [max_batch] (inactive slots may hold anything valid) -> logits [B, V]."""
+        """tokens/positions: [max_batch] (inactive slots may hold anything valid) -> logits [B, V].
+
+        Every slot's token is stored at its position, the inactive ones' too: a position whose page the slot shares with
+        another sequence is a ValueError (PagedKVCache.check_step), and a slot without a page there stores nothing."""
+        self.cache.check_step(positions)
         self._tok.copy_(tokens)
         self._pos.copy_(positions)
         self._lens.copy_(positions + 1)

@@ -246,3 +246,25 @@ def test_truncate_keeps_the_next_page():
         assert torch.equal(state[2], c.block_table) and torch.equal(state[3], c.seq_lens)
     c.truncate(1, 12)
     assert state[:2] == (c._owned, c._holders)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_decoding_into_a_shared_page_is_refused(dev):
+    """decode_step at a position whose page another sequence reads too: refused, with nothing written; truncated, it goes on."""
+    m = _llama(dev)
+    prompt = [(7 * i + 3) % 500 for i in range(17)]
+    gen = LlamaGenerator(m, max_batch=3, max_seq_len=64, block_size=8, use_graph=False)
+    gen.prefill(0, torch.tensor(prompt))
+    gen.cache.fork(0, [1])
+    pools = [t.clone() for t in gen.cache.k + gen.cache.v]
+    for pos in ([17, 9, 0], [0, 17, 0]):          # (slot 2 holds nothing: any position will do)
+        with pytest.raises(ValueError, match="shares"):
+            _decode(gen, [11, 12, 5], pos)
+    assert all(torch.equal(a, b) for a, b in zip(pools, gen.cache.k + gen.cache.v))
+    _decode(gen, [11, 12, 5], [17, 17, 40])
+    gen.cache.truncate(1, 9)
+    got = _decode(gen, [13, 12, 5], [18, 9, 0])
+    torch.testing.assert_close(got[0].float(), _alone(m, prompt, 11, 13).float(), **_near(dev))
+    torch.testing.assert_close(got[1].float(), _alone(m, prompt[:9], 12).float(), **_near(dev))
+    gen.cache.free(0)
+    _decode(gen, [13, 12, 5], [0, 0, 0])          # nothing is shared any more
