@@ -28,7 +28,7 @@ from ..framework.tensor import Tensor
 from ..ops import _native as N
 from ..ops import torch_ops as T
 from ..distributed.collective import ring_all_reduce
-from .paged import KVBlockCopier, chunk_attention, copy_kv_blocks  # noqa: F401
+from .paged import KVBlockCopier, attend_chunk, chunk_attention, copy_kv_blocks  # noqa: F401
 from .sampling import sample_tokens  # noqa: F401
 
 _wrap = Tensor._wrap
@@ -437,8 +437,8 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
         cu_q = torch.zeros(len(several) + 1, dtype=torch.int32)
         cu_q[1:] = torch.tensor([n for _, _, n, _ in several], dtype=torch.int32).cumsum(0)
         lens = torch.tensor([dec[b] + n for b, _, n, _ in several], dtype=torch.int32, device=t.device)
-        oc = chunk_attention(torch.cat([q for _, _, _, q in several]), kc, vc, cu_q.to(t.device), lens,
-                             bt[torch.tensor([b for b, _, _, _ in several], device=t.device)], layout="paddle_block")
+        oc = attend_chunk(torch.cat([q for _, _, _, q in several]), kc, vc, cu_q.to(t.device), lens,
+                          bt[torch.tensor([b for b, _, _, _ in several], device=t.device)], layout="paddle_block")
         for (_, s0, n, _), r in zip(several, cu_q.tolist()):
             out[s0:s0 + n] = oc[r:r + n]
     return _wrap(out.reshape(tok, Hq * D)), qkv, key_cache, value_cache

@@ -19,7 +19,8 @@ import torch
 
 from ..framework.tensor import Tensor
 from ..ops import torch_ops as T
-from . import PagedKVCache, chunk_attention, decode_attention, sample_tokens, write_kv
+from . import PagedKVCache, decode_attention, sample_tokens, write_kv
+from .paged import attend_chunk
 
 
 def sample_logits(logits, temperature=1.0, top_k=0, top_p=1.0, generator=None):
@@ -304,7 +305,7 @@ class LlamaGenerator:
             qk = T.rope(qkv[:, :, :nh + nkv], self.cos, self.sin, pos_l, style=0)
             q, k, v = qk[0, :, :nh], qk[0, :, nh:], qkv[0, :, nh + nkv:]
             write_kv(k, v, self.cache.k[li], self.cache.v[li], tok_batch, pos, self.cache.block_table)
-            o = chunk_attention(q, self.cache.k[li], self.cache.v[li], cu, keys, table)
+            o = attend_chunk(q, self.cache.k[li], self.cache.v[li], cu, keys, table)
             x, residual = self._layer_out(layer, o.reshape(1, total, nh * d), residual)
         self.cache.seq_lens[slot_t] = keys
         return self._logits_of(x[:, last], residual[:, last])[0]

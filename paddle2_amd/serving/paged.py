@@ -113,13 +113,30 @@ def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=Non
     return Tensor._wrap(out) if wrap else out
 
 
+def attend_chunk(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, layout="paged"):
+    """chunk_attention of checked torch tensors, for the framework's own paths: by its PyTorch definition where the kernel
+    does not take the type or the head dim, as decode_attention does."""
+    Hk = k_cache.shape[2 if layout == "paged" else 1]
+    if q.device.type != "cuda" or _kernel_takes(q, Hk):
+        return chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, layout=layout)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    with torch.no_grad():
+        _chunk_reference(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, 1 if layout == "paged" else 2,
+                         1.0 / math.sqrt(q.shape[2]), out)
+    return out
+
+
+def _kernel_takes(q, Hk):
+    return q.dtype in (torch.bfloat16, torch.float16) and q.shape[2] in _HEAD_DIMS and q.shape[1] <= 128 * Hk
+
+
 def _chunk_native(q, kc, vc, cu, lens, table, tok, head, scale, out):
     T, Hq, D = q.shape
     B, max_blocks = table.shape
     ks, sk, so = kc.shape, kc.stride(), out.stride()
     bs, Hk = ks[tok], ks[head]
     G = Hq // Hk
-    if q.dtype not in (torch.bfloat16, torch.float16) or D not in _HEAD_DIMS or G > 128:
+    if not _kernel_takes(q, Hk):
         raise ValueError(f"chunk_attention: {q.dtype} with head dim {D} and {G} query heads per kv head (bfloat16 or float16, "
                          f"{_HEAD_DIMS}, at most 128)")
     if not max_blocks or not ks[0]:

@@ -268,3 +268,41 @@ def test_decoding_into_a_shared_page_is_refused(dev):
     torch.testing.assert_close(got[1].float(), _alone(m, prompt[:9], 12).float(), **_near(dev))
     gen.cache.free(0)
     _decode(gen, [13, 12, 5], [0, 0, 0])          # nothing is shared any more
+
+
+# ============================================================================ models whose attention has no kernel of its own
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("kw", [dict(dtype="float32"), dict(num_attention_heads=8, num_key_value_heads=2)], ids=str)
+def test_extend_with_any_type_and_head_dim(dev, kw):
+    """A model that prefills and decodes also takes its prompts in pieces (32 bits; a head dim of 32)."""
+    from paddle2_amd.models import LlamaConfig, LlamaForCausalLM
+
+    paddle.seed(3)
+    kw = dict(dict(num_attention_heads=4, num_key_value_heads=2, dtype="bfloat16" if dev == "cuda" else "float32"), **kw)
+    m = LlamaForCausalLM(LlamaConfig.tiny(**kw))
+    if dev == "cuda":
+        paddle.set_device("gpu:0")
+        m.to(device="gpu:0")
+    m.eval()
+    prompts = [[(7 * i + 3) % 500 for i in range(21)], [9, 8, 7]]
+    gen = LlamaGenerator(m, max_batch=2, max_seq_len=64, block_size=8, use_graph=False)
+    whole = gen.prefill_batch([0, 1], prompts)
+    parts = gen.prefill_chunks([0, 1], prompts, 8)
+    tol = dict(atol=1e-4, rtol=1e-4) if kw["dtype"] == "float32" else _near(dev)
+    torch.testing.assert_close(parts.float(), whole.float(), **tol)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_block_multihead_attention_several_new_tokens_in_32_bits(dev):
+    g = torch.Generator().manual_seed(2)
+    W = paddle.Tensor._wrap
+    kc, vc = (torch.randn(6, 2, 16, 32, generator=g) for _ in range(2))
+    qkv = torch.randn(4, 8 * 32, generator=g)
+
+    def run(dev):
+        i32 = lambda v: W(torch.tensor(v, dtype=torch.int32, device=dev))  # noqa: E731
+        args = [W(t.clone().to(dev)) for t in (qkv, kc, vc)]
+        return serving.block_multihead_attention(*args, i32([0, 0]), i32([20, 7]), i32([3, 1]), None, None, i32([0, 3, 4]),
+                                                 i32([0, 3, 4]), i32([[0, 1], [2, 3]]), block_size=16)[0]._t.cpu()
+
+    torch.testing.assert_close(run(dev), run("cpu"), atol=1e-5, rtol=1e-5)
