@@ -208,6 +208,19 @@ class PagedKVCache:
             self.block_table[slot, len(have)] = b
             have.append(b)
 
+    def allocate_all(self, slots, num_tokens):
+        """Blocks for num_tokens[i] tokens of each sequence slots[i], and for its next token where the table has room for one;
+        all of them or, with nothing changed, an error."""
+        bs, most = self.block_size, self.max_blocks_per_seq
+        for n in num_tokens:
+            if n > most * bs:
+                raise IndexError(f"PagedKVCache: {n} tokens do not fit {most} blocks per sequence")
+        blocks = [min(n // bs + 1, most) for n in num_tokens]
+        if sum(max(0, k - len(self._owned.get(s, []))) for s, k in zip(slots, blocks)) > len(self._free):
+            raise RuntimeError("PagedKVCache out of blocks")
+        for s, k in zip(slots, blocks):
+            self.allocate(s, k * bs)
+
     def free(self, slot):
         for b in self._owned.pop(slot, []):
             self._drop(b)

@@ -273,20 +273,23 @@ class LlamaGenerator:
         """Append the tokens ``chunks[i]`` to sequence ``slots[i]``, over the ``held[i]`` tokens that the cache holds of it
         already: the next chunk of a prompt, another turn, drafted tokens.  ``held`` is the cache's seq_lens by default,
         which prefill and extend keep and decode_step does not.  All chunks run as one packed token batch; a
-        sequence's first chunk may be its prompt's start.  Returns the last-token logits [len(slots), V]."""
+        sequence's first chunk may be its prompt's start.  Returns the last-token logits [len(slots), V].
+
+        Nothing is changed when a slot is not the cache's, a sequence would outgrow its table (IndexError) or there are too
+        few free pages (RuntimeError)."""
+        slots = [self.cache._slot(int(s)) for s in slots]
         lens = [len(c) for c in chunks]
         if len(lens) != len(slots) or len(set(slots)) < len(lens) or min(lens, default=0) < 1:
             raise ValueError("extend: one non-empty chunk for each slot, every slot once")
         total = sum(lens)
         nh, nkv, d = self.nh, self.nkv, self.d
-        slot_t = torch.tensor(list(slots), dtype=torch.long, device=self.dev)
+        slot_t = torch.tensor(slots, dtype=torch.long, device=self.dev)
         held = self.cache.seq_lens[slot_t].tolist() if held is None else [int(h) for h in held]
         if len(held) != len(lens) or min(held, default=0) < 0:
             raise ValueError(f"extend: held {held} for {len(lens)} slots")
         for s, h in zip(slots, held):
             self.cache.check_writable(s, h)
-        for s, n, h in zip(slots, lens, held):
-            self.cache.allocate(s, h + n + 1)
+        self.cache.allocate_all(slots, [h + n for h, n in zip(held, lens)])
         ids = torch.as_tensor([int(t) for c in chunks for t in c], dtype=torch.long).to(self.dev)
         pos = torch.cat([torch.arange(h, h + n, dtype=torch.int32) for h, n in zip(held, lens)]).to(self.dev)
         tok_batch = torch.cat([torch.full((n,), s, dtype=torch.int32) for s, n in zip(slots, lens)]).to(self.dev)

@@ -306,3 +306,25 @@ def test_block_multihead_attention_several_new_tokens_in_32_bits(dev):
                                                  i32([0, 3, 4]), i32([[0, 1], [2, 3]]), block_size=16)[0]._t.cpu()
 
     torch.testing.assert_close(run(dev), run("cpu"), atol=1e-5, rtol=1e-5)
+
+
+# ============================================================================ extend at the ends of slots and tables
+def test_extend_fills_the_table_and_names_real_slots():
+    m = _llama("cpu")
+    gen = LlamaGenerator(m, max_batch=2, max_seq_len=32, block_size=8, use_graph=False)
+    prompt = [(7 * i + 3) % 500 for i in range(32)]
+    parts = gen.prefill_chunks([0], [prompt], 20)          # all 32 positions of the table
+    assert gen.cache.seq_lens.tolist() == [32, 0] and len(gen.cache._owned[0]) == 4
+    big = LlamaGenerator(m, max_batch=1, max_seq_len=64, block_size=8, use_graph=False)
+    torch.testing.assert_close(parts[0], big.prefill(0, torch.tensor(prompt)), **_near("cpu"))
+    state = ({k: list(v) for k, v in gen.cache._owned.items()}, list(gen.cache._free), gen.cache.block_table.clone())
+    for slots, chunks, held in (([0], [[1]], None), ([1], [[1] * 33], None), ([1], [[1]], [32]), ([-1], [[1]], None),
+                                ([2], [[1]], None), ([1, -1], [[1], [2]], [0, 0])):
+        with pytest.raises(IndexError):
+            gen.extend(slots, chunks, held)
+        assert state[:2] == (gen.cache._owned, gen.cache._free) and torch.equal(state[2], gen.cache.block_table)
+    small = LlamaGenerator(m, max_batch=2, max_seq_len=32, block_size=8, num_blocks=3, use_graph=False)
+    with pytest.raises(RuntimeError):
+        small.extend([0, 1], [[1] * 15, [2] * 9])          # four pages with the next tokens' places
+    assert small.cache.num_free_blocks == 3 and not any(small.cache._owned.values())
+    small.extend([0, 1], [[1] * 15, [2] * 7])
