@@ -6,6 +6,7 @@ same definitions run in PyTorch.  Inference only: nothing here records a gradien
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -222,6 +223,23 @@ def _chunk_reference(q, kc, vc, cu, lens, table, tok, scale, out):
         out[q0:q0 + n] = torch.where(z == 0, 0.0, o / z).reshape(n, Hq, D).to(out.dtype)
 
 
+def _check_pages(src, dst, blocks):
+    """What the native library checks, for a host without it."""
+    for t in (src, dst):
+        if torch.is_tensor(t) or isinstance(t, str):
+            raise TypeError(f"copy_kv_blocks: page numbers in a {type(t).__name__} (a sequence of integers)")
+    src, dst = [operator.index(i) for i in src], [operator.index(i) for i in dst]
+    if len(src) != len(dst):
+        raise ValueError("src and dst differ in length")
+    for i in src + dst:
+        if not 0 <= i < blocks:
+            raise ValueError(f"page {i} is not in the pool")
+    if len(set(dst)) < len(dst):
+        raise ValueError("a page is a destination twice")
+    if set(src) & set(dst):
+        raise ValueError("a page is both a source and a destination")
+
+
 class KVBlockCopier:
     """Copies pages inside the K and V pools of all layers in one launch.
 
@@ -248,23 +266,15 @@ class KVBlockCopier:
             self._ptrs, self._copy = [t.data_ptr() for t in pools], N.native().kv_copy
 
     def copy(self, src, dst):
-        """Page src[i] -> page dst[i] in every pool, on the current stream.  ``src`` / ``dst``: host integers.  A page may be
-        a source many times, a destination once, and never both; ValueError otherwise, with nothing copied."""
+        """Page src[i] -> page dst[i] in every pool, on the current stream.  ``src`` / ``dst``: sequences of host integers
+        (TypeError for others).  A page may be a source many times, a destination once, and never both; ValueError otherwise,
+        with nothing copied."""
         if self._native:
             _launch(self._dev, self._copy, self._ptrs, src, dst, self._blocks, self._bytes, self._stride)
             return
-        src, dst = [int(i) for i in src], [int(i) for i in dst]
-        if len(src) != len(dst):
-            raise ValueError("src and dst differ in length")
-        for i in src + dst:
-            if not 0 <= i < self._blocks:
-                raise ValueError(f"page {i} is not in the pool")
-        if len(set(dst)) < len(dst):
-            raise ValueError("a page is a destination twice")
-        if set(src) & set(dst):
-            raise ValueError("a page is both a source and a destination")
-        if src:
-            s, d = (torch.tensor(i, device=self._dev) for i in (src, dst))
+        (_check_pages if N.native() is None else N.native().kv_copy_check)(src, dst, self._blocks)
+        if len(src):
+            s, d = (torch.tensor(list(i), device=self._dev) for i in (src, dst))
             with torch.no_grad():
                 for t in self.pools:
                     t[d] = t[s]

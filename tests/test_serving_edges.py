@@ -328,3 +328,29 @@ def test_extend_fills_the_table_and_names_real_slots():
         small.extend([0, 1], [[1] * 15, [2] * 9])          # four pages with the next tokens' places
     assert small.cache.num_free_blocks == 3 and not any(small.cache._owned.values())
     small.extend([0, 1], [[1] * 15, [2] * 7])
+
+
+# ============================================================================ page copies
+@pytest.mark.parametrize("dev", ["cpu", "cpu without the library", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_copies_take_the_same_page_numbers_everywhere(dev, monkeypatch):
+    """Host integers in a sequence; tensors, fractions and text are a TypeError, pages that are wrong a ValueError."""
+    import numpy as np
+
+    from paddle2_amd.serving import paged
+
+    if dev == "cpu without the library":
+        monkeypatch.setattr(paged.N, "native", lambda: None)
+    start = torch.arange(6.0).reshape(6, 1).to(dev[:4].strip())
+    pool = start.clone()
+    c = serving.KVBlockCopier([pool], [])
+    for src, dst in ((torch.tensor([0]), torch.tensor([1])), ([0.0], [1.0]), ([0.5], [1]), ("0", "1"), ([0], None)):
+        with pytest.raises(TypeError):
+            c.copy(src, dst)
+    for src, dst in (([0], [6]), ([-1], [2]), ([2 ** 40], [2]), ([0, 1], [2, 2]), ([0, 1], [1, 2]), ([3], [3]), ([0, 1], [2])):
+        with pytest.raises(ValueError):
+            c.copy(src, dst)
+    assert torch.equal(pool, start)
+    for src, dst in ((range(1, 3), (3, 4)), (np.array([1, 2]), np.array([3, 4])), ([np.int64(1), 2], range(3, 5))):
+        pool.copy_(start)
+        c.copy(src, dst)
+        assert pool.flatten().tolist() == [0, 1, 2, 1, 2, 5]
