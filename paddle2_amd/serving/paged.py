@@ -244,10 +244,17 @@ class KVBlockCopier:
     """Copies pages inside the K and V pools of all layers in one launch.
 
     ``k_caches`` / ``v_caches``: one tensor per layer, [num_blocks, ...], all of one shape, type, device and stride, each
-    page contiguous.  The pools are checked once here and kept; ``copy`` may then be called as often as wanted."""
+    page contiguous.  The pools are checked once here and kept; ``copy`` may then be called as often as wanted, and checks
+    them again when one's memory has been replaced."""
 
     def __init__(self, k_caches, v_caches):
-        pools = [_u(t) for t in (list(k_caches) + list(v_caches))]
+        self._given = list(k_caches) + list(v_caches)
+        self._wrapped = any(isinstance(t, Tensor) for t in self._given)
+        self.pools = [_u(t) for t in self._given]
+        self._check()
+
+    def _check(self):
+        pools = self.pools
         if not pools:
             raise ValueError("copy_kv_blocks: no caches")
         a = pools[0]
@@ -256,21 +263,26 @@ class KVBlockCopier:
         for t in pools:
             if t.shape != a.shape or t.dtype != a.dtype or t.device != a.device or t.stride() != a.stride():
                 raise ValueError("copy_kv_blocks: the caches differ in shape, type, device or stride")
-        self.pools = pools
         self._dev = a.device
         self._blocks = a.shape[0]
         self._bytes = (a.numel() // max(a.shape[0], 1)) * a.element_size()
         self._stride = a.stride(0) * a.element_size()
         self._native = self._dev.type == "cuda" and N.use_native(a)
-        if self._native:
-            self._ptrs, self._copy = [t.data_ptr() for t in pools], N.native().kv_copy
+        self._ptrs = [t.data_ptr() for t in pools]
 
     def copy(self, src, dst):
         """Page src[i] -> page dst[i] in every pool, on the current stream.  ``src`` / ``dst``: sequences of host integers
         (TypeError for others).  A page may be a source many times, a destination once, and never both; ValueError otherwise,
         with nothing copied."""
+        if self._wrapped:
+            self.pools = [_u(t) for t in self._given]
+        if [t.data_ptr() for t in self.pools] != self._ptrs:
+            self._check()
+        self._checked_copy(src, dst)
+
+    def _checked_copy(self, src, dst):
         if self._native:
-            _launch(self._dev, self._copy, self._ptrs, src, dst, self._blocks, self._bytes, self._stride)
+            _launch(self._dev, N.native().kv_copy, self._ptrs, src, dst, self._blocks, self._bytes, self._stride)
             return
         (_check_pages if N.native() is None else N.native().kv_copy_check)(src, dst, self._blocks)
         if len(src):
@@ -283,4 +295,4 @@ class KVBlockCopier:
 def copy_kv_blocks(k_caches, v_caches, src, dst):
     """``KVBlockCopier(k_caches, v_caches).copy(src, dst)``: page src[i] of every layer's K and V pool -> page dst[i].  A
     program that copies often keeps the copier (PagedKVCache.copy_blocks does)."""
-    KVBlockCopier(k_caches, v_caches).copy(src, dst)
+    KVBlockCopier(k_caches, v_caches)._checked_copy(src, dst)

@@ -354,3 +354,25 @@ def test_copies_take_the_same_page_numbers_everywhere(dev, monkeypatch):
         pool.copy_(start)
         c.copy(src, dst)
         assert pool.flatten().tolist() == [0, 1, 2, 1, 2, 5]
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_copier_follows_its_pools(dev):
+    """Pools whose memory was replaced after the copier was made are copied where they lie now, and checked again."""
+    mk = lambda n=6: torch.arange(float(n), device=dev).reshape(n, 1).repeat(1, 8)  # noqa: E731
+    k, v, w = mk(), mk(), paddle.Tensor._wrap(mk())
+    c = serving.KVBlockCopier([k, v], [w])
+    old = [k.data, v.data, w._t]
+    k.data, v.data, w._t = mk(9) + 10, mk(9) + 20, mk(9) + 30
+    c.copy([8, 0], [3, 4])
+    for t, a in ((k, 10), (v, 20), (w._t, 30)):
+        assert t[:, 0].tolist() == [a, a + 1, a + 2, a + 8, a, a + 5, a + 6, a + 7, a + 8]
+    assert all(torch.equal(t, mk()) for t in old)
+    v.data = mk(4)
+    with pytest.raises(ValueError):           # of another shape than the others
+        c.copy([0], [1])
+    k.data, w._t = mk(4), mk(4)
+    with pytest.raises(ValueError):           # page 5 is not there any more
+        c.copy([0], [5])
+    c.copy([3], [0])
+    assert k[:, 0].tolist() == v[:, 0].tolist() == w._t[:, 0].tolist() == [3, 1, 2, 3]
