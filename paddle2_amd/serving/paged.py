@@ -49,6 +49,8 @@ def _ints(t, name, rows, cols, dev):
     shape = t.shape
     if len(shape) != (2 if cols else 1) or (rows is not None and shape[0] != rows):
         raise ValueError(f"chunk_attention: {name} has shape {tuple(shape)}, expected ({rows or 'B'}{', pages' if cols else ''})")
+    if t.dtype is torch.int64:   # (what does not fit 32 bits stays as far out as it can)
+        t = t.clamp(-2**31, 2**31 - 1)
     return t if t.dtype is torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
 
 

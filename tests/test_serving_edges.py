@@ -376,3 +376,23 @@ def test_copier_follows_its_pools(dev):
         c.copy([0], [5])
     c.copy([3], [0])
     assert k[:, 0].tolist() == v[:, 0].tolist() == w._t[:, 0].tolist() == [3, 1, 2, 3]
+
+
+# ============================================================================ chunk attention: numbers past 32 bits
+@pytest.mark.parametrize("dev", DEVS)
+def test_chunk_attention_takes_64_bit_numbers_as_they_are(dev):
+    """Lengths and page numbers past 2^31 are cut to the table and outside the pool; they do not wrap."""
+    g = torch.Generator().manual_seed(4)
+    dt = torch.float32 if dev == "cpu" else torch.bfloat16
+    q = torch.randn(5, 4, 64, generator=g).to(dev, dt)
+    kc, vc = (torch.randn(4, 16, 2, 64, generator=g).to(dev, dt) for _ in range(2))
+    cu = torch.tensor([0, 2, 5], device=dev)
+    table = torch.tensor([[1, 2 ** 32 + 3], [0, 2]], device=dev)
+    lens = torch.tensor([30, 2 ** 32 + 7], device=dev)
+    got = serving.chunk_attention(q, kc, vc, cu, lens, table)
+    same = serving.chunk_attention(q, kc, vc, cu, torch.tensor([30, 32], device=dev), torch.tensor([[1, -1], [0, 2]], device=dev))
+    assert torch.equal(got, same)
+    far = serving.chunk_attention(q, kc, vc, torch.tensor([0, 2, 2 ** 32 + 5], device=dev), lens.clamp(max=32), table)
+    assert torch.equal(far, same)
+    none = serving.chunk_attention(q, kc, vc, cu, torch.tensor([-2 ** 40, 32], device=dev), table)
+    assert (none[:2] == 0).all() and torch.equal(none[2:], same[2:])
