@@ -391,7 +391,8 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
     """Ragged batch over a paged cache [blocks, nh, block_size, hd]: sequences with
     seq_lens_encoder > 0 run causal prefill (flash kernel) and fill the cache; the others append
     seq_lens_this_time tokens behind their seq_lens_decoder cached ones: decode attention for one token,
-    chunk attention for several.  Returns (out [token_num, nh*hd], qkv, key_cache, value_cache)."""
+    chunk attention for several, causal among themselves (NotImplementedError with a ``tgt_mask`` or a
+    ``pre_key_cache``).  Returns (out [token_num, nh*hd], qkv, key_cache, value_cache)."""
     t = _u(qkv)
     if qkv_bias is not None:
         t = t + _u(qkv_bias).reshape(1, -1)
@@ -404,6 +405,8 @@ def block_multihead_attention(qkv, key_cache, value_cache, seq_lens_encoder, seq
     now = _u(seq_lens_this_time).reshape(-1).tolist()
     cu = _u(cu_seqlens_q).reshape(-1).tolist()
     bt = _u(block_tables)
+    if (tgt_mask is not None or pre_key_cache is not None) and any(n > 1 and e == 0 for n, e in zip(now, enc)):
+        raise NotImplementedError("block_multihead_attention: tgt_mask or pre_key_cache with several new tokens over a cache")
     qkv3 = t.reshape(tok, Hq + 2 * Hk, D)
     out = torch.empty(tok, Hq, D, dtype=t.dtype, device=t.device)
     cos = sin = None

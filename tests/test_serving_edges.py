@@ -396,3 +396,25 @@ def test_chunk_attention_takes_64_bit_numbers_as_they_are(dev):
     assert torch.equal(far, same)
     none = serving.chunk_attention(q, kc, vc, cu, torch.tensor([-2 ** 40, 32], device=dev), table)
     assert (none[:2] == 0).all() and torch.equal(none[2:], same[2:])
+
+
+def test_block_multihead_attention_refuses_masks_over_several_new_tokens():
+    """Several new tokens over a cache are attended causally: a mask of their own, or a prefix cache, is not passed over in
+    silence, and nothing has been written."""
+    g = torch.Generator().manual_seed(2)
+    W = paddle.Tensor._wrap
+    kc, vc = (torch.randn(6, 2, 16, 32, generator=g) for _ in range(2))
+    before = kc.clone(), vc.clone()
+    i32 = lambda v: W(torch.tensor(v, dtype=torch.int32))  # noqa: E731
+
+    def run(now, **kw):
+        cu = [0, now[0], sum(now)]
+        qkv = torch.randn(sum(now), 8 * 32, generator=g)
+        return serving.block_multihead_attention(W(qkv), W(kc), W(vc), i32([0, 0]), i32([20, 7]), i32(now), None, None,
+                                                 i32(cu), i32(cu), i32([[0, 1], [2, 3]]), block_size=16, **kw)
+
+    for kw in (dict(tgt_mask=W(torch.zeros(2, 1, 3, 32))), dict(pre_key_cache=W(torch.zeros(2, 2, 4, 32)))):
+        with pytest.raises(NotImplementedError):
+            run([1, 3], **kw)
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+    run([3, 1], mask=W(torch.zeros(1)))         # (the prompts' mask: there is no prompt)
