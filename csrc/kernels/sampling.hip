@@ -17,7 +17,7 @@
 //                  groups and 512) is done here alone: the k-th best group's largest logit bounds the k-th best logit from
 //                  below, so some k groups are read, and the few logits above the bound are ranked all against all.
 // Rows that fit none of this (a larger k, an infinite logit, a border in the tail or with more than 8,192 logits in its
-// bin, a number below 2^-40) are taken from the start in choose_kernel: radix selection on the ordered bits of the logits.
+// bin, a number below 2^-40 or from 1 on) are taken from the start in choose_kernel: radix selection on the ordered bits of the logits.
 //
 // Measured: 256 rows of 131,072 bf16 logits with settings of their own 102 us (peaks 15, 4.6 TB/s; bins 38 and sweep 39, bound
 // by some 25 double-precision operations a logit, bins by an LDS atomic each too; choose 26, bound by latency); 32 of
@@ -209,7 +209,7 @@ enum Kind { kGreedy, kPlain, kTopP, kShortK, kFromStart };
 template <typename T>
 __device__ __forceinline__ Kind kind_of(const Args<T>& a, const Of& r, float top) {
   if (!(r.t > 0.f) || top == -INFINITY) return kGreedy;
-  if (top == INFINITY || !(r.u >= 9.094947e-13f)) return kFromStart;   // 2^-40
+  if (top == INFINITY || !(r.u >= 9.094947e-13f) || r.u >= 1.f) return kFromStart;   // 2^-40
   if (r.k) return r.k <= a.groups / 2 && r.k <= kMaxK ? kShortK : kFromStart;
   return r.p < 1.f ? kTopP : kPlain;
 }
@@ -674,15 +674,16 @@ __device__ __forceinline__ void choose_from_start(const Args<T>& a, const Of& of
     __syncthreads();
   }
   // ---- kept mass per chunk, then the chunk, lane and element where the cumulative mass passes u * total
-  // A number below 2^-40 draws the first kept token of any weight above 0, also one that is below the integers' unit.
+  // A number below 2^-40 draws the first kept token of any weight above 0, one from 1 on the last, also where that is below
+  // the integers' unit: they are counted.
   const float mp = of.m, uf = of.u;
-  const bool first_kept = !(uf >= 9.094947e-13f);
+  const bool last_kept = uf >= 1.f, counted = last_kept || !(uf >= 9.094947e-13f);
   auto kept = [&](float x, int i) -> u64 {
     const unsigned ky = key_of(x);
     if (i >= V || ky < kmin || (ky == kmin && i > last_tie)) return 0;
     const double w = weight(r, x);
     if (!(w >= (double)mp || x == r.top || !(mp == mp))) return 0;
-    return first_kept ? (u64)(w > 0.0) : fixed(r, w);
+    return counted ? (u64)(w > 0.0) : fixed(r, w);
   };
   u64 mine = 0;
   for (int c = wv; c < chunks; c += kWaves) {
@@ -697,8 +698,8 @@ __device__ __forceinline__ void choose_from_start(const Args<T>& a, const Of& of
     mine += lane == 0 ? s : 0;
   }
   const u64 total = group_sum<kWaves>(mine, red);
-  u64 want = first_kept ? 0 : (u64)fmin((double)uf * (double)total, 9.0e18);
-  if (want >= total) want = total - 1;
+  u64 want = counted ? 0 : (u64)fmin((double)uf * (double)total, 9.0e18);
+  if (last_kept || want >= total) want = total - 1;
   group_find<kWaves, kMaxChunks / 64 / kWaves>(part, chunks, red, found, [&](u64) { return want; });
   if (wv == 0) {
     const int at = (int)found[0];

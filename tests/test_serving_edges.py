@@ -418,3 +418,24 @@ def test_block_multihead_attention_refuses_masks_over_several_new_tokens():
             run([1, 3], **kw)
     assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
     run([3, 1], mask=W(torch.zeros(1)))         # (the prompts' mask: there is no prompt)
+
+
+# ============================================================================ sampling at the ends of its ranges
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("V", [2, 700, 40000])
+def test_numbers_at_or_above_one_draw_the_last_kept_token(dev, V):
+    """Also where it weighs next to nothing."""
+    x = torch.zeros(6, V)
+    x[:, 1:] = -300.0
+    x[:, V - 1] = -60.0
+    x[1, V - 1] = float("-inf")
+    x[2] = float("-inf")
+    x[2, 0] = 3.0
+    u = torch.tensor([1.0, 1.0, 1.0, float("inf"), 7.0, 1.0])
+    last = [V - 1, V - 2, 0, V - 1, V - 1, V - 1]
+    assert serving.sample_tokens(x.to(dev), u.to(dev)).tolist() == last
+    assert serving.sample_tokens(x.to(dev), u.to(dev), top_k=1).tolist() == [0] * 6
+    second = [V - 1, 1 if V > 2 else 0, 0, V - 1, V - 1, V - 1]
+    assert serving.sample_tokens(x.to(dev), u.to(dev), top_k=2).tolist() == second
+    assert serving.sample_tokens(x.to(dev), u.to(dev), min_p=1e-20).tolist() == [0] * 6
+    assert serving.sample_tokens(x.to(dev), u.to(dev), top_p=0.9).tolist() == [0] * 6
