@@ -255,10 +255,10 @@ struct Weigher {
     return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;   // w <= 2^50: rounded to an integer
   }
   // bin of a logit, not decreasing as x falls; the last one holds all the rest.  wide_bin: twice as wide, so that the
-  // last one weighs nothing (2^-64)
+  // last one weighs nothing (2^-64); halves, whose difference does not pass the largest number
   __device__ __forceinline__ int bin(float x) const { return (int)fminf((top - x) * bin_scale, (float)(kBins - 1)); }
   __device__ __forceinline__ int wide_bin(float x) const {
-    return (int)fminf((top - x) * bin_scale * 0.5f, (float)(kBins - 1));
+    return (int)fminf((0.5f * top - 0.5f * x) * bin_scale, (float)(kBins - 1));
   }
 };
 __device__ __forceinline__ Weigher weigher(float top, float t, int shift) {

@@ -439,3 +439,22 @@ def test_numbers_at_or_above_one_draw_the_last_kept_token(dev, V):
     assert serving.sample_tokens(x.to(dev), u.to(dev), top_k=2).tolist() == second
     assert serving.sample_tokens(x.to(dev), u.to(dev), min_p=1e-20).tolist() == [0] * 6
     assert serving.sample_tokens(x.to(dev), u.to(dev), top_p=0.9).tolist() == [0] * 6
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("t", [1e37, 1e38, 3e38, float("inf")])
+def test_top_k_over_the_whole_range_of_32_bits_gpu(t):
+    """Logits whose distance passes the largest number of 32 bits, at temperatures where both still weigh: as on the CPU."""
+    g = torch.Generator().manual_seed(8)
+    x = torch.full((64, 3000), -3.4e38)
+    x[:, 5::7] = float("-inf")
+    for i in (40, 1700, 2999):
+        x[:, i] = 3.4e38 * torch.rand(64, generator=g)
+    x[:, 2222] = 3.4e38
+    u = torch.rand(64, generator=g)
+    tt = torch.full((64,), t)
+    for k in (2, 5, 40):
+        for p in (1.0, 0.99):
+            want = serving.sample_tokens(x, u, temperature=tt, top_k=k, top_p=p)
+            got = serving.sample_tokens(x.cuda(), u.cuda(), temperature=tt.cuda(), top_k=k, top_p=p)
+            assert torch.equal(got.cpu(), want), (k, p)
