@@ -43,6 +43,10 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kDefer = 8.f;   // the running maximum moves only when a row outgrows it by 2^8
+// Weights are exp2(s - m + lift): float16 ends at 2^16, so 2^(8 + 7) fits, and its smallest step, 2^-24, is 2^-31 of the weight
+// at m (without the lift 30,000 keys of 2^-25 each counted as nothing).  bfloat16 has the range of 32 bits.
+template <bool F16>
+constexpr float kLift = F16 ? 7.f : 0.f;
 constexpr int kBM = 128, kBN = 64;
 
 __device__ const u16x8 kZeros[16] = {};   // a row of D = 128
@@ -349,8 +353,8 @@ __device__ __forceinline__ void few_rows(const Args& a, const Seq& s, int hk, in
       }
     mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
     mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-    const float mn = fmaxf(m, mt), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - base);
+    const float mn = fmaxf(m, mt), top = mn == -INFINITY ? 0.f : mn, base = top - kLift<F16>;
+    const float alpha = __builtin_amdgcn_exp2f(m - top);
     m = mn;
     bf16x8 pf;
     float ps = 0.f;
@@ -781,7 +785,7 @@ __global__ __launch_bounds__(256 * KG, KG == 2 ? 1 : 2) void chunk_kernel(Args a
     asm volatile("" : "+v"(o_k), "+v"(o_va), "+v"(o_vb));   // the XORs stay in the loop: hoisted they spilled
     if constexpr (!UNI) stage_begin(n0);
     const int next = o_k + (buf ? -TILE : TILE);
-    const float base = m == -INFINITY ? 0.f : m;
+    const float base = (m == -INFINITY ? 0.f : m) - kLift<F16>;
     float ls[4] = {0.f, 0.f, 0.f, 0.f};
     auto weight = [&](int i) {    // of the lane's score i
       float p = __builtin_amdgcn_exp2f(fmaf(cur[i >> 4][i & 15], sl2, -base));

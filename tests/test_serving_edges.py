@@ -458,3 +458,34 @@ def test_top_k_over_the_whole_range_of_32_bits_gpu(t):
             want = serving.sample_tokens(x, u, temperature=tt, top_k=k, top_p=p)
             got = serving.sample_tokens(x.cuda(), u.cuda(), temperature=tt.cuda(), top_k=k, top_p=p)
             assert torch.equal(got.cpu(), want), (k, p)
+
+
+# ============================================================================ chunk attention: weights below 16 bits' range
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("new", [1, 300])
+def test_chunk_attention_small_weights_in_16_bits_gpu(new, D, monkeypatch):
+    """Two keys far above 30,000 others, whose weights of 2^-25 each are nothing in float16 but 5e-4 of the sum together, over
+    values 40 times as large, with the keys in one piece: the sum has them.  Tolerance: half a step for the output and for
+    every weight; below float16's normal range, which the lift puts at 2^-21 of the largest weight, half of its smallest step,
+    2^-25 / 2^7, for each key; scores are one product of 17, so 32 bits move a weight by 2^-18 at most."""
+    from paddle2_amd.serving import paged
+
+    monkeypatch.setattr(paged, "_CHUNK_WGS", 1)
+    held, Hk = 30000, 4
+    L = held + new
+    pages = -(-L // 64)
+    kc, vc = torch.zeros(pages, 64, Hk, D), torch.full((pages, 64, Hk, D), 40.0)
+    for where in (7, L // 2):
+        kc[where // 64, where % 64, :, 0] = 17.328125
+        vc[where // 64, where % 64] = 1.0
+    q = torch.zeros(new, 2 * Hk, D)
+    q[..., 0] = 1.0
+    n = held + 1 + torch.arange(new, dtype=torch.float64)[:, None, None]
+    w = torch.tensor(17.328125, dtype=torch.float64).exp()
+    want = (2 * w + 40 * (n - 2)) / (2 * w + n - 2)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    out = serving.chunk_attention(q.cuda().half(), kc.cuda().half(), vc.cuda().half(), i32([0, new]), i32([L]),
+                                  i32([list(range(pages))]), scale=1.0)
+    tol = 1.01 * 2.0 ** -11 * 2 * want + 40 * n * 2.0 ** -32 / 2 + 2.0 ** -18 * want
+    assert ((out.double().cpu() - want).abs() <= tol).all(), ((out.double().cpu() - want).abs() / tol).max()
