@@ -81,7 +81,7 @@ int pd_chunk_attn(int, const void*, long, long, const void*, const void*, long, 
 int pd_kv_copy(const uint64_t*, int, const int*, const int*, int, long, long, void*);
 int pd_sample(int, const void*, long, int, int, const float*, const float*, float, const int*, int, const float*, float,
               const float*, float, int64_t*, void*, void*);
-long pd_sample_workspace(int, int);
+long pd_sample_workspace(int, int, int, float, int, int, int, float);
 long pd_bn_workspace(int, long, int);
 int pd_wo_splits(int, int, int, int);
 int pd_dec_splits(int, int, int);
@@ -406,7 +406,12 @@ PYBIND11_MODULE(_C, m) {
                     P<int64_t*>(out), P<void*>(ws), P<void*>(st)),
           "sample");
   });
-  m.def("sample_workspace", &pd_sample_workspace);
+  m.def("sample_workspace",
+        [](int B, int V, bool temp_rows, float temp, bool k_rows, int top_k, bool p_rows, float top_p) {
+          return pd_sample_workspace(B, V, temp_rows, temp, k_rows, top_k, p_rows, top_p);
+        },
+        py::arg("B"), py::arg("V"), py::arg("temp_rows"), py::arg("temp"), py::arg("k_rows"), py::arg("top_k"),
+        py::arg("p_rows"), py::arg("top_p"));
   m.def("decode_attn", [](uintptr_t q, long sq_b, long sq_h, uintptr_t kc, uintptr_t vc, long s_blk, long s_tok,
                           long s_head, uintptr_t table, int max_blocks, int block_size, uintptr_t seq_lens, int max_len,
                           uintptr_t part_o, uintptr_t part_ml, uintptr_t out, long so_b, long so_h, int B, int Hq,

@@ -178,7 +178,7 @@ struct Args {
   const int* top_ks;
   int top_k;
   u64* mass;       // [B][chunks] kept mass of a chunk (of the bins above the border's)
-  u64* hist;       // [B][kBins] mass per bin; the last: of all the rest
+  u64* hist;       // [B][kBins] mass per bin; the last: of all the rest (null: no row can need it, nor the list)
   u64* list;       // [B][kList] logits of the border's bin: key << 32 | index
   int* listed;     // [B] how many
   float* peaks;    // [B][groups] largest logit of a group
@@ -296,6 +296,7 @@ __global__ __launch_bounds__(256) void peaks_kernel(Args<T> a) {
     const int g = (c * 64 + lane) / a.group_lanes;
     if ((lane & (a.group_lanes - 1)) == a.group_lanes - 1 && g < a.groups) a.peaks[(long)b * a.groups + g] = m;
   });
+  if (!a.hist) return;   // (no row takes top-p alone)
   for (int i = blockIdx.x * 256 + threadIdx.x; i < kBins; i += gridDim.x * 256) a.hist[(long)b * kBins + i] = 0;
   if (blockIdx.x == 0 && threadIdx.x == 0) a.listed[b] = 0;
 }
@@ -1032,10 +1033,23 @@ using namespace pd;
 // logits per group: small ones allow a larger top-k (half the groups), large ones keep the list of their peaks short
 static int sample_group(int V) { return V <= 65536 ? 32 : 128; }
 
-// bytes of scratch for B rows of V logits
-extern "C" long pd_sample_workspace(int B, int V) {
+// What some row may need, of a call's settings: tensors (rows), or numbers
+struct Needs {
+  bool warm, always_k, p;   // a temperature; top-k in every row; top-p alone
+};
+static Needs sample_needs(int V, bool temp_rows, float temp, bool k_rows, int top_k, bool p_rows, float top_p) {
+  Needs n;
+  n.warm = temp_rows || temp > 0.f;
+  n.always_k = !k_rows && top_k > 0 && top_k < V;
+  n.p = n.warm && !n.always_k && (p_rows || top_p < 1.f);
+  return n;
+}
+
+// bytes of scratch for B rows of V logits: 82 KB a row with top-p alone, else a hundredth to a tenth of the logits
+extern "C" long pd_sample_workspace(int B, int V, int temp_rows, float temp, int k_rows, int top_k, int p_rows, float top_p) {
   const long chunks = (V + smp::kChunk - 1) / smp::kChunk, per = sample_group(V), groups = (V + per - 1) / per;
-  return (long)B * (8 * (chunks + smp::kBins + smp::kList) + 4 * (groups + 1));
+  const bool p = sample_needs(V, temp_rows, temp, k_rows, top_k, p_rows, top_p).p;
+  return (long)B * (8 * (chunks + (p ? smp::kBins + smp::kList : 0)) + 4 * (groups + 1));
 }
 
 extern "C" int pd_sample(int dt, const void* logits, long stride, int B, int V, const float* uniform, const float* temps,
@@ -1054,21 +1068,19 @@ extern "C" int pd_sample(int dt, const void* logits, long stride, int B, int V, 
   };
   const dim3 narrow(slices_of(4, 2048), B), wide(slices_of(smp::kWide, 1024), B);
   hipStream_t st = (hipStream_t)stream;
-  smp::u64* const mass = (smp::u64*)workspace;
-  smp::u64* const hist = mass + (long)B * chunks;
-  smp::u64* const list = hist + (long)B * smp::kBins;
-  int* const listed = (int*)(list + (long)B * smp::kList);
-  float* const peaks = (float*)(listed + B);
   // kernels that no row can need are not launched: the settings that are numbers say so
-  const bool maybe_warm = temps || temp > 0.f;
-  const bool maybe_short = top_ks || (top_k > 0 && top_k < V), always_k = !top_ks && maybe_short;
-  const bool maybe_p = maybe_warm && !always_k && (top_ps || top_p < 1.f);
+  const Needs needs = sample_needs(V, temps, temp, top_ks, top_k, top_ps, top_p);
+  smp::u64* const mass = (smp::u64*)workspace;
+  smp::u64* const hist = needs.p ? mass + (long)B * chunks : nullptr;
+  smp::u64* const list = needs.p ? hist + (long)B * smp::kBins : nullptr;
+  int* const listed = (int*)(needs.p ? list + (long)B * smp::kList : mass + (long)B * chunks);
+  float* const peaks = (float*)(listed + B);
   PD_DISPATCH_FLOAT(dt, T, {
     const smp::Args<T> a{(const T*)logits, stride, V, chunks, groups, per / 8, shift, uniform, {temps, temp}, {top_ps, top_p},
                          {min_ps, min_p}, top_ks, top_k, mass, hist, list, listed, peaks, out};
     smp::peaks_kernel<T><<<narrow, 256, 0, st>>>(a);
-    if (maybe_warm && !always_k) smp::bins_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
-    if (maybe_p) smp::sweep_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
+    if (needs.warm && !needs.always_k) smp::bins_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
+    if (needs.p) smp::sweep_kernel<T><<<wide, smp::kWide * 64, 0, st>>>(a);
     if (V <= 65536) smp::choose_kernel<T, 8><<<B, 512, 0, st>>>(a);
     else smp::choose_kernel<T, 16><<<B, 1024, 0, st>>>(a);
   });

@@ -77,7 +77,8 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         if not u.is_contiguous():
             u = u.detach().contiguous()
         n = N.native()
-        ws = torch.empty(n.sample_workspace(B, V), dtype=torch.uint8, device=dev)
+        ws = torch.empty(n.sample_workspace(B, V, t[0] is not None, t[1], k[0] is not None, k[1], p[0] is not None, p[1]),
+                         dtype=torch.uint8, device=dev)
         _launch(dev, n.sample, N.DT_CODE[dt], x.data_ptr(), x.stride(0), B, V, u.data_ptr(), N.ptr(t[0]), t[1], N.ptr(k[0]),
                 k[1], N.ptr(p[0]), p[1], N.ptr(m[0]), m[1], out.data_ptr(), ws.data_ptr())
     else:

@@ -489,3 +489,20 @@ def test_chunk_attention_small_weights_in_16_bits_gpu(new, D, monkeypatch):
                                   i32([list(range(pages))]), scale=1.0)
     tol = 1.01 * 2.0 ** -11 * 2 * want + 40 * n * 2.0 ** -32 / 2 + 2.0 ** -18 * want
     assert ((out.double().cpu() - want).abs() <= tol).all(), ((out.double().cpu() - want).abs() / tol).max()
+
+
+# ============================================================================ scratch of sampling
+def test_sampling_scratch_follows_the_settings():
+    """Bins and the list of a border are for top-p alone; a call that no row can need them in asks for none."""
+    m = serving.sampling.N.native()
+    if m is None:
+        pytest.skip("no library")
+    B, V = 256, 32000
+    off = dict(temp_rows=False, temp=1.0, k_rows=False, top_k=0, p_rows=False, top_p=1.0)
+    size = lambda **kw: m.sample_workspace(B, V, **dict(off, **kw)) / B      # noqa: E731
+    few = 8 * 63 + 4 * 1001            # the chunks' masses and the groups' largest logits
+    for kw in (dict(), dict(temp=0.0), dict(temp=0.0, top_p=0.5), dict(top_k=40, top_p=0.9), dict(k_rows=True)):
+        assert size(**kw) <= few + 8
+    for kw in (dict(top_p=0.9), dict(p_rows=True), dict(k_rows=True, top_p=0.9), dict(top_k=V, top_p=0.9),
+               dict(temp_rows=True, temp=0.0, top_p=0.9)):
+        assert size(**kw) >= few + 8 * (2048 + 8192)
