@@ -16,7 +16,8 @@ from ..ops import _native as N
 _HEAD_DIMS = (64, 128)
 _CHUNK_WGS = 512        # workgroups that fit the chip at once
 _CHUNK_MIN_KEYS = 256   # keys of a piece at least (128: the join costs more than the shorter pieces give)
-_FEW_ROWS = 16          # rows (query heads of a kv head times new tokens) per sequence up to which they are few, on average
+_FEW_ROWS = 16          # rows (query heads of a kv head times new tokens) per sequence up to which they are few, on average;
+                        # 8 times as many (128, a tile of many) in the longest there can be
 _PAIR_TILES = 256       # tiles up to which two groups of waves share one (the CUs),
 _PAIR_ROWS = 64         # if of 128 rows: where the sequences have that many, on average
 _MAX_KEYS = 2**31 - 2**14   # positions are 32-bit, and a tile's loads reach past its last key
@@ -173,7 +174,11 @@ def _chunk_plan(T, B, G, Hk, capacity):
     # over many sequences: up to four rounds of smaller ones instead, since the lengths differ (64 x 8,000: 318 -> 295 us);
     # many rows are left whole, their pieces' O costs more than it evens out.
     longest = min(capacity // _CHUNK_MIN_KEYS, 64)
-    if G <= 16 and T * G <= _FEW_ROWS * B:
+    # Few rows in every sequence, as far as the host can see: on average, and where all others bring one token the longest has
+    # no more than a tile of many.  255 single tokens and a piece of 2,000, 32 heads, over 1,000 - 2,000: 1,990 us by tiles of
+    # 16 and 1,190 with tiles of 128 beside them, 31 and one of 300: 429 and 325; the other way 32 x 2 tokens, 8 heads on 1,
+    # over 2,000 - 4,000: 20 and 23, 32 x 4, 32 on 8: 90 and 93, 64 x 4: 184 and 170.
+    if G <= 16 and T * G <= _FEW_ROWS * B and (T - B + 1) * G <= 8 * _FEW_ROWS:
         tiles = max(min(B, T), -(-T // (16 // G))) * Hk
         # No more tiles than CUs, but work for all: one workgroup of eight waves a CU, half as many pieces to join (8 x 4
         # tokens over 350 - 700, 32 heads: 18.9 us, with four waves 21.6; 1 over 16,000, 32 heads on 8: 24.8 and 31.6; the

@@ -506,3 +506,16 @@ def test_sampling_scratch_follows_the_settings():
     for kw in (dict(top_p=0.9), dict(p_rows=True), dict(k_rows=True, top_p=0.9), dict(top_k=V, top_p=0.9),
                dict(temp_rows=True, temp=0.0, top_p=0.9)):
         assert size(**kw) >= few + 8 * (2048 + 8192)
+
+
+# ============================================================================ chunk attention: the choice of the kernel
+def test_few_rows_are_few_for_every_sequence_of_the_batch():
+    """The kernel for few rows alone is taken where no sequence can have more rows than one tile of many, not on average."""
+    from paddle2_amd.serving import paged
+
+    if paged.N.native() is None:
+        pytest.skip("no library")
+    rows = lambda T, B, G: paged._chunk_plan(T, B, G, 8, 32768)[0]  # noqa: E731
+    assert rows(255 + 2000, 256, 1) == 128 and rows(63 + 300, 64, 4) == 128 and rows(7 + 500, 8, 1) == 128
+    for T, B, G in ((1, 1, 1), (64, 64, 8), (256, 256, 16), (32, 8, 1), (32, 8, 4), (16, 1, 1), (3, 64, 4)):
+        assert rows(T, B, G) == 16
