@@ -519,3 +519,36 @@ def test_few_rows_are_few_for_every_sequence_of_the_batch():
     assert rows(255 + 2000, 256, 1) == 128 and rows(63 + 300, 64, 4) == 128 and rows(7 + 500, 8, 1) == 128
     for T, B, G in ((1, 1, 1), (64, 64, 8), (256, 256, 16), (32, 8, 1), (32, 8, 4), (16, 1, 1), (3, 64, 4)):
         assert rows(T, B, G) == 16
+
+
+# ============================================================================ generation over shared pages
+@pytest.mark.parametrize("dev", DEVS)
+def test_forked_generation_is_that_of_single_prompts(dev):
+    """Greedy continuations over shared pages are those over unshared ones, token by token: every step runs all slots, so a
+    row's products do not depend on its neighbours."""
+    m = _llama(dev)
+    prompts = [[1, 5, 9, 3, 11, 4, 8, 2], [7, 2, 8]]
+    gen = LlamaGenerator(m, max_batch=6, max_seq_len=64, block_size=8, use_graph=dev == "cuda")
+    plain = gen.generate(prompts, 9)
+    again = gen.generate(prompts, 9, num_return_sequences=3)
+    assert again == [plain[i // 3] for i in range(6)]
+    assert gen.generate(prompts, 9, sampler="fused") == plain
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_chunked_generation(dev):
+    """Prompts in pieces, then decoding: the logits of each step are those after a whole prefill."""
+    m = _llama(dev)
+    prompts = [[(7 * i + 3) % 500 for i in range(19)], [7, 2, 8]]
+    made = []
+    for chunk in (None, 4):
+        gen = LlamaGenerator(m, max_batch=2, max_seq_len=64, block_size=8, use_graph=dev == "cuda")
+        if chunk:
+            gen.prefill_chunks([0, 1], prompts, chunk)
+        else:
+            gen.prefill_batch([0, 1], prompts)
+        gen.cache.allocate(0, 30), gen.cache.allocate(1, 30)
+        made.append([_decode(gen, [5 + i, 9 + i], [19 + i, 3 + i]).float().clone() for i in range(5)])
+    for a, b in zip(*made):
+        torch.testing.assert_close(a, b, **_near(dev))
+    assert [len(o) for o in gen.generate(prompts, 5, chunk_size=4)] == [5, 5]
