@@ -287,7 +287,9 @@ class LlamaGenerator:
         held = self.cache.seq_lens[slot_t].tolist() if held is None else [int(h) for h in held]
         if len(held) != len(lens) or min(held, default=0) < 0:
             raise ValueError(f"extend: held {held} for {len(lens)} slots")
-        for s, h in zip(slots, held):
+        for s, n, h in zip(slots, lens, held):
+            if h + n > self.cos.shape[0]:
+                raise IndexError(f"extend: {h + n} tokens of slot {s} pass the rotary table of {self.cos.shape[0]} positions")
             self.cache.check_writable(s, h)
         self.cache.allocate_all(slots, [h + n for h, n in zip(held, lens)])
         ids = torch.as_tensor([int(t) for c in chunks for t in c], dtype=torch.long).to(self.dev)

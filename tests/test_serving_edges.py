@@ -552,3 +552,18 @@ def test_chunked_generation(dev):
     for a, b in zip(*made):
         torch.testing.assert_close(a, b, **_near(dev))
     assert [len(o) for o in gen.generate(prompts, 5, chunk_size=4)] == [5, 5]
+
+
+# ============================================================================ calls past a table's or a page's end
+def test_extend_past_the_rotary_table_is_refused():
+    """The last page may reach past the positions that have a rotation: refused, with nothing changed."""
+    gen = LlamaGenerator(_llama("cpu", max_position_embeddings=16), max_batch=1, max_seq_len=20, block_size=16, use_graph=False)
+    assert gen.cos.shape[0] == 20
+    gen.extend([0], [[3] * 18])
+    state = list(gen.cache._owned[0]), list(gen.cache._free), [t.clone() for t in gen.cache.k]
+    for chunk in ([1] * 3, [1] * 14):
+        with pytest.raises(IndexError, match="rotary"):
+            gen.extend([0], [chunk])
+        assert state[:2] == (gen.cache._owned[0], gen.cache._free)
+        assert all(torch.equal(a, b) for a, b in zip(state[2], gen.cache.k))
+    gen.extend([0], [[1, 2]])
