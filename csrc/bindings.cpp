@@ -378,11 +378,12 @@ PYBIND11_MODULE(_C, m) {
                          uintptr_t cu, uintptr_t lens, uintptr_t out, long so_tok, long so_head, int B, int T, int Hq,
                          int Hk, int D, int rows, int groups, int splits, int min_keys, float scale,
                          uintptr_t part_o, uintptr_t part_ml, uintptr_t pieces, uintptr_t st) {
-    check(pd_chunk_attn(f16, P<const void*>(q), sq_tok, sq_head, P<const void*>(k), P<const void*>(v), s_blk, s_tok,
-                        s_head, P<const int*>(table), max_blocks, num_blocks, block, P<const int*>(cu),
-                        P<const int*>(lens), P<void*>(out), so_tok, so_head, B, T, Hq, Hk, D, rows,
-                        groups, splits, min_keys, scale, P<float*>(part_o), P<float*>(part_ml), P<int*>(pieces), P<void*>(st)),
-          "chunk_attn");
+    const int rc = pd_chunk_attn(f16, P<const void*>(q), sq_tok, sq_head, P<const void*>(k), P<const void*>(v), s_blk, s_tok,
+                                 s_head, P<const int*>(table), max_blocks, num_blocks, block, P<const int*>(cu),
+                                 P<const int*>(lens), P<void*>(out), so_tok, so_head, B, T, Hq, Hk, D, rows, groups, splits,
+                                 min_keys, scale, P<float*>(part_o), P<float*>(part_ml), P<int*>(pieces), P<void*>(st));
+    if (rc == -3) throw std::invalid_argument("chunk_attention: a page, or a step between pages, of 2^31 elements or more");
+    check(rc, "chunk_attn");
   });
   // src / dst: page numbers; every page inside the pool, no destination twice, none also a source (std::invalid_argument
   // -> ValueError)

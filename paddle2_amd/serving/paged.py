@@ -69,8 +69,9 @@ def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=Non
     no key (position below 0) gives zeros; a page number outside the pool reads as zeros; lengths past the table are
     cut to it.  Rows past cu_seqlens_q[B] are left as they are in ``out`` and are undefined in a new output.
 
-    bfloat16 and float16 with D 64 or 128 on the GPU, any Hq / Hk up to 128; rows of q, out and the caches must be
-    16-byte aligned.  Returns out [T, Hq, D]."""
+    bfloat16 and float16 with D 64 or 128 on the GPU, any Hq / Hk up to 128; K and V caches of the same strides, a page of
+    less than 2^31 elements, rows of out and the caches 16-byte aligned (ValueError otherwise; queries that are not are
+    copied).  Returns out [T, Hq, D]."""
     wrap = isinstance(q, Tensor)
     q, k_cache, v_cache, out = _u(q), _u(k_cache), _u(v_cache), _u(out)
     dev, dt, qs, ks = q.device, q.dtype, q.shape, k_cache.shape

@@ -567,3 +567,16 @@ def test_extend_past_the_rotary_table_is_refused():
         assert state[:2] == (gen.cache._owned[0], gen.cache._free)
         assert all(torch.equal(a, b) for a, b in zip(state[2], gen.cache.k))
     gen.extend([0], [[1, 2]])
+
+
+def test_pages_past_32_bits_are_a_value_error():
+    """A page of 2^31 elements or more (the library says so before it touches the device)."""
+    from paddle2_amd.serving import paged
+
+    m = paged.N.native()
+    if m is None:
+        pytest.skip("no library")
+    for s_blk, s_tok, s_head in ((2 ** 31, 128, 128), (2 ** 30, 2 ** 27, 128), (2 ** 20, 128, 2 ** 31)):
+        with pytest.raises(ValueError, match="2\\^31"):
+            m.chunk_attn(0, 16, 128, 128, 16, 16, s_blk, s_tok, s_head, 16, 1, 1, 64, 16, 16, 16, 128, 128, 1, 1, 2, 2, 128, 16,
+                         1, 1, 256, 1.0, 0, 0, 0, 0)
