@@ -257,8 +257,8 @@ class KVBlockCopier:
 
     def __init__(self, k_caches, v_caches):
         self._given = list(k_caches) + list(v_caches)
-        self._wrapped = any(isinstance(t, Tensor) for t in self._given)
-        self.pools = [_u(t) for t in self._given]
+        self._wrapped = any(issubclass(c, Tensor) for c in set(map(type, self._given)))
+        self.pools = [_u(t) for t in self._given] if self._wrapped else self._given
         self._check()
 
     def _check(self):
@@ -268,8 +268,9 @@ class KVBlockCopier:
         a = pools[0]
         if a.dim() < 2 or not a[:1].is_contiguous() or (a.shape[0] > 1 and a.stride(0) < a[0].numel()):
             raise ValueError("copy_kv_blocks: the pages of a cache must be contiguous")
+        shape, dtype, device, stride = a.shape, a.dtype, a.device, a.stride()
         for t in pools:
-            if t.shape != a.shape or t.dtype != a.dtype or t.device != a.device or t.stride() != a.stride():
+            if t.shape != shape or t.dtype is not dtype or t.device != device or t.stride() != stride:
                 raise ValueError("copy_kv_blocks: the caches differ in shape, type, device or stride")
         self._dev = a.device
         self._blocks = a.shape[0]
