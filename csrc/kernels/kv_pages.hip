@@ -7,6 +7,8 @@
 //    (1,024 + 2,880 bytes of the 4 KB of arguments), so no table is uploaded and a captured graph owns its plan.
 //  * One workgroup moves 16 KB (4 x 16 bytes a thread, all loads in flight before the first store): a single page of
 //    64 tokens x 32 heads x 128 in 64 pools is 2,048 workgroups.
+// Measured (64 pools, pages of 64 tokens x 32 heads x 128 in bf16, pages that no cache holds): one page 15.6 us, 4.3 TB/s (11.2
+// when the same page is copied again and again, from the last-level cache); four 54.5, 4.9; sixteen 186, 5.8.
 #include "common.h"
 
 namespace pd {

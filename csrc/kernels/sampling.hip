@@ -6,9 +6,11 @@
 //   token = the first index, in index order, whose cumulative kept mass exceeds u * (kept mass).
 //
 // A choice next to a border turns on the last bits of these sums, so weights are computed in 64 bits and summed as
-// integers of 2^-shift (shift = 62 - bits of V): integer sums do not depend on the order they are taken in, so a row's
-// token is the same in every launch.  No sort.  Four launches; a row is cut into chunks of 512 logits (a wave's load)
-// and groups of 32 or 128:
+// integers of 2^-shift, shift = min(50, 62 - bits of V) (50 up to 4,096 tokens, 45 at 131,072, 42 at 2^20): integer sums do
+// not depend on the order they are taken in, so a row's token is the same in every launch.  A weight is off by half a unit
+// and, from its series, by 2e-13 of itself; rows taken from the start use exp instead.  Which way a row goes depends on the
+// row and its settings alone.  No sort.  Four launches; a row is cut into chunks of 512 logits (a wave's load) and groups of
+// 32 or 128:
 //   peaks_kernel   every group's largest logit;
 //   bins_kernel    knows the row's largest.  Without top-k and top-p: the kept mass of every chunk.  Top-p alone: masses
 //                  over 2,047 bins of 1/64 in log2 of the weight, and of the tail behind them;
@@ -17,14 +19,17 @@
 //                  groups and 512) is done here alone: the k-th best group's largest logit bounds the k-th best logit from
 //                  below, so some k groups are read, and the few logits above the bound are ranked all against all.
 // Rows that fit none of this (a larger k, an infinite logit, a border in the tail or with more than 8,192 logits in its
-// bin, a number below 2^-40 or from 1 on) are taken from the start in choose_kernel: radix selection on the ordered bits of the logits.
+// bin, a number below 2^-40 or from 1 on) are taken from the start in choose_kernel: radix selection on the ordered bits of
+// the logits.
 //
-// Measured: 256 rows of 131,072 bf16 logits with settings of their own 102 us (peaks 15, 4.6 TB/s; bins 38 and sweep 39, bound
-// by some 25 double-precision operations a logit, bins by an LDS atomic each too; choose 26, bound by latency); 32 of
-// 50,257 fp32 with top-k and top-p 13 (two launches); 64 of 32,000 fp16 with min-p 15 (three); one of 32,000 with top-p 25
-// (four, 3 - 9 each).  Min-p alone skips the weights of logits below its floor: 256 x 131,072 with a deviation of 0.7, 1.5
-// and 2.5 take 61, 55 and 41 us, without that 59, 60 and 49.  choose_kernel with its arguments in registers alone, one
-// inlined call of the rare path, is 4 - 9 us shorter than with that path as a function.
+// Measured: 256 rows of 131,072 bf16 logits with settings of their own 99 - 107 us (peaks 15, 4.6 TB/s; bins 39 and sweep 42:
+// 45 % of the rows have work there, whose slices lie unevenly on the CUs, busy 55 - 65 % of the time, and vector instructions
+// fill two thirds of a busy one's issue slots; choose 26, bound by latency); 32 of 50,257 fp32 with top-k and top-p 13 (two
+// launches); 64 of 32,000 fp16 with min-p 15 (three); one of 32,000 with top-p 23 - 28 (four, 3 - 9 each).  From the start: 32
+// rows of 32,000 with k = 513 67 us (k = 500: 41), 256 such rows 80, 32 of 131,072 158, all logits equal 151 - 173.  Min-p alone
+// skips the weights of logits below its floor: 256 x 131,072 with a deviation of 0.7, 1.5 and 2.5 take 61, 55 and 41 us,
+// without that 59, 60 and 49.  choose_kernel with its arguments in registers alone, one inlined call of the rare path, is
+// 4 - 9 us shorter than with that path as a function.
 #include "common.h"
 
 namespace pd {

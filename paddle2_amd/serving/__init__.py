@@ -269,9 +269,10 @@ class PagedKVCache:
 
     def fork(self, slot, new_slots, num_tokens=None):
         """Sequences ``new_slots`` (free ones) become copies of the first ``num_tokens`` tokens of ``slot`` (default: its
-        seq_lens).  Full pages are shared; the page of position ``num_tokens``, where the next token goes, is each one's own
-        (a copy where tokens stand in it, and none where the table ends or ``slot`` holds no page), so all of them may grow
-        on their own.  RuntimeError, with nothing changed, when there are too few free pages."""
+        seq_lens, which prefill and extend keep and decode_step does not: after decoding, say how many).  Full pages are
+        shared; the page of position ``num_tokens``, where the next token goes, is each one's own (a copy where tokens stand
+        in it, and none where the table ends or ``slot`` holds no page), so all of them may grow on their own.
+        RuntimeError, with nothing changed, when there are too few free pages."""
         new_slots = [self._slot(int(s)) for s in new_slots]
         have = self._owned.get(self._slot(slot), [])
         n = int(self.seq_lens[slot]) if num_tokens is None else int(num_tokens)

@@ -69,6 +69,10 @@ def chunk_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table=Non
     no key (position below 0) gives zeros; a page number outside the pool reads as zeros; lengths past the table are
     cut to it.  Rows past cu_seqlens_q[B] are left as they are in ``out`` and are undefined in a new output.
 
+    With one token for every sequence it computes what decode_attention does (which takes other types too, by torch): in
+    0.35 - 1.0 of its time where query heads share keys or there is one sequence, in 1.0 - 1.25 of it for 8 and more sequences
+    of thousands of tokens with as many kv heads as query heads.
+
     bfloat16 and float16 with D 64 or 128 on the GPU, any Hq / Hk up to 128; K and V caches of the same strides, a page of
     less than 2^31 elements, rows of out and the caches 16-byte aligned (ValueError otherwise; queries that are not are
     copied).  Returns out [T, Hq, D]."""
@@ -191,8 +195,9 @@ def _chunk_plan(T, B, G, Hk, capacity):
     tiles = max(min(B, T), -(-T // (128 // G))) * Hk
     # No more tiles than CUs, parts of tiles at the sequences' ends counted: two groups of waves per tile, whose halves of
     # the keys are joined through LDS (700 tokens, 32 heads: 20 us, with one 29; 1,000 over 3,000, 32 heads on 8: 74 and 78;
-    # 128 over 16,000, 16 on 4: 36 and 40; the other way 2 x 2,000 over 10,000, 8 on 1: 183 and 176).  With 512 tiles it is
-    # 65 and 57, with 64 rows per sequence no difference.
+    # 128 over 16,000, 16 on 4: 36 and 40; the other way 2 x 2,000 over 10,000, 8 on 1: 183 and 176).  With 512 tiles 2,048
+    # tokens with nothing cached take 53.8 and 55.9, but 4 x 500 tokens 57 and 51, 4,096 tokens 169 and 152.  With 64 rows per
+    # sequence no difference.
     most = N.native().chunk_attn_tiles(T, B, G, 128) * Hk
     groups = 2 if most <= _PAIR_TILES and T * G >= _PAIR_ROWS * B else 1
     return 128, groups, max(1, min(_CHUNK_WGS // (groups * tiles), longest))

@@ -48,8 +48,10 @@ def sample_tokens(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     drawn, NaN counts as -inf, +inf shares all mass among its like; a row with nothing else gives 0.  A number at or
     above 1 in ``uniform`` draws the last kept token.
 
-    Weights are computed and summed in 64 bits, as integers, so the token depends on the row and its number alone: the
-    same in every launch, batch and graph.  V is at most 1,048,576 on the GPU."""
+    Weights are computed in 64 bits and summed as integers of 2^-min(50, 62 - bits of V) of the largest, so on the GPU the
+    token depends on the row, its settings and its number alone: the same in every launch, batch and graph.  A weight is off
+    by half of such a unit and 2e-13 of itself, so a number closer to a border than that may fall on its other side than in
+    exact arithmetic.  V is at most 1,048,576 on the GPU."""
     wrap = isinstance(logits, Tensor)
     x, u, out = _u(logits), _u(uniform), _u(out)
     shape, dev, dt = x.shape, x.device, x.dtype
