@@ -580,3 +580,97 @@ def test_pages_past_32_bits_are_a_value_error():
         with pytest.raises(ValueError, match="2\\^31"):
             m.chunk_attn(0, 16, 128, 128, 16, 16, s_blk, s_tok, s_head, 16, 1, 1, 64, 16, 16, 16, 128, 128, 1, 1, 2, 2, 128, 16,
                          1, 1, 256, 1.0, 0, 0, 0, 0)
+
+
+# ============================================================================ the cache as a whole
+@pytest.mark.parametrize("dev", DEVS)
+@pytest.mark.parametrize("seed", range(6))
+def test_cache_holds_every_sequence_through_random_changes(dev, seed):
+    """Sequences that grow token by token for all slots at once, or by several, fork, go back, end and are compacted: each
+    holds its own tokens, whatever the others do, and the pages' counts stay true."""
+    import random
+
+    rng = random.Random(seed)
+    slots, bs, most = 5, 4, 6
+    c = serving.PagedKVCache(2, rng.choice([13, 18, 30]), bs, 1, 8, slots, bs * most, dtype=torch.bfloat16,
+                             device=torch.device(dev, 0) if dev == "cuda" else torch.device(dev))
+    held = {}                                   # slot -> the values of its tokens
+    dev = c.k[0].device
+
+    def put(tokens):                            # [(slot, position, value)], in one call
+        seqs, pos, val = (torch.tensor(x, device=dev) for x in zip(*tokens))
+        rows = val.to(torch.bfloat16)[:, None, None].expand(-1, 1, 8).contiguous()
+        for k, v in zip(c.k, c.v):
+            serving.write_kv(rows, -rows, k, v, seqs, pos, c.block_table)
+
+    def step():                                 # every slot writes, as decode_step does
+        pos = [len(held[s]) if s in held else rng.randrange(bs * most) for s in range(slots)]
+        for s in held:
+            if pos[s] >= bs * most:
+                return
+            c.allocate(s, pos[s] + 1)
+        val = [rng.randrange(200) for _ in range(slots)]
+        c.check_step(torch.tensor(pos))
+        put(list(zip(range(slots), pos, val)))
+        for s in held:
+            held[s].append(val[s])
+            c.seq_lens[s] = len(held[s])
+
+    def extend():
+        s = rng.randrange(slots)
+        at, n = len(held.get(s, [])), rng.randint(1, 7)
+        if at + n <= bs * most:
+            c.allocate_all([s], [at + n])
+            c.check_writable(s, at)
+            val = [rng.randrange(200) for _ in range(n)]
+            put([(s, at + i, x) for i, x in enumerate(val)])
+            held[s] = held.get(s, []) + val
+            c.seq_lens[s] = len(held[s])
+
+    def fork():
+        free = [s for s in range(slots) if s not in held]
+        if held and free:
+            s, new = rng.choice(sorted(held)), rng.sample(free, rng.randint(1, len(free)))
+            n = rng.randint(0, len(held[s]))
+            c.fork(s, new, n)
+            held.update({x: held[s][:n] for x in new})
+
+    def truncate():
+        if held:
+            s = rng.choice(sorted(held))
+            n = rng.choice([rng.randint(0, len(held[s])), len(held[s]) // bs * bs])
+            c.truncate(s, n)
+            held[s] = held[s][:n]
+
+    def end():
+        if held and rng.random() < 0.5:
+            s = rng.choice(sorted(held))
+            c.free(s)
+            del held[s]
+
+    for _ in range(120):
+        before = (sorted(c._free), {s: list(h) for s, h in c._owned.items() if h}, list(c._holders))
+        op = rng.choice([step, step, extend, extend, fork, truncate, end, c.compact])
+        try:
+            op()
+        except RuntimeError:                    # out of pages
+            if op is not step:
+                assert before == (sorted(c._free), {s: list(h) for s, h in c._owned.items() if h}, list(c._holders))
+        holders = [0] * len(c._holders)
+        for h in c._owned.values():
+            for b in h:
+                holders[b] += 1
+        assert holders == c._holders and sorted(c._free) == [b for b, n in enumerate(holders) if not n]
+        assert c._shared == sum(n > 1 for n in holders)
+        table = c.block_table.tolist()
+        for s in range(slots):
+            own = c._owned.get(s, [])
+            assert table[s] == own + [-1] * (most - len(own))
+            n = len(held.get(s, []))
+            assert int(c.seq_lens[s]) == n and all(holders[b] == 1 for b in own[n // bs:])
+            if n:
+                j = torch.arange(n, device=dev)
+                at = c.block_table[s].long()[j // bs], j % bs
+                want = torch.tensor(held[s], dtype=torch.bfloat16, device=dev)
+                for k, v in zip(c.k, c.v):
+                    assert torch.equal(k[at][:, 0, 0], want) and torch.equal(v[at][:, 0, 7], -want)
