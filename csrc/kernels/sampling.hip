@@ -680,31 +680,42 @@ __device__ __forceinline__ void choose_from_start(const Args<T>& a, const Of& of
     __syncthreads();
   }
   // ---- kept mass per chunk, then the chunk, lane and element where the cumulative mass passes u * total
-  // A number below 2^-40 draws the first kept token of any weight above 0, one from 1 on the last, also where that is below
-  // the integers' unit: they are counted.
+  // The number 0 draws the first kept token of any weight above 0, one from 1 on the last, also where that is below the
+  // integers' unit: they are counted.  One between 0 and 2^-40 is compared in integers of 2^(1 - shift) of u * total; a weight
+  // above u * total, which passes it alone, counts as the next number.
   const float mp = of.m, uf = of.u;
-  const bool last_kept = uf >= 1.f, counted = last_kept || !(uf >= 9.094947e-13f);
+  const bool last_kept = uf >= 1.f, counted = last_kept || !(uf > 0.f), small = !counted && uf < 9.094947e-13f;
+  const u64 at_target = 1ull << (a.shift - 1);
+  double finer = 0.0;
   auto kept = [&](float x, int i) -> u64 {
     const unsigned ky = key_of(x);
     if (i >= V || ky < kmin || (ky == kmin && i > last_tie)) return 0;
     const double w = weight(r, x);
     if (!(w >= (double)mp || x == r.top || !(mp == mp))) return 0;
+    if (finer > 0.0) return (u64)fmin(w * finer + 0.5, (double)(at_target + 1));
     return counted ? (u64)(w > 0.0) : fixed(r, w);
   };
-  u64 mine = 0;
-  for (int c = wv; c < chunks; c += kWaves) {
-    float x[8];
-    const int i = c * kChunk + lane * 8;
-    load8(row, i, V, x);
-    u64 s = 0;
+  auto masses = [&]() {
+    u64 mine = 0;
+    for (int c = wv; c < chunks; c += kWaves) {
+      float x[8];
+      const int i = c * kChunk + lane * 8;
+      load8(row, i, V, x);
+      u64 s = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) s += kept(x[j], i + j);
-    s = wave_sum64(s);
-    if (lane == 0) part[c] = s;
-    mine += lane == 0 ? s : 0;
+      for (int j = 0; j < 8; ++j) s += kept(x[j], i + j);
+      s = wave_sum64(s);
+      if (lane == 0) part[c] = s;
+      mine += lane == 0 ? s : 0;
+    }
+    return group_sum<kWaves>(mine, red);
+  };
+  u64 total = masses(), want = counted ? 0 : (u64)fmin((double)uf * (double)total, 9.0e18);
+  if (small) {
+    finer = (double)at_target * r.unit / ((double)uf * (double)total);
+    total = masses();
+    want = at_target;
   }
-  const u64 total = group_sum<kWaves>(mine, red);
-  u64 want = counted ? 0 : (u64)fmin((double)uf * (double)total, 9.0e18);
   if (last_kept || want >= total) want = total - 1;
   group_find<kWaves, kMaxChunks / 64 / kWaves>(part, chunks, red, found, [&](u64) { return want; });
   if (wv == 0) {

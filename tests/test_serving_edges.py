@@ -674,3 +674,21 @@ def test_cache_holds_every_sequence_through_random_changes(dev, seed):
                 want = torch.tensor(held[s], dtype=torch.bfloat16, device=dev)
                 for k, v in zip(c.k, c.v):
                     assert torch.equal(k[at][:, 0, 0], want) and torch.equal(v[at][:, 0, 7], -want)
+
+
+@pytest.mark.parametrize("dev", DEVS)
+def test_numbers_near_zero_draw_by_mass(dev):
+    """Numbers below every unit of the masses: the first token whose cumulative mass exceeds them, not the first of all."""
+    x = torch.tensor([-float("inf"), -100.0, -70.0, -40.0, -32.0, 0.0, -float("inf"), 3e-9])
+    u = torch.tensor([0.0, 1e-45, 5e-44, 1e-42, 1e-30, 1e-17, 1e-13, 8e-13, 1e-11])
+    want = [1, 1, 2, 2, 3, 4, 5, 5, 5]
+    for V in (8, 700, 40000):
+        row = torch.full((V,), -float("inf"))
+        row[V - 8:] = x
+        rows, at = row.expand(len(u), V).to(dev), V - 8
+        assert serving.sample_tokens(rows, u.to(dev)).tolist() == [at + w for w in want]
+        assert serving.sample_tokens(rows, u.to(dev), top_k=4).tolist() == [at + max(w, 3) for w in want]
+        assert serving.sample_tokens(rows, u.to(dev), min_p=1e-15).tolist() == [at + max(w, 4) for w in want]
+        assert serving.sample_tokens(rows, u.to(dev), top_p=0.9).tolist() == [at + 5] * len(u)
+        flat = torch.zeros(len(u), V, device=dev)
+        assert serving.sample_tokens(flat, u.to(dev)).tolist() == [0] * len(u)
