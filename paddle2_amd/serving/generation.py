@@ -391,7 +391,10 @@ class LlamaGenerator:
         computed once and its pages are shared (PagedKVCache.fork).  ``chunk_size``: prompts run in pieces of that many
         tokens (prefill_chunks).  ``sampler``: "multinomial" draws with torch.multinomial (``sample_logits``), "fused" with
         ``sample_tokens``; the default is "multinomial", except where only ``sample_tokens`` can serve: ``min_p`` above 0, or
-        a list of one value per prompt for temperature, top_k, top_p or min_p."""
+        a list of one value per prompt for temperature, top_k, top_p or min_p.
+
+        Prompts replace what slots 0, 1, .. held, and every slot is free afterwards, also when a call fails half way; one that
+        is refused (ValueError: bad arguments, slots that share pages, other continuations' slots in use) changes nothing."""
         n_ret = int(num_return_sequences)
         assert n_ret >= 1 and len(prompts) * n_ret <= self.max_batch
         if n_ret > 1:
